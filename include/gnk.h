@@ -43,8 +43,9 @@ typedef enum gnk_status {
  * the meaning of an argument or return code (kernel changes behind an unchanged signature do not count); a binding compares
  * gnk_abi_version() of the loaded library with the GNK_ABI_VERSION it was written against and refuses a mismatch.
  *   1: round 1.   2: rounds 2-3 -- gnk_scaled_mm_ws / gnk_scaled_mm_t, the fused quantize pair, gnk_quantize_int8_noalloc, the MX and BitNet
- *      entry points added; gnk_set_debug_flags removed from the shipped library; gnk_set_gemm_variant accepts 5, 6, -2 and -3; gnk_set_tile_rescale added. */
-#define GNK_ABI_VERSION 2
+ *      entry points added; gnk_set_debug_flags removed from the shipped library; gnk_set_gemm_variant accepts 5, 6, -2 and -3; gnk_set_tile_rescale added.
+ *   3: the products grouped by expert and their quantizer (gnk_grouped_scaled_mm_rows / _depth, gnk_quantize_int8_grouped). */
+#define GNK_ABI_VERSION 3
 int gnk_abi_version(void);
 
 /* Message for the last non-zero status returned on this thread ("" if none). */
@@ -260,6 +261,47 @@ int64_t gnk_quantize_int8_noalloc_max_rows(void);
 int gnk_quantize_int8_noalloc(const void *x, int x_dtype, int64_t R, int64_t C, int64_t sxr, int64_t sxc,
                               int8_t *q, int64_t sqr, int64_t sqc, void *scale, float eps,
                               int sr, uint64_t seed, uint64_t offset, void *stream);
+
+/*
+ * Products grouped by expert (no reference counterpart: its Linears are dense).  Rows are sorted by group; group e holds rows
+ * ends[e - 1] .. ends[e] - 1 (ends[-1] = 0), `ends` being E int32 values ON THE DEVICE that do not decrease and do not exceed T -- nothing is
+ * read back, so the calls can be captured into a graph and replayed with other sizes.  (Ends that break this give unspecified results, but no
+ * access outside the operands: every end is clamped into [0, T].)  A group may be empty; rows behind the last end belong to no group.
+ *
+ * gnk_grouped_scaled_mm_rows:   C[t,n] = cast_out( (f32(sum_k A[t,k] * B[e,k,n]) * row_scale[t]) * col_scale[e,n] ),  e the group of row t; rows
+ *   of no group come out as zeros.  A (T, K) with strides (sat, sak); B (E, K, N) with strides (sbe, sbk, sbn); col_scale (E, N), or (E,) with
+ *   col_scale_is_scalar.  The forward product and the gradient of the input of a layer of experts.
+ * gnk_grouped_scaled_mm_depth:  C[e,m,n] = cast_out( (f32(sum_{t in e} A[m,t] * B[t,n]) * row_scale[e,m]) * col_scale[e,n] ); a group without rows
+ *   gives 0 * row_scale * col_scale.  A (M, T) with strides (sam, sat); B (T, N) with strides (sbt, sbn); row_scale (E, M), col_scale (E, N), or (E,).
+ *   The gradient of the experts' weights.
+ * Dtypes, accumulation and scales as in gnk_scaled_mm (order 0); C contiguous.  T < 2^31, E < 2^20, feature sizes up to 2^22.
+ * workspace: gnk_grouped_scaled_mm_*_workspace_bytes() bytes, 16-byte aligned.  0 when the kernels can read both operands where they lie (16-byte
+ * aligned bases and pitches, the contiguous extent a multiple of 16: rows form A K-contiguous and B K- or N-contiguous, depth form A M-contiguous and
+ * B N-contiguous); otherwise room for a padded copy of those that they cannot.  Overlapping calls need a workspace each.
+ */
+int64_t gnk_grouped_scaled_mm_rows_workspace_bytes(const void *A, const void *B, int64_t T, int64_t E, int64_t N, int64_t K, int64_t sat, int64_t sak,
+                                                   int64_t sbe, int64_t sbk, int64_t sbn);
+int gnk_grouped_scaled_mm_rows(const void *A, int a_dtype, const void *B, int b_dtype, void *C, int out_dtype, const void *row_scale,
+                               const void *col_scale, int scale_dtype, int col_scale_is_scalar, const int32_t *ends, int64_t T, int64_t E, int64_t N,
+                               int64_t K, int64_t sat, int64_t sak, int64_t sbe, int64_t sbk, int64_t sbn, void *workspace, int64_t workspace_bytes,
+                               void *stream);
+int64_t gnk_grouped_scaled_mm_depth_workspace_bytes(const void *A, const void *B, int64_t T, int64_t M, int64_t N, int64_t sam, int64_t sat, int64_t sbt,
+                                                    int64_t sbn);
+int gnk_grouped_scaled_mm_depth(const void *A, int a_dtype, const void *B, int b_dtype, void *C, int out_dtype, const void *row_scale,
+                                const void *col_scale, int scale_dtype, int col_scale_is_scalar, const int32_t *ends, int64_t T, int64_t E, int64_t M,
+                                int64_t N, int64_t sam, int64_t sat, int64_t sbt, int64_t sbn, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * gnk_quantize_int8 along the rows of every group (the quantization in front of gnk_grouped_scaled_mm_depth; with ends = N, 2 N, ... also the
+ * column-wise one of a stack of weights):  scale[e,c] = max_{t in e} |x[t,c]| * fl(1 / 127) (fp32, stored as x_dtype; 0 for a group without
+ * rows; eager torch's `amax / 127` on a device, within 1.5 fp32 steps of gnk_quantize_int8's quotient),
+ * q[t,c] = clip(round_half_even(x[t,c] / max(scale[e,c], eps)), -128, 127) with the unrounded scale, 0 for rows of no group.
+ * x (T, C) with strides (sxt, sxc); q (T, C) and scale (E, C) contiguous; `ends` as above.  sr, seed, offset as in gnk_quantize_int8 with
+ * e = t * C + c + offset.  workspace: gnk_quantize_int8_grouped_workspace_bytes() bytes, 4-byte aligned, need not be cleared.
+ */
+int64_t gnk_quantize_int8_grouped_workspace_bytes(int64_t T, int64_t E, int64_t C);
+int gnk_quantize_int8_grouped(const void *x, int x_dtype, const int32_t *ends, int64_t T, int64_t E, int64_t C, int64_t sxt, int64_t sxc, int8_t *q,
+                              void *scale, float eps, int sr, uint64_t seed, uint64_t offset, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

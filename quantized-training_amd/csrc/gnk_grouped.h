@@ -1,0 +1,286 @@
+// gnk_grouped.h -- MFMA products of 8-bit operands grouped by expert: rows sorted by group, group sizes known on the GPU only.
+//
+//   rows :  C[t, n]    = (f32(sum_k A[t, k] B[e(t), k, n]) * row_scale[t])    * col_scale[e(t), n]     (forward, gradient of the input)
+//   depth:  C[e, m, n] = (f32(sum_{t in e} A[m, t] B[t, n]) * row_scale[e, m]) * col_scale[e, n]       (gradients of the weights)
+//
+// Group e holds rows ends[e - 1] .. ends[e] - 1 (ends[-1] = 0); rows behind the last end belong to no group and come out as zeros.
+// The host knows neither the sizes nor the number of tiles: it launches the most workgroups the sizes could need (sum of ceil(T_e / BM)
+// <= T / BM + E, one more for the rows behind), every workgroup scans the ends with one wave-wide prefix sum (64 groups per step) to find
+// its tile, and the surplus leaves at once.  Every end is clamped into [previous end, T], so that no value of `ends` reaches outside
+// the operands.  A group's tile is then an ordinary tile of gnk_gemm_kernel.h / gnk_gemm_w4.h: same LDS images, fragments and epilogue.
+#pragma once
+#include "gnk_gemm_dispatch.h"
+
+struct GroupedParams {
+    GemmParams g;            // A, B, C, scales of the whole call; N; rows: K; depth: M
+    const int *ends;
+    int64_t T, E;
+    int64_t b_group;         // rows: bytes from one group's B to the next
+    int64_t ext_a, ext_b;    // depth: staged extents of A (>= M) and B (>= N); rows: ext_b (>= N) -- multiples of 16 for M/N-major operands
+    int out_bytes, scale_bytes;
+};
+
+typedef int (*gnk_grouped_launcher)(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st);
+#define GNK_DECLARE_GROUPED(NAME) int NAME(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st)
+GNK_DECLARE_GROUPED(gnk_grouped_i8);
+GNK_DECLARE_GROUPED(gnk_grouped_f8_00);
+GNK_DECLARE_GROUPED(gnk_grouped_f8_01);
+GNK_DECLARE_GROUPED(gnk_grouped_f8_10);
+GNK_DECLARE_GROUPED(gnk_grouped_f8_11);
+
+namespace gnk_grouped {
+
+using namespace gnk_gemm;
+
+// One tile: rows [lo, hi) of group e (e == E: the rows behind the last group), row tile tm of that group, column tile tn.
+struct Tile {
+    int e, tm, tn;
+    int64_t lo, hi;
+    bool work;               // false: a surplus workgroup
+};
+
+__device__ __forceinline__ int64_t clamp_end(int v, int64_t T) { return v < 0 ? 0 : (v < T ? v : T); }
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform64(int64_t v) {
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)((uint64_t)v >> 32));
+    return (int64_t)(((uint64_t)hi << 32) | lo);
+}
+
+// inclusive prefix sum over the wave
+__device__ __forceinline__ int wave_prefix(int v, int lane) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(v, d, 64);
+        v += lane >= d ? o : 0;
+    }
+    return v;
+}
+
+// Group and rows of lane `lane` in the 64-group step that starts at group g0: group E takes the rows behind the last end.
+__device__ __forceinline__ void lane_group(const int *ends, int64_t E, int64_t T, int64_t g0, int lane, int64_t &lo, int64_t &hi) {
+    const int64_t e = g0 + lane;
+    lo = e > 0 && e <= E ? clamp_end(ends[e - 1], T) : 0;
+    hi = e < E ? clamp_end(ends[e], T) : (e == E ? T : lo);
+    if (hi < lo) hi = lo;
+}
+
+// Every group (and the rows behind the last one) is cut into pieces of 1 << sh rows, numbered in group order.
+__device__ __forceinline__ int pieces_of(int64_t rows, int sh) { return (int)((rows + (1LL << sh) - 1) >> sh); }
+
+__device__ __forceinline__ int count_pieces(const int *ends, int64_t E, int64_t T, int lane, int sh) {
+    int total = 0;
+    for (int64_t g0 = 0; g0 <= E; g0 += 64) {
+        int64_t lo, hi;
+        lane_group(ends, E, T, g0, lane, lo, hi);
+        total += uniform(__shfl(wave_prefix(pieces_of(hi - lo, sh), lane), 63, 64));
+    }
+    return total;
+}
+
+// piece number `want`: its group e (E: rows of no group; -1: there are fewer pieces), its number within the group and the group's rows
+__device__ __forceinline__ void find_piece(const int *ends, int64_t E, int64_t T, int lane, int sh, int want, int &e, int &idx, int64_t &lo, int64_t &hi) {
+    int before = 0;
+    for (int64_t g0 = 0; g0 <= E; g0 += 64) {
+        int64_t l, h;
+        lane_group(ends, E, T, g0, lane, l, h);
+        const int n = pieces_of(h - l, sh), incl = wave_prefix(n, lane) + before;
+        const unsigned long long hit = __ballot(incl > want);
+        if (hit) {
+            const int src = __builtin_ctzll(hit);
+            e = (int)g0 + src;
+            idx = want - (__shfl(incl, src, 64) - __shfl(n, src, 64));
+            lo = __shfl((long long)l, src, 64);
+            hi = __shfl((long long)h, src, 64);
+            e = uniform(e); idx = uniform(idx); lo = uniform64(lo); hi = uniform64(hi);
+            return;
+        }
+        before = uniform(__shfl(incl, 63, 64));
+    }
+    e = -1; idx = 0; lo = hi = 0;
+}
+
+// rows form: tiles are counted on the device, then given to the XCDs in contiguous runs and walked in strips as tile_of_block does
+template <int BM>
+__device__ __forceinline__ Tile rows_tile(const GroupedParams &p, int grid_n, int lane) {
+    constexpr int SH = BM == 256 ? 8 : BM == 128 ? 7 : BM == 64 ? 6 : BM == 32 ? 5 : 4;
+    static_assert(BM == 1 << SH, "row tiles are powers of two");
+    Tile t;
+    const int grid_m = count_pieces(p.ends, p.E, p.T, lane, SH);
+    t.work = (int64_t)blockIdx.x < (int64_t)grid_m * grid_n;
+    if (!t.work) return t;
+    int tm, tn;
+    tile_of_block(grid_m, grid_n, tm, tn);
+    find_piece(p.ends, p.E, p.T, lane, SH, tm, t.e, t.tm, t.lo, t.hi);
+    t.tn = tn;
+    return t;
+}
+
+__device__ __forceinline__ Tile depth_tile(const GroupedParams &p, int grid_m, int grid_n) {
+    Tile t;
+    const int per = grid_m * grid_n;
+    int tm, tn;
+    // groups in order; within one, the strips of tile_of_block without its XCD split (a group's operands fit every L2 badly anyway)
+    const int wg = (int)blockIdx.x;
+    t.e = wg / per;
+    const int in = wg - t.e * per;
+    constexpr int GROUP_M = 4;
+    const int width = GROUP_M * grid_n, strip = in / width, first = strip * GROUP_M, gsz = min(grid_m - first, GROUP_M), r = in - strip * width;
+    tm = first + r % gsz;
+    tn = r / gsz;
+    t.tm = tm; t.tn = tn;
+    t.lo = t.e > 0 ? clamp_end(p.ends[t.e - 1], p.T) : 0;
+    t.hi = clamp_end(p.ends[t.e], p.T);
+    if (t.hi < t.lo) t.hi = t.lo;
+    t.work = true;
+    return t;
+}
+
+// The ordinary product of one tile: pointers and extents of its group.  ext_a / ext_b: staged extents (rows of A, columns of B).
+template <bool DEPTH>
+__device__ __forceinline__ GemmParams tile_params(const GroupedParams &p, const Tile &t, int64_t &ext_a, int64_t &ext_b) {
+    GemmParams g = p.g;
+    const int64_t rows = t.hi - t.lo;
+    if constexpr (DEPTH) {
+        g.K = rows;
+        g.A += t.lo * g.lda;
+        g.B += t.lo * g.ldb;
+        g.C = (char *)g.C + (int64_t)t.e * g.M * g.N * p.out_bytes;
+        g.s0 = (const char *)g.s0 + (int64_t)t.e * g.M * p.scale_bytes;
+        ext_a = p.ext_a;
+    } else {
+        g.M = rows;
+        g.A += t.lo * g.lda;
+        g.B += (int64_t)t.e * p.b_group;
+        g.C = (char *)g.C + t.lo * g.N * p.out_bytes;
+        g.s0 = (const char *)g.s0 + t.lo * p.scale_bytes;
+        ext_a = rows;
+    }
+    g.s1 = (const char *)g.s1 + (g.col_scalar ? (int64_t)t.e : (int64_t)t.e * g.N) * p.scale_bytes;
+    ext_b = p.ext_b;
+    return g;
+}
+
+// zeros into rows [m0, min(m0 + BM, rows)) x columns [n0, min(n0 + BN, N)) of a row-major (rows, N) output
+template <int BM, int BN, int NT>
+__device__ __forceinline__ void zero_tile(char *C, int64_t rows, int64_t N, int64_t m0, int64_t n0, int out_bytes) {
+    const int64_t m1 = m0 + BM < rows ? m0 + BM : rows, n1 = n0 + BN < N ? n0 + BN : N;
+    const int64_t halves = (n1 - n0) * (out_bytes >> 1);          // outputs are 2 or 4 bytes wide
+    for (int64_t m = m0; m < m1; ++m) {
+        unsigned short *dst = (unsigned short *)(C + (m * N + n0) * out_bytes);
+        for (int64_t i = threadIdx.x; i < halves; i += NT) dst[i] = 0;
+    }
+}
+
+// ------------------------------------------------------------------------------ two-buffer kernel (any K, any group size)
+// The loop of gemm_kernel (row / column epilogue) on one group's tile.  128 x 128 over four waves: 64 KiB of LDS and at most 256
+// registers, two workgroups per CU.
+template <class Cfg, bool DEPTH>
+__global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cfg::NT == 256 ? 2 : 1))) two_buffer_kernel(const GroupedParams gp) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int MT = Cfg::MT, NTL = Cfg::NTL;
+    typedef typename AccT<Cfg::OP>::type acc_t;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
+    if (!tile.work) return;
+    const int64_t m0 = (int64_t)tile.tm * Cfg::BM, n0 = (int64_t)tile.tn * Cfg::BN;
+    if (!DEPTH && tile.e == gp.E) {      // rows of no group
+        zero_tile<Cfg::BM, Cfg::BN, Cfg::NT>((char *)gp.g.C + tile.lo * gp.g.N * gp.out_bytes, tile.hi - tile.lo, gp.g.N, m0, n0, gp.out_bytes);
+        return;
+    }
+    int64_t ext_a, ext_b;
+    const GemmParams p = tile_params<DEPTH>(gp, tile, ext_a, ext_b);
+
+    char *const As0 = smem;
+    char *const Bs0 = smem + 2 * Cfg::A_BYTES;
+    ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, EPI_ROWCOL> spf;
+    spf.issue(p, m0, n0);
+    Stager<Cfg::A_KMAJOR, Cfg::BM, Cfg::NW> sa;
+    Stager<Cfg::B_KMAJOR, Cfg::BN, Cfg::NW> sb;
+    sa.init(p.A, p.lda, m0, ext_a, wave, lane);
+    sb.init(p.B, p.ldb, n0, ext_b, wave, lane);
+    acc_t acc[MT][NTL];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) acc[i][j] = (acc_t){0, 0, 0, 0};
+
+    const int nk = (int)((p.K + GNK_BK - 1) / GNK_BK), ktail = (int)(p.K % GNK_BK);
+    if (nk > 0) {
+        if (nk == 1 && ktail) {
+            sa.issue_tail(As0, p.lda, m0, ext_a, wave, lane, ktail);
+            sb.issue_tail(Bs0, p.ldb, n0, ext_b, wave, lane, ktail);
+        } else {
+            sa.issue(As0, wave);
+            sb.issue(Bs0, wave);
+        }
+    }
+    for (int t = 0; t < nk; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const int cur = t & 1;
+        if (ktail && t + 1 == nk) {
+            zero_tail<Cfg::A_KMAJOR, Cfg::BM, Cfg::NT>(As0 + cur * Cfg::A_BYTES, ktail);
+            zero_tail<Cfg::B_KMAJOR, Cfg::BN, Cfg::NT>(Bs0 + cur * Cfg::B_BYTES, ktail);
+            __syncthreads();
+        }
+        if (t + 1 < nk) {
+            if (ktail && t + 2 == nk) {
+                sa.issue_tail(As0 + (cur ^ 1) * Cfg::A_BYTES, p.lda, m0, ext_a, wave, lane, ktail);
+                sb.issue_tail(Bs0 + (cur ^ 1) * Cfg::B_BYTES, p.ldb, n0, ext_b, wave, lane, ktail);
+            } else {
+                sa.issue(As0 + (cur ^ 1) * Cfg::A_BYTES, wave);
+                sb.issue(Bs0 + (cur ^ 1) * Cfg::B_BYTES, wave);
+            }
+        }
+        compute_step<Cfg, false>(As0 + cur * Cfg::A_BYTES, Bs0 + cur * Cfg::B_BYTES, acc, wm, wn, lane);
+    }
+    spf.park(p, smem + Cfg::LDS_BYTES);
+    __syncthreads();
+    run_epilogue<Cfg>(p, acc, nullptr, smem, wave, lane, m0 + wm * Cfg::WTM, n0 + wn * Cfg::WTN, (const float *)(smem + Cfg::LDS_BYTES),
+                      wm * Cfg::WTM, wn * Cfg::WTN);
+}
+
+// most row tiles the groups can need: every group wastes less than one tile, and the rows behind the last group are one group more
+static inline int64_t max_row_tiles(int64_t T, int64_t E, int64_t bm) {
+    const int64_t by_rows = T / bm + E + 1;
+    return by_rows < T ? by_rows : T;       // no tile is empty
+}
+
+template <class Kernel> static int reserve_lds(Kernel k, int bytes, std::atomic<bool> (&done)[64]) {
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return gnk_fail(GNK_ERR_LAUNCH, "grouped mm: no current HIP device");
+    if (!done[dev].load(std::memory_order_acquire)) {      // opt in to > 64 KiB of dynamic LDS once per device and kernel
+        if (hipFuncSetAttribute((const void *)k, hipFuncAttributeMaxDynamicSharedMemorySize, bytes) != hipSuccess)
+            return gnk_fail(GNK_ERR_LAUNCH, "grouped mm: cannot reserve %d bytes of LDS", bytes);
+        done[dev].store(true, std::memory_order_release);
+    }
+    return GNK_OK;
+}
+
+template <class Cfg, bool DEPTH> int launch_two_buffer(const GroupedParams &p0, hipStream_t st) {
+    constexpr int LDS_TOTAL = Cfg::LDS_BYTES + ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, EPI_ROWCOL>::BYTES;
+    GroupedParams p = p0;
+    p.g.grid_n = (int)((p.g.N + Cfg::BN - 1) / Cfg::BN);
+    p.g.grid_m = DEPTH ? (int)((p.g.M + Cfg::BM - 1) / Cfg::BM) : 0;
+    const int64_t blocks = (DEPTH ? p.E * p.g.grid_m : max_row_tiles(p.T, p.E, Cfg::BM)) * p.g.grid_n;
+    if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "grouped mm: too many tiles");
+    static std::atomic<bool> attr_set[64];
+    const int rc = reserve_lds(two_buffer_kernel<Cfg, DEPTH>, LDS_TOTAL, attr_set);
+    if (rc) return rc;
+    hipLaunchKernelGGL((two_buffer_kernel<Cfg, DEPTH>), dim3((unsigned)blocks), dim3(Cfg::NT), LDS_TOTAL, st, p);
+    return gnk_check_launch("grouped mm");
+}
+
+template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st) {
+    if (depth) return launch_two_buffer<GemmCfg<128, 128, 2, 2, false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
+    if (b_kmajor) return launch_two_buffer<GemmCfg<128, 128, 2, 2, true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
+    return launch_two_buffer<GemmCfg<128, 128, 2, 2, true, false, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
+}
+
+}  // namespace gnk_grouped
+
+#define GNK_DEFINE_GROUPED(NAME, OP, FA, FB) \
+    int NAME(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st) { return gnk_grouped::launch<OP, FA, FB>(depth, b_kmajor, p, st); }

@@ -192,6 +192,75 @@ std::tuple<at::Tensor, at::Tensor> quantize_int8_colwise_given(const at::Tensor 
     return {q, scale};
 }
 
+// ---------------------------------------------------------------------------------------------- products grouped by expert (gn_kernels/grouped.py)
+void grouped_args(const at::Tensor &A, const at::Tensor &B, const at::Tensor &sA, const at::Tensor &sB, const at::Tensor &ends, const char *op) {
+    TORCH_CHECK(is_float(sA.scalar_type()) && sB.scalar_type() == sA.scalar_type(), "gn_kernels::", op, ": scale dtypes ", sA.scalar_type(), ", ",
+                sB.scalar_type(), " are not one of bf16 / fp16 / fp32");
+    TORCH_CHECK(sA.is_contiguous() && sB.is_contiguous(), "gn_kernels::", op, ": scales must be contiguous");
+    TORCH_CHECK(ends.scalar_type() == at::kInt && ends.dim() == 1 && ends.is_contiguous(), "gn_kernels::", op, ": offs must be a contiguous 1-D int32 tensor");
+    TORCH_CHECK(B.device() == A.device() && sA.device() == A.device() && sB.device() == A.device() && ends.device() == A.device(), "gn_kernels::", op,
+                ": all tensors must be on one device");
+}
+
+at::Tensor workspace_for(const at::Tensor &A, int64_t bytes) { return bytes > 0 ? at::empty({bytes}, A.options().dtype(at::kByte)) : at::Tensor(); }
+
+at::Tensor grouped_scaled_mm(const at::Tensor &A, const at::Tensor &B, const at::Tensor &sA, const at::Tensor &sB, const at::Tensor &ends) {
+    const char *op = "grouped_scaled_mm";
+    grouped_args(A, B, sA, sB, ends, op);
+    TORCH_CHECK(A.dim() == 2 && B.dim() == 3 && B.size(1) == A.size(1) && ends.size(0) == B.size(0) && sA.numel() == A.size(0) &&
+                (sB.numel() == B.size(0) * B.size(2) || sB.numel() == B.size(0)), "gn_kernels::", op, ": shapes ", A.sizes(), ", ", B.sizes(), ", ", sA.sizes(),
+                ", ", sB.sizes(), ", ", ends.sizes(), " do not go together");
+    const int64_t T = A.size(0), K = A.size(1), E = B.size(0), N = B.size(2);
+    at::Tensor C = at::empty({T, N}, sA.options());
+    const int ad = dtype_code(A.scalar_type(), op), bd = dtype_code(B.scalar_type(), op), sd = dtype_code(sA.scalar_type(), op);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(A.device());
+    const int64_t nws = gnk_grouped_scaled_mm_rows_workspace_bytes(A.data_ptr(), B.data_ptr(), T, E, N, K, A.stride(0), A.stride(1), B.stride(0), B.stride(1),
+                                                                   B.stride(2));
+    const at::Tensor ws = workspace_for(A, nws);
+    check(gnk_grouped_scaled_mm_rows(A.data_ptr(), ad, B.data_ptr(), bd, C.data_ptr(), sd, sA.data_ptr(), sB.data_ptr(), sd, sB.size(2) == 1 && N != 1,
+                                     (const int32_t *)ends.data_ptr(), T, E, N, K, A.stride(0), A.stride(1), B.stride(0), B.stride(1), B.stride(2),
+                                     nws > 0 ? ws.data_ptr() : nullptr, nws, stream_of(A)),
+          op);
+    return C;
+}
+
+at::Tensor grouped_scaled_mm_depth(const at::Tensor &A, const at::Tensor &B, const at::Tensor &sA, const at::Tensor &sB, const at::Tensor &ends) {
+    const char *op = "grouped_scaled_mm_depth";
+    grouped_args(A, B, sA, sB, ends, op);
+    const int64_t E = ends.size(0), M = A.size(0), T = A.size(1), N = B.size(1);
+    TORCH_CHECK(A.dim() == 2 && B.dim() == 2 && B.size(0) == T && sA.numel() == E * M && (sB.numel() == E * N || sB.numel() == E), "gn_kernels::", op,
+                ": shapes ", A.sizes(), ", ", B.sizes(), ", ", sA.sizes(), ", ", sB.sizes(), ", ", ends.sizes(), " do not go together");
+    at::Tensor C = at::empty({E, M, N}, sA.options());
+    const int ad = dtype_code(A.scalar_type(), op), bd = dtype_code(B.scalar_type(), op), sd = dtype_code(sA.scalar_type(), op);
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(A.device());
+    const int64_t nws =
+        gnk_grouped_scaled_mm_depth_workspace_bytes(A.data_ptr(), B.data_ptr(), T, M, N, A.stride(0), A.stride(1), B.stride(0), B.stride(1));
+    const at::Tensor ws = workspace_for(A, nws);
+    check(gnk_grouped_scaled_mm_depth(A.data_ptr(), ad, B.data_ptr(), bd, C.data_ptr(), sd, sA.data_ptr(), sB.data_ptr(), sd, sB.size(2) == 1 && N != 1,
+                                      (const int32_t *)ends.data_ptr(), T, E, M, N, A.stride(0), A.stride(1), B.stride(0), B.stride(1),
+                                      nws > 0 ? ws.data_ptr() : nullptr, nws, stream_of(A)),
+          op);
+    return C;
+}
+
+std::tuple<at::Tensor, at::Tensor> quantize_int8_grouped(const at::Tensor &x, const at::Tensor &ends, bool sr, double eps, const c10::optional<at::Tensor> &rng) {
+    const char *op = "quantize_int8_grouped";
+    TORCH_CHECK(is_float(x.scalar_type()) && x.dim() == 2, "gn_kernels::", op, ": unsupported input (shape ", x.sizes(), ", dtype ", x.scalar_type(), ")");
+    TORCH_CHECK(ends.scalar_type() == at::kInt && ends.dim() == 1 && ends.is_contiguous() && ends.device() == x.device(), "gn_kernels::", op,
+                ": offs must be a contiguous 1-D int32 tensor on x's device");
+    const int64_t T = x.size(0), C = x.size(1), E = ends.size(0);
+    at::Tensor q = at::empty({T, C}, x.options().dtype(at::kChar)), scale = at::empty({E, 1, C}, x.options());
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    const int64_t nws = gnk_quantize_int8_grouped_workspace_bytes(T, E, C);
+    const at::Tensor ws = workspace_for(x, nws);
+    uint64_t seed;
+    sr_args(sr, rng, seed);
+    check(gnk_quantize_int8_grouped(x.data_ptr(), dtype_code(x.scalar_type(), op), (const int32_t *)ends.data_ptr(), T, E, C, x.stride(0), x.stride(1),
+                                    (int8_t *)q.data_ptr(), scale.data_ptr(), (float)eps, sr, seed, 0, nws > 0 ? ws.data_ptr() : nullptr, nws, stream_of(x)),
+          op);
+    return {q, scale};
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(gn_kernels, CUDA, m) {
@@ -202,4 +271,7 @@ TORCH_LIBRARY_IMPL(gn_kernels, CUDA, m) {
     m.impl("quantize_int8", &quantize_int8);
     m.impl("quantize_int8_rowwise_colmax", &quantize_int8_rowwise_colmax);
     m.impl("quantize_int8_colwise_given", &quantize_int8_colwise_given);
+    m.impl("grouped_scaled_mm", &grouped_scaled_mm);
+    m.impl("grouped_scaled_mm_depth", &grouped_scaled_mm_depth);
+    m.impl("quantize_int8_grouped", &quantize_int8_grouped);
 }

@@ -5,6 +5,7 @@ NotImplementedError when called."""
 from . import _cabi
 from . import bitnet  # noqa: F401  (registers the bitnet_* device ops)
 from .fp8 import fp8_mm, scaled_fp8_mm
+from .grouped import grouped_scaled_mm, quantize_int8_grouped
 from .mm import _triton_mm, int8_mm, scaled_mm, scaled_mm_t
 from .mx import dequantize_mxfp4, mxfp4_mm, mxfp8_mm, pack_block_scales_nv, quantize_mx
 from .quantize import quantize_int8
@@ -42,7 +43,9 @@ __all__ = [
     "int8_mm",
     "scaled_mm",
     "scaled_mm_t",
+    "grouped_scaled_mm",
     "quantize_int8",
+    "quantize_int8_grouped",
     "quantize_mx",
     "quantize_nvfp4",
     "quantize_nvfp4_triton",

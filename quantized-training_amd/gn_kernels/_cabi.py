@@ -11,7 +11,7 @@ import torch
 
 # GNK_LIBRARY: tuning only (an A/B build of the same sources, e.g. `make ABLATE=1 OUT=...`); the shipped library is the default
 _LIB_PATH = Path(os.environ.get("GNK_LIBRARY") or Path(__file__).resolve().parent / "libgnk_hip.so")
-ABI_VERSION = 2   # include/gnk.h GNK_ABI_VERSION
+ABI_VERSION = 3   # include/gnk.h GNK_ABI_VERSION
 
 BF16, F16, F32, I8, E4M3, E5M2, I32 = range(7)
 DTYPE_CODE = {
@@ -30,7 +30,8 @@ _lib = None
 # Same kernels, same C ABI; only the per-call host path changes (dispatcher -> C++ -> C ABI instead of dispatcher -> Python -> ctypes).
 # GNK_NO_TORCH_SHIM=1 keeps the Python implementations (A/B timing of the host path, and the tests' second leg).
 _SHIM_PATH = Path(__file__).resolve().parent / "libgnk_torch_ops.so"
-_SHIM_OPS = ("int8_mm", "scaled_mm", "scaled_mm_t", "tile_scaled_mm", "quantize_int8", "quantize_int8_rowwise_colmax", "quantize_int8_colwise_given")
+_SHIM_OPS = ("int8_mm", "scaled_mm", "scaled_mm_t", "tile_scaled_mm", "quantize_int8", "quantize_int8_rowwise_colmax", "quantize_int8_colwise_given",
+             "grouped_scaled_mm", "grouped_scaled_mm_depth", "quantize_int8_grouped")
 _shim_loaded = None
 
 
@@ -105,6 +106,15 @@ def load() -> ctypes.CDLL:
     L.gnk_scaled_mm_workspace_bytes.restype = i64
     L.gnk_tile_scaled_mm.argtypes = [vp, ci, vp, ci, vp, ci, vp, vp, ci] + [i64] * 14 + [vp]
     L.gnk_fp8_mm.argtypes = [vp, ci, vp, ci, vp, ci] + [i64] * 7 + [vp]
+    L.gnk_grouped_scaled_mm_rows_workspace_bytes.argtypes = [vp, vp] + [i64] * 9
+    L.gnk_grouped_scaled_mm_rows_workspace_bytes.restype = i64
+    L.gnk_grouped_scaled_mm_rows.argtypes = [vp, ci, vp, ci, vp, ci, vp, vp, ci, ci, vp] + [i64] * 9 + [vp, i64, vp]
+    L.gnk_grouped_scaled_mm_depth_workspace_bytes.argtypes = [vp, vp] + [i64] * 7
+    L.gnk_grouped_scaled_mm_depth_workspace_bytes.restype = i64
+    L.gnk_grouped_scaled_mm_depth.argtypes = [vp, ci, vp, ci, vp, ci, vp, vp, ci, ci, vp] + [i64] * 8 + [vp, i64, vp]
+    L.gnk_quantize_int8_grouped_workspace_bytes.argtypes = [i64] * 3
+    L.gnk_quantize_int8_grouped_workspace_bytes.restype = i64
+    L.gnk_quantize_int8_grouped.argtypes = [vp, ci, vp] + [i64] * 5 + [vp, vp, f32, ci, u64, u64, vp, i64, vp]
     if L.gnk_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libgnk_hip.so ABI {L.gnk_abi_version()} != expected {ABI_VERSION}; rebuild it")
     _lib = L
