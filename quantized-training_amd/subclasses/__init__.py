@@ -7,7 +7,7 @@ path (no INT4 MFMA on CDNA4); its names import and raise when used.
 """
 from .bitnet import BitNetTrainingLinearWeight, convert_bitnet
 from .int8 import Int8LinearWeight, Int8QTConfig, convert_int8_quantized_training, quantize_int8
-from .mixed_precision import MixedPrecisionConfig, MixedPrecisionLinearWeight, convert_mixed_precision
+from .mixed_precision import MixedPrecisionConfig, MixedPrecisionLinearWeight, convert_mixed_precision, convert_mixed_precision_experts
 
 
 def _out_of_scope(name: str):
@@ -32,5 +32,6 @@ __all__ = [
     "MixedPrecisionConfig",
     "MixedPrecisionLinearWeight",
     "convert_mixed_precision",
+    "convert_mixed_precision_experts",
     "quantize_int8",
 ]

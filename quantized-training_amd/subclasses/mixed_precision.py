@@ -24,8 +24,8 @@ import torch.nn.functional as F
 import torch.utils._pytree as pytree
 from torch import Tensor, nn
 
+from gn_kernels import grouped_scaled_mm, quantize_int8_grouped, scaled_mm, scaled_mm_t
 from gn_kernels import quantize as _qop
-from gn_kernels import scaled_mm, scaled_mm_t
 
 from .int8 import quantize_int8
 
@@ -102,6 +102,8 @@ class MixedPrecisionLinearWeight(Tensor):
     def __torch_function__(cls, func, types, args=(), kwargs=None):
         if func is F.linear:
             return _Int8MixedPrecisionLinear.apply(*args, **(kwargs or {}))
+        if func in _GROUPED_MM:
+            return _grouped_mm(*args, **(kwargs or {}))
         with torch._C.DisableTorchFunctionSubclass():
             return func(*args, **(kwargs or {}))
 
@@ -119,7 +121,7 @@ class MixedPrecisionLinearWeight(Tensor):
         out = func(*pytree.tree_map_only(cls, unwrap, args), **pytree.tree_map_only(cls, unwrap, kwargs or {}))
         if func is aten.copy_.default:
             return args[0]                       # in-place: hand back the original wrapper
-        if func in _REWRAP_OPS:
+        if func in _REWRAP_OPS or (func is aten.transpose.int and args[0].ndim == 3):     # a stack of experts' weights, seen as (E, K, N)
             return pytree.tree_map_only(Tensor, lambda t: cls(t, seen[0]), out)
         return out
 
@@ -324,6 +326,73 @@ class _Int8MixedPrecisionLinear(torch.autograd.Function):
             grad_bias = go2d.sum(0)
 
         return grad_input, grad_weight, grad_bias
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# A stack of experts' weights: `F.grouped_mm(x, weight.transpose(-2, -1), offs=offs)` on a MixedPrecisionLinearWeight (E, N, K).  No
+# counterpart in the reference (its models are dense); the arithmetic per expert is that of the Linear above.  Rows are sorted by expert
+# and `offs` stays on the device, so every operand is quantized along its contraction by one kernel over all groups:
+#   forward   x per row, w per (e, n)            rows form, (T, K) x (E, K, N)
+#   dX        dY per row, w per (e, k)           rows form, (T, N) x (E, N, K); the columns of one expert are a "group" of N rows
+#   dW        dY and x per (group, column)       the contraction runs over each group's rows, (N, T) x (T, K) -> (E, N, K)
+# Rows behind the last group are zeros in y and dX and count for nothing in dW.
+_GROUPED_MM = {f for f in (getattr(F, "grouped_mm", None), getattr(torch, "_grouped_mm", None)) if f is not None}
+
+
+class _Int8MixedPrecisionGroupedMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, input: Tensor, weight: MixedPrecisionLinearWeight, offs: Tensor):
+        cfg, w = weight.config, weight._data
+        E, K, N = w.shape
+        wt = w.transpose(1, 2)                                    # (E, N, K), contiguous in the usual call
+        xq, xs = quantize_int8(input, cfg.stochastic_rounding, dim=1)
+        wq, ws = quantize_int8(wt.reshape(E * N, K), cfg.stochastic_rounding, dim=1)
+        ctx.save_for_backward(input, w, offs)
+        ctx.config = cfg
+        return grouped_scaled_mm(xq, wq.view(E, N, K).transpose(1, 2), xs, ws.view(E, 1, N), offs)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        input, w, offs = ctx.saved_tensors
+        sr = ctx.config.stochastic_rounding
+        E, K, N = w.shape
+        grad_input = grad_weight = None
+        if ctx.needs_input_grad[0]:
+            gq, gs = quantize_int8(grad_output, sr, dim=1)
+            ends = torch.arange(N, E * N + 1, max(N, 1), dtype=torch.int32, device=w.device) if N else offs.new_zeros(E)
+            wq, ws = quantize_int8_grouped(w.transpose(1, 2).reshape(E * N, K), ends, sr)
+            grad_input = grouped_scaled_mm(gq, wq.view(E, N, K), gs, ws, offs)
+        if ctx.needs_input_grad[1]:
+            xq, xs = quantize_int8_grouped(input, offs, sr)
+            gq, gs = quantize_int8_grouped(grad_output, offs, sr)
+            grad_weight = grouped_scaled_mm(gq.T, xq, gs.view(E, N, 1), xs, offs).transpose(1, 2)      # stored (E, N, K), as the weight is
+        return grad_input, grad_weight, None
+
+
+def _grouped_mm(mat_a: Tensor, mat_b: Tensor, *, offs: Tensor | None = None, bias: Tensor | None = None, out_dtype: torch.dtype | None = None) -> Tensor:
+    """`torch.nn.functional.grouped_mm(x (T, K), weight (E, K, N), offs=...)` whose three products run in INT8."""
+    if not isinstance(mat_b, MixedPrecisionLinearWeight) or isinstance(mat_a, MixedPrecisionLinearWeight):
+        raise NotImplementedError("grouped_mm: the mixed-precision weight is the second operand")
+    cfg = mat_b.config
+    if not (cfg.output and cfg.grad_input and cfg.grad_weight and cfg.dtype == "int8"):
+        raise NotImplementedError(f"grouped_mm runs all three products in INT8, {cfg} asks for something else")
+    if mat_a.ndim != 2 or mat_b.ndim != 3 or offs is None or bias is not None or out_dtype not in (None, mat_a.dtype):
+        raise NotImplementedError("grouped_mm on a mixed-precision weight takes x (T, K), weight (E, K, N) and offs; no bias, no other output type")
+    if mat_a.shape[1] != mat_b.shape[1] or offs.shape != (mat_b.shape[0],) or mat_a.dtype != mat_b.dtype:
+        raise RuntimeError(f"grouped_mm: x {tuple(mat_a.shape)} {mat_a.dtype}, weight {tuple(mat_b.shape)} {mat_b.dtype} and offs {tuple(offs.shape)} do not go together")
+    return _Int8MixedPrecisionGroupedMM.apply(mat_a, mat_b, offs)
+
+
+def convert_mixed_precision_experts(module: nn.Module, *, config: MixedPrecisionConfig = MixedPrecisionConfig()):
+    """Wrap every stack of experts' weights under `module` -- a floating 3-D nn.Parameter (E, N, K) outside convolutions -- in a
+    MixedPrecisionLinearWeight (in place).  The module has to multiply with `F.grouped_mm(x, weight.transpose(-2, -1), offs=offs)`."""
+    for m in module.modules():
+        if isinstance(m, nn.modules.conv._ConvNd):
+            continue
+        for name, p in list(m.named_parameters(recurse=False)):
+            if p.ndim == 3 and p.is_floating_point() and not isinstance(p, MixedPrecisionLinearWeight):
+                setattr(m, name, nn.Parameter(MixedPrecisionLinearWeight(p.detach(), config=config), requires_grad=p.requires_grad))
+    return module
 
 
 def convert_mixed_precision(module: nn.Module, *, config: MixedPrecisionConfig = MixedPrecisionConfig()):
