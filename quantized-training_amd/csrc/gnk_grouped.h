@@ -9,7 +9,11 @@
 // its tile, and the surplus leaves at once.  Every end is clamped into [previous end, T], so that no value of `ends` reaches outside
 // the operands.  A group's tile is then an ordinary tile of gnk_gemm_kernel.h / gnk_gemm_w4.h: same LDS images, fragments and epilogue.
 #pragma once
+#include <math.h>
+
 #include "gnk_gemm_dispatch.h"
+#include "gnk_gemm_w4.h"
+#include "gnk_gemm_w4_more_asm.inc"
 
 struct GroupedParams {
     GemmParams g;            // A, B, C, scales of the whole call; N; rows: K; depth: M
@@ -243,6 +247,85 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cf
                       wm * Cfg::WTM, wn * Cfg::WTN);
 }
 
+// ------------------------------------------------------------------------------ 256 x 256, one wave per SIMD (gnk_gemm_w4.h)
+// rows: K % 256 == 0, the dense loop on the group's tile.  depth: the contraction ends where the group does, so the loop reads through buffer
+// descriptors that end there too: k-rows past the end are out of range and arrive in LDS as zeros, which add nothing in int8 and fp8; the loop
+// runs over ceil(T_e / 256) * 256 of them (a group without rows: once over zeros).  Host-checked: T * pitch < 2^32 (the descriptors' sizes).
+template <class Cfg, bool DEPTH>
+__global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef typename W4Select<Cfg, Cfg::OP>::type K;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n) : rows_tile<256>(gp, gp.g.grid_n, lane);
+    if (!tile.work) return;
+    const int64_t m0 = (int64_t)tile.tm * 256, n0 = (int64_t)tile.tn * 256;
+    if (!DEPTH && tile.e == gp.E) {
+        zero_tile<256, 256, 256>((char *)gp.g.C + tile.lo * gp.g.N * gp.out_bytes, tile.hi - tile.lo, gp.g.N, m0, n0, gp.out_bytes);
+        return;
+    }
+    int64_t ext_a, ext_b;
+    const GemmParams p = tile_params<DEPTH>(gp, tile, ext_a, ext_b);
+
+    const int t = threadIdx.x;
+    const int64_t mi = m0 + t < p.M - 1 ? m0 + t : p.M - 1;
+    const int64_t ni = p.col_scalar ? 0 : (n0 + t < p.N - 1 ? n0 + t : p.N - 1);
+    const unsigned raw_r = gnk_load_raw_rt(p.s0, p.scale_dtype, mi), raw_c = gnk_load_raw_rt(p.s1, p.scale_dtype, ni);
+
+    StagerW4<Cfg::A_KMAJOR> sa;
+    StagerW4<Cfg::B_KMAJOR> sb;
+    sa.init(p.A, p.lda, m0, ext_a, wave, lane);
+    sb.init(p.B, p.ldb, n0, ext_b, wave, lane);
+
+    const unsigned lds0 = (unsigned)(uintptr_t)(GNK_LDS char *)smem;
+    const unsigned va = lds0 + K::frag0(Cfg::A_KMAJOR, wm * 128, lane);
+    const unsigned vb = lds0 + 4 * Cfg::OPER_BYTES + K::frag0(Cfg::B_KMAJOR, wn * 128, lane);
+    const unsigned alo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)sa.base), ahi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)sa.base >> 32));
+    const unsigned blo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)sb.base), bhi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)sb.base >> 32));
+    const unsigned stepa = __builtin_amdgcn_readfirstlane((unsigned)sa.step), stepb = __builtin_amdgcn_readfirstlane((unsigned)sb.step);
+    const unsigned ldsw = __builtin_amdgcn_readfirstlane(lds0 + wave * 1024);
+#define GNK_GROUPED_W4_IN                                                                                                             \
+                 [alo] "s"(alo), [ahi] "s"(ahi), [blo] "s"(blo), [bhi] "s"(bhi), [stepa] "s"(stepa), [stepb] "s"(stepb),              \
+                 [lds] "s"(ldsw), [nit] "s"(nit), [va] "v"(va), [vb] "v"(vb),                                                         \
+                 [oa0] "v"(sa.off[0]), [oa1] "v"(sa.off[1]), [oa2] "v"(sa.off[2]), [oa3] "v"(sa.off[3]),                              \
+                 [ob0] "v"(sb.off[0]), [ob1] "v"(sb.off[1]), [ob2] "v"(sb.off[2]), [ob3] "v"(sb.off[3]),                              \
+                 [fa] "i"(Cfg::FA), [fb] "i"(Cfg::FB)
+    if constexpr (DEPTH) {
+        const int nit = uniform(p.K > 0 ? (int)((p.K + 255) >> 8) : 1);
+        // the bytes from the tile's first column in its first row to the end of the group's last row
+        const unsigned abytes = __builtin_amdgcn_readfirstlane(p.K > 0 ? (unsigned)(p.K * p.lda - m0) : 0u);
+        const unsigned bbytes = __builtin_amdgcn_readfirstlane(p.K > 0 ? (unsigned)(p.K * p.ldb - n0) : 0u);
+        if constexpr (Cfg::OP == OP_I8)
+            asm volatile(GNK_W4_ASM_I8_MM_RAGGED : : GNK_GROUPED_W4_IN, [abytes] "s"(abytes), [bbytes] "s"(bbytes) : GNK_W4_CLOBBERS_RAGGED);
+        else
+            asm volatile(GNK_W4_ASM_F8_MM_RAGGED : : GNK_GROUPED_W4_IN, [abytes] "s"(abytes), [bbytes] "s"(bbytes) : GNK_W4_CLOBBERS_RAGGED);
+    } else {
+        const int ns = (int)(p.K / Cfg::SK);   // a multiple of 4, >= 4 (host-checked)
+        const int nit = __builtin_amdgcn_readfirstlane(ns >> 2), rem = __builtin_amdgcn_readfirstlane(ns - 1);
+#define GNK_GROUPED_W4_RUN(TEXT)                                                                                                      \
+        asm volatile(TEXT : : GNK_GROUPED_W4_IN, [rem] "s"(rem), [oa4] "v"(sa.off[4]), [oa5] "v"(sa.off[5]), [oa6] "v"(sa.off[6]),    \
+                     [oa7] "v"(sa.off[7]), [ob4] "v"(sb.off[4]), [ob5] "v"(sb.off[5]), [ob6] "v"(sb.off[6]), [ob7] "v"(sb.off[7])     \
+                     : GNK_W4_CLOBBERS)
+        if constexpr (Cfg::OP == OP_I8) {
+            if constexpr (Cfg::B_KMAJOR) GNK_GROUPED_W4_RUN(GNK_W4_ASM_I8_KK);
+            else GNK_GROUPED_W4_RUN(GNK_W4_ASM_I8_KM);
+        } else {
+            if constexpr (Cfg::B_KMAJOR) GNK_GROUPED_W4_RUN(GNK_W4_ASM_F8_KK);
+            else GNK_GROUPED_W4_RUN(GNK_W4_ASM_F8_KM);
+        }
+#undef GNK_GROUPED_W4_RUN
+    }
+#undef GNK_GROUPED_W4_IN
+    // the asm ends behind vmcnt(0) + a barrier: LDS is free for the epilogue
+    float *const lsc = (float *)(smem + Cfg::LDS_BYTES);
+    *(GNK_LDS float *)(GNK_LDS char *)((char *)lsc + 4 * threadIdx.x) = gnk_raw_to_f32_rt(raw_r, p.scale_dtype);
+    *(GNK_LDS float *)(GNK_LDS char *)((char *)lsc + 4 * (256 + threadIdx.x)) = gnk_raw_to_f32_rt(raw_c, p.scale_dtype);
+    __syncthreads();
+    K::template finish_half<0>(p, smem, wave, lane, m0 + wm * 128, n0 + wn * 128, lsc, wm * 128, wn * 128);
+    K::template finish_half<1>(p, smem, wave, lane, m0 + wm * 128, n0 + wn * 128, lsc, wm * 128, wn * 128);
+}
+
 // most row tiles the groups can need: every group wastes less than one tile, and the rows behind the last group are one group more
 static inline int64_t max_row_tiles(int64_t T, int64_t E, int64_t bm) {
     const int64_t by_rows = T / bm + E + 1;
@@ -274,7 +357,45 @@ template <class Cfg, bool DEPTH> int launch_two_buffer(const GroupedParams &p0, 
     return gnk_check_launch("grouped mm");
 }
 
+template <class Cfg, bool DEPTH> int launch_w4(const GroupedParams &p0, hipStream_t st) {
+    constexpr int LDS_TOTAL = Cfg::LDS_BYTES + 2048;
+    GroupedParams p = p0;
+    p.g.grid_n = (int)((p.g.N + 255) / 256);
+    p.g.grid_m = DEPTH ? (int)((p.g.M + 255) / 256) : 0;
+    const int64_t blocks = (DEPTH ? p.E * p.g.grid_m : max_row_tiles(p.T, p.E, 256)) * p.g.grid_n;
+    if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "grouped mm: too many tiles");
+    static std::atomic<bool> attr_set[64];
+    const int rc = reserve_lds(w4_kernel<Cfg, DEPTH>, LDS_TOTAL, attr_set);
+    if (rc) return rc;
+    hipLaunchKernelGGL((w4_kernel<Cfg, DEPTH>), dim3((unsigned)blocks), dim3(256), LDS_TOTAL, st, p);
+    return gnk_check_launch("grouped mm (one wave per SIMD)");
+}
+
+// Tile choice, by the cost model of the dense products (gnk_api.hip: us per round of workgroups, one 256 x 256 or two 128 x 128 per CU) on
+// the sizes that the host knows: groups of T / E rows, half a tile of edge each.
+static inline bool prefer_w4(const GroupedParams &p, bool depth) {
+    const double cus = (double)gnk_num_cus();
+    const double groups = (double)(p.E < p.T ? p.E : p.T), rows = (double)p.T;
+    auto tiles = [&](double bm) {
+        const double gn = ceil((double)p.g.N / bm);
+        if (depth) return (double)p.E * ceil((double)p.g.M / bm) * gn;
+        const double m = rows / bm + 0.5 * groups;
+        return (m > groups ? m : groups) * gn;
+    };
+    const double ks = depth ? rows / (double)p.E / 128.0 : (double)p.g.K / 128.0;
+    const double edge = depth ? 1.0 : 0.0;       // a 256-k step of the ragged loop is half empty on average
+    const double t256 = ceil(tiles(256) / cus) * (12.0 + 1.08 * (ks + edge)), t128 = ceil(tiles(128) / (2.0 * cus)) * (6.0 + 1.0 * ks);
+    return t256 <= t128;
+}
+
 template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st) {
+    const bool can_w4 = depth ? p.T * (p.g.lda > p.g.ldb ? p.g.lda : p.g.ldb) < (1LL << 32) : p.g.K >= 256 && p.g.K % 256 == 0;
+    const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1 and 5 choose between the two here as well
+    if (can_w4 && forced != GNK_VARIANT_128 && (forced == GNK_VARIANT_256_W4 || prefer_w4(p, depth))) {
+        if (depth) return launch_w4<PP2Cfg<false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
+        if (b_kmajor) return launch_w4<PP2Cfg<true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
+        return launch_w4<PP2Cfg<true, false, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
+    }
     if (depth) return launch_two_buffer<GemmCfg<128, 128, 2, 2, false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
     if (b_kmajor) return launch_two_buffer<GemmCfg<128, 128, 2, 2, true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
     return launch_two_buffer<GemmCfg<128, 128, 2, 2, true, false, OP, FA, FB, EPI_ROWCOL>, false>(p, st);

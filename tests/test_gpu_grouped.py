@@ -368,3 +368,37 @@ def test_refusals_on_device():
     rc = L.gnk_grouped_scaled_mm_rows(i8(8, 17).data_ptr(), _cabi.I8, i8(2, 17, 16).data_ptr(), _cabi.I8, sc(8, 16).data_ptr(), _cabi.BF16, sc(8).data_ptr(),
                                       sc(2, 16).data_ptr(), _cabi.BF16, 0, offs_of([4, 4]).data_ptr(), 8, 2, 16, 17, 17, 1, 272, 16, 1, None, 0, None)
     assert rc == -4 and b"workspace" in L.gnk_last_error()      # K = 17 needs operand copies
+
+
+# ------------------------------------------------------------------------------------------------ tile variants
+@pytest.fixture(params=[1, 5], ids=["tile128", "tile256w4"])
+def forced(request):
+    L = _cabi.load()
+    old = L.gnk_set_gemm_variant(request.param)
+    yield
+    L.gnk_set_gemm_variant(old)
+
+
+@pytest.mark.parametrize("name", list(SIZES))
+@pytest.mark.parametrize("dt", ["int8", "e4m3", "e5m2"])
+def test_variants_group_sizes(forced, name, dt):
+    sizes, pad = SIZES[name]
+    for order in ((0, 2, 1), (0, 1, 2)):
+        run_rows(sizes, pad, 512, 272, dt, "bf16", order)
+    run_depth(sizes, pad, 272, 528, dt, "bf16")
+
+
+@pytest.mark.parametrize("sizes", [[255, 256, 257], [1, 2, 63, 64, 65], [1023, 1, 1025], [511, 0, 513]])
+def test_variants_depth_ends(forced, sizes):
+    """Ends on, before and behind every step of the contraction; what lies behind a group must not leak into it."""
+    for M, N in ((256, 256), (16, 32), (100, 300)):
+        run_depth(sizes, 3, M, N, "int8", "f32")
+        run_depth(sizes, 3, M, N, "e4m3", "bf16")
+
+
+@pytest.mark.parametrize("out", list(OUT))
+@pytest.mark.parametrize("N", [256, 260, 255])
+def test_variants_outputs(forced, out, N):
+    run_rows([300, 0, 270], 3, 256, N, "int8", out)
+    run_depth([300, 0, 270], 3, N, 264, "int8", out)
+    run_depth([300, 0, 270], 3, 264, N, "int8", out, scalar=True)

@@ -14,6 +14,11 @@ Register plan (fixed; listed as clobbers so the compiler keeps its own values el
     v[128:255]  two fragment sets: set c at v[128 + 64 c ..]: A fragments first (32 registers), then B (32)
     s[72:73] / s[74:75]  A / B base pointers (advanced by s76 / s77 per issue while s80 / s90 > 0), s78 LDS address of this wave's
                 first piece, s79 iterations left (4 stages each), s81 scratch
+    s[92:95] / s[96:99]  ragged loops only (K ends anywhere, both operands M/N-major): A / B buffer descriptors in place of the base pointers;
+                base and bytes left move together, so k-rows past the end are out of the buffer's range and arrive in LDS as zeros
+
+16-bit floats ("f16" / "bf16"): a 64-byte stage holds 32 k.  A K-major operand is byte for byte the int8 one (16 bytes of a row per lane
+and MFMA); an M/N-major stage is [32 k][512 B], 16-byte chunk c of k-row k at c ^ gnk_mn16_swz(k), read with ds_read_b64_tr_b16.
 
 LDS: 64 KiB per operand.  An M/N-major operand is a ring of four 64-k stages ([64 k][256 B], gnk_mn64_*): 4 pieces per wave and stage,
 stage t + 4 issued during stage t.  A K-major operand is a ring of two 128-k "super-stages" ([256 rows][128 B], gnk_kmaj_*: the image of the
@@ -29,13 +34,14 @@ from pathlib import Path
 # 16 = clock stamps around the loop (results right; build with -DGNK_W4_STAMP)
 ABL = int(os.environ.get("GNK_W4_ABL", "0"))
 OUT = Path(__file__).resolve().parent.parent / "quantized-training_amd" / "csrc" / "gnk_gemm_w4_asm.inc"
+MORE = OUT.with_name("gnk_gemm_w4_more_asm.inc")
 
 STAGE_BYTES = 16384      # one operand, one 64-k stage
 SS_BYTES = 32768         # one K-major operand, one 128-k super-stage
 B_RING = 65536           # B's buffers live behind A's (folded into the B read addresses by the caller)
 SET0 = 128               # first VGPR of fragment set 0
-OPERANDS = {"a": dict(ptr="s[72:73]", lo="s72", hi="s73", step="s76", cnt="s80", ring=0, abase=112, src="%[va]", off="oa"),
-            "b": dict(ptr="s[74:75]", lo="s74", hi="s75", step="s77", cnt="s90", ring=B_RING, abase=120, src="%[vb]", off="ob")}
+OPERANDS = {"a": dict(ptr="s[72:73]", lo="s72", hi="s73", step="s76", cnt="s80", ring=0, abase=112, src="%[va]", off="oa", srd="s[92:95]", srd0=92),
+            "b": dict(ptr="s[74:75]", lo="s74", hi="s75", step="s77", cnt="s90", ring=B_RING, abase=120, src="%[vb]", off="ob", srd="s[96:99]", srd0=96)}
 
 
 def frag_reg(cset, operand, f, width):
@@ -48,13 +54,17 @@ def rng(r, n):
 
 
 class Gen:
-    def __init__(self, op, ak, bk):
+    def __init__(self, op, ak, bk, ragged=False):
         self.op = op
+        self.ragged = ragged
+        assert not ragged or not (ak or bk)
         self.kmaj = {"a": ak, "b": bk}
         self.lines = []
         # int8: 16-row fragments of 4 registers (one 64-k MFMA each); fp8: 32-row fragments of 8 registers
-        self.fw = 4 if op == "i8" else 8
-        self.nf = 8 if op == "i8" else 4
+        # (16-bit floats: 16-row fragments of 4 registers, one 32-k MFMA each)
+        self.wide = op == "f8"
+        self.fw = 8 if self.wide else 4
+        self.nf = 4 if self.wide else 8
         self.vm, self.vm_prologue = self.waits()
 
     def e(self, s):
@@ -70,16 +80,17 @@ class Gen:
                 r = frag_reg(cset, operand, f, self.fw)
                 if self.kmaj[operand]:
                     off, ks = ((t >> 1) & 1) * SS_BYTES, t & 1
-                    if self.op == "i8":   # 16 rows x 128 B per fragment: + 2 f KiB; address register ks
+                    if not self.wide:     # 16 rows x 128 B per fragment: + 2 f KiB; address register ks
                         out.append(f"ds_read_b128 v{rng(r, 4)}, v{abase + ks} offset:{off + f * 2048}")
                     else:                 # 32 rows x 128 B per fragment: + 4 f KiB; chunks (h, 2 + h) of the 64-k half: registers 2 ks, 2 ks + 1
                         out.append(f"ds_read_b128 v{rng(r, 4)}, v{abase + 2 * ks} offset:{off + f * 4096}")
                         out.append(f"ds_read_b128 v{rng(r + 4, 4)}, v{abase + 2 * ks + 1} offset:{off + f * 4096}")
                 else:
                     off = (t & 3) * STAGE_BYTES
-                    if self.op == "i8":   # two transposing reads: k rows +0..7 and +8..15 (2 KiB apart)
-                        out.append(f"ds_read_b64_tr_b8 v{rng(r, 2)}, v{abase + f} offset:{off}")
-                        out.append(f"ds_read_b64_tr_b8 v{rng(r + 2, 2)}, v{abase + f} offset:{off + 2048}")
+                    if not self.wide:     # two transposing reads, 2 KiB apart: k rows +0..7 and +8..15 of 256 B (16-bit: +0..3 and +4..7 of 512 B)
+                        tr = "b8" if self.op == "i8" else "b16"
+                        out.append(f"ds_read_b64_tr_{tr} v{rng(r, 2)}, v{abase + f} offset:{off}")
+                        out.append(f"ds_read_b64_tr_{tr} v{rng(r + 2, 2)}, v{abase + f} offset:{off + 2048}")
                     else:                 # fragment f covers 16-column chunks 2 f, 2 f + 1 (lane bit 4 picks); k rows +0, +8, +32, +40
                         for q, ko in enumerate((0, 8, 32, 40)):
                             out.append(f"ds_read_b64_tr_b8 v{rng(r + 2 * q, 2)}, v{abase + f} offset:{off + ko * 256}")
@@ -132,7 +143,8 @@ class Gen:
     def emit_piece(self, pc, out=None):
         operand, lds, i, _ = pc
         o = OPERANDS[operand]
-        ins = [f"s_add_u32 m0, s78, {lds}", "s_nop 0", f"global_load_lds_dwordx4 %[{o['off']}{i}], {o['ptr']}"]
+        load = f"buffer_load_dwordx4 %[{o['off']}{i}], {o['srd']}, 0 offen lds" if self.ragged else f"global_load_lds_dwordx4 %[{o['off']}{i}], {o['ptr']}"
+        ins = [f"s_add_u32 m0, s78, {lds}", "s_nop 0", load]
         if out is None:
             for x in ins:
                 self.e(x)
@@ -140,6 +152,13 @@ class Gen:
 
     def advance(self, operand):
         o = OPERANDS[operand]
+        if self.ragged:
+            b = o["srd0"]
+            self.e(f"s_add_u32 s{b}, s{b}, {o['step']}")
+            self.e(f"s_addc_u32 s{b + 1}, s{b + 1}, 0")
+            self.e(f"s_sub_u32 s{b + 2}, s{b + 2}, {o['step']}")
+            self.e(f"s_cselect_b32 s{b + 2}, 0, s{b + 2}")        # borrow: nothing is left
+            return
         self.e(f"s_cmp_gt_i32 {o['cnt']}, 0")
         self.e(f"s_cselect_b32 s81, {o['step']}, 0")
         self.e(f"s_add_u32 {o['lo']}, {o['lo']}, s81")
@@ -148,12 +167,13 @@ class Gen:
 
     def mfmas(self, cset):
         out = []
-        if self.op == "i8":
+        if not self.wide:
+            ins = {"i8": "v_mfma_i32_16x16x64_i8", "f16": "v_mfma_f32_16x16x32_f16", "bf16": "v_mfma_f32_16x16x32_bf16"}[self.op]
             for s in range(16):
                 i, h = s >> 1, s & 1
                 for j in range(4):
                     t = 32 * h + 4 * i + j
-                    out.append(f"v_mfma_i32_16x16x64_i8 a{rng(4 * t, 4)}, v{rng(frag_reg(cset, 'b', 4 * h + j, 4), 4)}, "
+                    out.append(f"{ins} a{rng(4 * t, 4)}, v{rng(frag_reg(cset, 'b', 4 * h + j, 4), 4)}, "
                                f"v{rng(frag_reg(cset, 'a', i, 4), 4)}, a{rng(4 * t, 4)}")
         else:
             for s in range(16):
@@ -205,11 +225,15 @@ class Gen:
 
     def build(self):
         e = self.e
-        e("s_mov_b32 s72, %[alo]"); e("s_mov_b32 s73, %[ahi]"); e("s_mov_b32 s74, %[blo]"); e("s_mov_b32 s75, %[bhi]")
+        if self.ragged:
+            e("s_mov_b32 s92, %[alo]"); e("s_mov_b32 s93, %[ahi]"); e("s_mov_b32 s94, %[abytes]"); e("s_mov_b32 s95, 0x00027000")
+            e("s_mov_b32 s96, %[blo]"); e("s_mov_b32 s97, %[bhi]"); e("s_mov_b32 s98, %[bbytes]"); e("s_mov_b32 s99, 0x00027000")
+        else:
+            e("s_mov_b32 s72, %[alo]"); e("s_mov_b32 s73, %[ahi]"); e("s_mov_b32 s74, %[blo]"); e("s_mov_b32 s75, %[bhi]")
         e("s_mov_b32 s76, %[stepa]"); e("s_mov_b32 s77, %[stepb]"); e("s_mov_b32 s78, %[lds]")
         e("s_mov_b32 s79, %[nit]")
         # advances left: stages - 1 of a M/N-major operand, super-stages - 1 of a K-major one (%[rem] = stages - 1, odd)
-        for operand in ("a", "b"):
+        for operand in ("a", "b") if not self.ragged else ():
             o = OPERANDS[operand]
             if self.kmaj[operand]:
                 e(f"s_lshr_b32 {o['cnt']}, %[rem], 1")
@@ -220,12 +244,12 @@ class Gen:
             o = OPERANDS[operand]
             base, src = o["abase"], o["src"]
             if self.kmaj[operand]:
-                xs = (0, 64) if self.op == "i8" else (0, 32, 64, 96)
+                xs = (0, 64) if not self.wide else (0, 32, 64, 96)
                 for i, x in enumerate(xs):
                     e(f"v_xor_b32 v{base + i}, {x}, {src}")
             else:
                 for f in range(self.nf):
-                    e(f"v_xor_b32 v{base + f}, {(16 if self.op == 'i8' else 32) * f}, {src}")
+                    e(f"v_xor_b32 v{base + f}, {(16 if self.op == 'i8' else 32) * f}, {src}")    # 16 columns: 16 B (int8), 32 B (16-bit); fp8: 32 columns
         # prologue: four stages of every operand in flight
         # the 256 accumulator clears go out between the LDS-DMA issues (each of which holds the wave's next vector-memory issue for
         # ~60-100 cycles while the VALU is free), not behind them
@@ -266,16 +290,26 @@ class Gen:
         return "".join(f'    "{l}\\n\\t"\n' for l in self.lines)
 
 
+def macro(name, g):
+    body = g.build()
+    print(name, "vmcnt per stage", g.vm, "prologue", g.vm_prologue)
+    return f"#define {name} \\\n" + body.replace("\n", " \\\n").rstrip(" \\\n") + "\n"
+
+
+HEAD = "// GENERATED by tools/gen_w4_asm.py -- do not edit; see that file for the register plan.\n#pragma once\n"
+
+
 def main():
-    parts = ["// GENERATED by tools/gen_w4_asm.py -- do not edit; see that file for the register plan.\n#pragma once\n"]
+    # loops beside the dense 8-bit ones: ragged K (products grouped by expert), 16-bit floats
+    more = [HEAD] + [macro(f"GNK_W4_ASM_{op.upper()}_MM_RAGGED", Gen(op, False, False, ragged=True)) for op in ("i8", "f8")]
+    more += [macro(f"GNK_W4_ASM_F16_{'K' if ak else 'M'}{'K' if bk else 'M'}", Gen("f16", ak, bk)) for ak, bk in ((True, True), (True, False), (False, False))]
+    more.append("#define GNK_W4_CLOBBERS_RAGGED GNK_W4_CLOBBERS, " + ", ".join(f'"s{r}"' for r in range(92, 100)) + "\n")
+    MORE.write_text("\n".join(more))
+    parts = [HEAD]
     for op in ("i8", "f8"):
         for ak in (True, False):
             for bk in (True, False):
-                name = f"GNK_W4_ASM_{op.upper()}_{'K' if ak else 'M'}{'K' if bk else 'M'}"
-                g = Gen(op, ak, bk)
-                body = g.build()
-                print(name, "vmcnt per stage", g.vm, "prologue", g.vm_prologue)
-                parts.append(f"#define {name} \\\n" + body.replace("\n", " \\\n").rstrip(" \\\n") + "\n")
+                parts.append(macro(f"GNK_W4_ASM_{op.upper()}_{'K' if ak else 'M'}{'K' if bk else 'M'}", Gen(op, ak, bk)))
     clob = ['"memory"', '"scc"', '"vcc"'] + [f'"a{r}"' for r in range(256)] + [f'"v{r}"' for r in range(112, 256)] + [f'"s{r}"' for r in range(72, 92)]
     parts.append("#define GNK_W4_CLOBBERS " + ", ".join(clob) + "\n")
     for n in range(16):
