@@ -1,0 +1,474 @@
+// gnk_ortho.hip -- orthogonalisation of matrices by Newton-Schulz products on the 16-bit matrix cores (gfx950).
+//
+//   X_0 = G / max(|G|_F, eps);   S = X X^T (wide) or X^T X (tall),  Q = a I + b S + c S^2,  X <- Q X (wide) or X Q (tall),   `steps` times
+//
+// Three products per step.  Everything between them is kept in fp16 with power-of-two scales and accumulated in fp32: the polynomial amplifies what
+// is small (by a per step where S is near 0), and with it the rounding of the intermediate matrices; bf16's 8 bits leave 1-5 % in the result, fp16's
+// 11 bits an eighth of that at the same matrix rate.  Ranges: |X| <= 1 element by element while its singular values stay around 1, so
+//   X_0 as G 2^p with |G|_F 2^p in [2^14, 2^15): no rounding at all for bf16 and fp16 inputs (1 / |G|_F goes into the products' factors);
+//   later X as X 2^10, S as S 2^10, Q as Q 2^s with |a| + 2 |b| + 4 |c| < 2^(15 - s): nothing overflows, and what underflows is below 2^-24.
+// Shapes are padded with zeros to multiples of 128 in the workspace: zero rows and columns stay zero through every product.
+//
+// The products: `wide` S = X X^T reads both operands along K, Q X reads X as it lies (N-contiguous, transposed on the way out of LDS); `tall` S = X^T X
+// reads X as it lies on both sides, X Q reads along K (Q is symmetric); S^2 = S S^T.  So nothing is ever transposed in memory.
+// Bound: the matrix cores, m^2 n + m^3 + 2 m^2 n operations per step (m <= n; S and S^2 are symmetric).
+#include <math.h>
+#include <string.h>
+
+#include "gnk_gemm_w4.h"
+#include "gnk_gemm_w4_more_asm.inc"
+
+namespace {
+
+using namespace gnk_gemm;
+
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+typedef _Float16 v4h __attribute__((ext_vector_type(4)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+constexpr int PAD = 128;                     // rows and columns of every intermediate are padded to this
+constexpr float SX = 1024.0f, SS = 1024.0f;  // scales of X (after step 0) and S
+constexpr int MAX_PARTS = 64;                // partial sums of squares per matrix
+
+enum { SCALE = 0, POLY = 1 };                // epilogues: acc * f;  acc * f + D * g + (diagonal) h
+
+struct Product {
+    const char *A, *B;
+    void *C;
+    const char *D;                           // POLY: the matrix S
+    int64_t ba, bb, bc, bd;                  // bytes from one matrix of the stack to the next
+    int64_t M, N, K;                         // output extents that are stored; K a multiple of 128
+    int64_t lda, ldb, ldd;                   // bytes
+    int64_t ext_a, ext_b;                    // staged extents (elements, >= M / N, multiples of 128)
+    float f, g, h;
+    const float *fdev;                       // SCALE: a further factor per matrix (step 0), or NULL
+    int fstride;
+    int out_dtype;
+    int batch, grid_m, grid_n;
+};
+
+// Tile of a workgroup: the XCDs take contiguous runs of tiles (matrices one after the other), each walked in strips of four tile rows.
+__device__ __forceinline__ void batch_tile(const Product &p, int &b, int &tm, int &tn) {
+    const int per = p.grid_m * p.grid_n, nwg = per * p.batch;
+    const int xcd = (int)blockIdx.x & 7, idx = (int)blockIdx.x >> 3, q = nwg >> 3, r = nwg & 7;
+    const int wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+    b = wg / per;
+    const int in = wg - b * per;
+    const int width = 4 * p.grid_n, strip = in / width, first = strip * 4, gsz = min(p.grid_m - first, 4), rest = in - strip * width;
+    tm = first + rest % gsz;
+    tn = rest / gsz;
+}
+
+// acc (lane: row m, columns n .. n + 3) -> the stored value
+template <int EPI>
+__device__ __forceinline__ void finish_value(const Product &p, const char *D, float f, v4f &acc, int64_t m, int64_t n) {
+    if constexpr (EPI == SCALE) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r] *= f;
+    } else {
+        const int64_t mm = m < p.ext_a ? m : p.ext_a - 1, nn = n < p.ext_b ? n : p.ext_b - 4;
+        const v4h d = *(const v4h *)(D + mm * p.ldd + 2 * nn);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(acc[r], f, __builtin_fmaf((float)d[r], p.g, m == n + r ? p.h : 0.0f));
+    }
+}
+
+__device__ __forceinline__ GemmParams store_params(const Product &p, int b) {
+    GemmParams g;
+    __builtin_memset(&g, 0, sizeof(g));
+    g.C = (char *)p.C + b * p.bc;
+    g.M = p.M; g.N = p.N; g.K = p.K;
+    g.out_dtype = p.out_dtype;
+    return g;
+}
+
+__device__ __forceinline__ float factor(const Product &p, int b) { return p.fdev ? p.f * p.fdev[(int64_t)b * p.fstride] : p.f; }
+
+// ------------------------------------------------------------------------------ 128 x 128 tiles, two buffers
+template <bool KMAJOR> struct Stager16 {
+    const char *base;
+    unsigned off[4];
+    int64_t step;
+    __device__ __forceinline__ void init(const char *ptr, int64_t ld, int64_t r0, int wave, int lane) {
+        base = KMAJOR ? ptr + r0 * ld : ptr + 2 * r0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int p = (i * 4 + wave) * 64 + lane;
+            int r, c;
+            if constexpr (KMAJOR) gnk_kmaj_stage_src(p, r, c);
+            else gnk_mn16_stage_src<256>(p, r, c);
+            off[i] = (unsigned)(r * ld + 16 * c);
+        }
+        step = KMAJOR ? 128 : 64 * ld;
+    }
+    __device__ __forceinline__ void issue(char *tile, int wave) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            __builtin_amdgcn_global_load_lds((const GNK_GLOBAL void *)(base + off[i]), (GNK_LDS void *)(tile + (i * 4 + wave) * 1024), 16, 0, 0);
+        base += step;
+    }
+};
+
+template <bool KMAJOR> __device__ __forceinline__ v8h frag16(const char *tile, int rb, int ks, int lane) {
+    v4i v;
+    if constexpr (KMAJOR) {
+        v = *(const GNK_LDS v4i *)(const GNK_LDS char *)(tile + gnk_kmaj_frag_offset(rb, ks, lane));
+    } else {
+        const int o = gnk_mn16_frag_offset<256>(rb, ks, lane);
+        const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((GNK_LDS v4s *)(tile + o)));
+        const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((GNK_LDS v4s *)(tile + o + 4 * 256)));
+        v = (v4i){lo[0], lo[1], hi[0], hi[1]};
+    }
+    return __builtin_bit_cast(v8h, v);
+}
+
+template <bool AK, bool BK, int EPI>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) product128_kernel(const Product p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef GemmCfg<128, 128, 2, 2, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;     // fp32 accumulators and the epilogue's maps
+    constexpr int TILE = 128 * 128;                                          // bytes of one operand's 64-k step
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    int b, tm, tn;
+    batch_tile(p, b, tm, tn);
+    const int64_t m0 = (int64_t)tm * 128, n0 = (int64_t)tn * 128;
+    Stager16<AK> sa;
+    Stager16<BK> sb;
+    sa.init(p.A + b * p.ba, p.lda, m0, wave, lane);
+    sb.init(p.B + b * p.bb, p.ldb, n0, wave, lane);
+    v4f acc[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
+    char *const As = smem, *const Bs = smem + 2 * TILE;
+    const int nk = (int)(p.K / 64);
+    sa.issue(As, wave);
+    sb.issue(Bs, wave);
+    for (int t = 0; t < nk; ++t) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        const int cur = (t & 1) * TILE, nxt = TILE - cur;
+        if (t + 1 < nk) {
+            sa.issue(As + nxt, wave);
+            sb.issue(Bs + nxt, wave);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            v8h fa[4], fb[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) fb[j] = frag16<BK>(Bs + cur, wn * 64 + 16 * j, ks, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fa[i] = frag16<AK>(As + cur, wm * 64 + 16 * i, ks, lane);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[j], fa[i], acc[i][j], 0, 0, 0);
+        }
+    }
+    const float f = factor(p, b);
+    const char *D = p.D + b * p.bd;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, D, f, acc[i][j], m0 + wm * 64 + 16 * i + (lane & 15), n0 + wn * 64 + 16 * j + 4 * (lane >> 4));
+    __syncthreads();
+    const GemmParams g = store_params(p, b);
+    run_epilogue<Cfg>(g, acc, nullptr, smem, wave, lane, m0 + wm * 64, n0 + wn * 64);
+}
+
+// ------------------------------------------------------------------------------ 256 x 256 tiles, one wave per SIMD (gnk_gemm_w4.h)
+// The 8-bit loop with 16-bit fragments: a 64-byte stage holds 32 k, so K must be a multiple of 128 (four stages per iteration).
+template <bool KMAJOR> struct StagerW4H {
+    const char *base;
+    unsigned off[8];
+    int64_t step;
+    __device__ __forceinline__ void init(const char *ptr, int64_t ld, int64_t r0, int64_t extent, int wave, int lane) {
+        base = KMAJOR ? ptr + r0 * ld : ptr + 2 * r0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int p = (i * 4 + wave) * 64 + lane;
+            if constexpr (KMAJOR) {
+                int r, c;
+                gnk_kmaj_stage_src(p, r, c);
+                const int64_t rmax = extent - 1 - r0, row = r < rmax ? r : rmax;
+                off[i] = (unsigned)(row * ld + 16 * c);
+            } else {
+                int k, c;
+                gnk_mn16_stage_src<512>(p & 1023, k, c);
+                const int64_t cmax = 2 * (extent - r0) - 16, col = 16 * c < cmax ? 16 * c : cmax;
+                off[i] = (unsigned)(k * ld + col);        // pieces 4-7 repeat 0-3 (unused)
+            }
+        }
+        step = KMAJOR ? 128 : 32 * ld;
+    }
+};
+
+template <int H, int I> __device__ __forceinline__ void fetch_row(v4f (&acc)[8][4]) {
+    int r[16];
+    w4_read16<8 * H + I>(r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        acc[I][j] = (v4f){__int_as_float(r[4 * j]), __int_as_float(r[4 * j + 1]), __int_as_float(r[4 * j + 2]), __int_as_float(r[4 * j + 3])};
+}
+
+// columns 64 H .. 64 H + 63 of the wave tile: accumulators -> values -> memory
+template <class Cfg, int EPI, int H>
+__device__ __forceinline__ void finish_half(const Product &p, const GemmParams &g, const char *D, float f, char *smem, int wave, int lane, int64_t mw, int64_t nw) {
+    v4f acc[8][4];
+    fetch_row<H, 0>(acc); fetch_row<H, 1>(acc); fetch_row<H, 2>(acc); fetch_row<H, 3>(acc);
+    fetch_row<H, 4>(acc); fetch_row<H, 5>(acc); fetch_row<H, 6>(acc); fetch_row<H, 7>(acc);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, D, f, acc[i][j], mw + 16 * i + (lane & 15), nw + 64 * H + 16 * j + 4 * (lane >> 4));
+    run_epilogue<Cfg>(g, acc, nullptr, smem, wave * 2 + H, lane, mw, nw + 64 * H);
+}
+
+template <bool AK, bool BK, int EPI>
+__global__ void __launch_bounds__(256) product256_kernel(const Product p) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    typedef GemmCfg<256, 256, 2, 4, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;      // the epilogue's maps: 128 x 64 halves of a wave's 128 x 128
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1;
+    int b, tm, tn;
+    batch_tile(p, b, tm, tn);
+    const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * 256;
+    StagerW4H<AK> sa;
+    StagerW4H<BK> sb;
+    sa.init(p.A + b * p.ba, p.lda, m0, p.ext_a, wave, lane);
+    sb.init(p.B + b * p.bb, p.ldb, n0, p.ext_b, wave, lane);
+    const unsigned lds0 = (unsigned)(uintptr_t)(GNK_LDS char *)smem;
+    const unsigned va = lds0 + (AK ? gnk_kmaj_frag_offset(wm * 128, 0, lane) : gnk_mn16_frag_offset<512>(wm * 128, 0, lane));
+    const unsigned vb = lds0 + 65536 + (BK ? gnk_kmaj_frag_offset(wn * 128, 0, lane) : gnk_mn16_frag_offset<512>(wn * 128, 0, lane));
+    const unsigned alo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)sa.base), ahi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)sa.base >> 32));
+    const unsigned blo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)sb.base), bhi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)sb.base >> 32));
+    const unsigned stepa = __builtin_amdgcn_readfirstlane((unsigned)sa.step), stepb = __builtin_amdgcn_readfirstlane((unsigned)sb.step);
+    const unsigned ldsw = __builtin_amdgcn_readfirstlane(lds0 + wave * 1024);
+    const int ns = (int)(p.K / 32);
+    const int nit = __builtin_amdgcn_readfirstlane(ns >> 2), rem = __builtin_amdgcn_readfirstlane(ns - 1);
+#define GNK_ORTHO_RUN(TEXT)                                                                                                           \
+    asm volatile(TEXT : : [alo] "s"(alo), [ahi] "s"(ahi), [blo] "s"(blo), [bhi] "s"(bhi), [stepa] "s"(stepa), [stepb] "s"(stepb),      \
+                 [lds] "s"(ldsw), [nit] "s"(nit), [rem] "s"(rem), [va] "v"(va), [vb] "v"(vb),                                         \
+                 [oa0] "v"(sa.off[0]), [oa1] "v"(sa.off[1]), [oa2] "v"(sa.off[2]), [oa3] "v"(sa.off[3]),                              \
+                 [oa4] "v"(sa.off[4]), [oa5] "v"(sa.off[5]), [oa6] "v"(sa.off[6]), [oa7] "v"(sa.off[7]),                              \
+                 [ob0] "v"(sb.off[0]), [ob1] "v"(sb.off[1]), [ob2] "v"(sb.off[2]), [ob3] "v"(sb.off[3]),                              \
+                 [ob4] "v"(sb.off[4]), [ob5] "v"(sb.off[5]), [ob6] "v"(sb.off[6]), [ob7] "v"(sb.off[7]) : GNK_W4_CLOBBERS)
+    if constexpr (AK && BK) GNK_ORTHO_RUN(GNK_W4_ASM_F16_KK);
+    else if constexpr (AK) GNK_ORTHO_RUN(GNK_W4_ASM_F16_KM);
+    else GNK_ORTHO_RUN(GNK_W4_ASM_F16_MM);
+#undef GNK_ORTHO_RUN
+    // the asm ends behind vmcnt(0) + a barrier: LDS is free for the epilogue
+    const float f = factor(p, b);
+    const char *D = p.D + b * p.bd;
+    const GemmParams g = store_params(p, b);
+    const int64_t mw = m0 + wm * 128, nw = n0 + wn * 128;
+    finish_half<Cfg, EPI, 0>(p, g, D, f, smem, wave, lane, mw, nw);
+    finish_half<Cfg, EPI, 1>(p, g, D, f, smem, wave, lane, mw, nw);
+}
+
+// ------------------------------------------------------------------------------ sums of squares, conversion
+template <int DT> __device__ __forceinline__ float load1(const void *p, int64_t i) { return gnk_load_scalar<DT>(p, i); }
+
+template <int DT>
+__global__ void __launch_bounds__(256) square_sum_kernel(const void *__restrict__ G, double *__restrict__ parts, int64_t numel, int nparts) {
+    // fp64: the squares of any fp32 fit, and nothing is lost on the way
+    const int64_t b = blockIdx.y, per = (numel + nparts - 1) / nparts, i0 = (int64_t)blockIdx.x * per, i1 = i0 + per < numel ? i0 + per : numel;
+    double s = 0.0;
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
+        const double v = load1<DT>(G, b * numel + i);
+        s += v * v;
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+    __shared__ double red[4];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) parts[b * nparts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// fac[b] = {factor of step 0's S, factor of step 0's update}: what takes G 2^p back to X_0
+template <int DT>
+__global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G, unsigned short *__restrict__ X, const double *__restrict__ parts, float *__restrict__ fac,
+                                                      int64_t rows, int64_t cols, int64_t rows_p, int64_t cols_p, int nparts, float eps) {
+    const int64_t b = blockIdx.y;
+    double sum = 0.0;
+    for (int k = 0; k < nparts; ++k) sum += parts[b * nparts + k];      // every block adds in the same order
+    const double norm = sqrt(sum);
+    int p = 0;
+    double inv = 1.0 / (norm > (double)eps ? norm : (double)eps);
+    const bool finite = norm < 1.0e300;                                  // false for NaN and Inf: every output becomes NaN through the factors
+    if (finite && norm > 0.0) p = 14 - ilogb(norm);
+    if (!finite) inv = __builtin_nan("");
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        const double x0 = ldexp(inv, -p);
+        fac[2 * b] = (float)(x0 * x0);
+        fac[2 * b + 1] = (float)x0;
+    }
+    const int64_t quads = rows_p * cols_p / 4;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / (cols_p / 4), c = (i - r * (cols_p / 4)) * 4;
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = finite && r < rows && c + k < cols ? load1<DT>(G, (b * rows + r) * cols + c + k) : 0.0f;
+            v[k] = ldexpf(v[k], p);
+        }
+        const v2i o = {(int)gnk_pack2_f16(v[0], v[1]), (int)gnk_pack2_f16(v[2], v[3])};
+        *(v2i *)(X + (b * rows_p + r) * cols_p + c) = o;
+    }
+}
+
+template <int BM, bool AK, bool BK, int EPI> int launch(const Product &p0, hipStream_t st) {
+    constexpr int LDS_TOTAL = BM == 256 ? 131072 : 65536;
+    auto *const kernel = BM == 256 ? product256_kernel<AK, BK, EPI> : product128_kernel<AK, BK, EPI>;
+    Product p = p0;
+    p.grid_m = (int)((p.ext_a + BM - 1) / BM);
+    p.grid_n = (int)((p.ext_b + BM - 1) / BM);
+    static std::atomic<bool> attr_set[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return gnk_fail(GNK_ERR_LAUNCH, "orthogonalize: no current HIP device");
+    if (!attr_set[dev].load(std::memory_order_acquire)) {
+        if (hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS_TOTAL) != hipSuccess)
+            return gnk_fail(GNK_ERR_LAUNCH, "orthogonalize: cannot reserve LDS");
+        attr_set[dev].store(true, std::memory_order_release);
+    }
+    const int64_t blocks = (int64_t)p.grid_m * p.grid_n * p.batch;
+    if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), LDS_TOTAL, st, p);
+    return gnk_check_launch("orthogonalize");
+}
+
+int64_t up(int64_t v) { return (v + PAD - 1) / PAD * PAD; }
+
+struct Plan {
+    int64_t rp, cp, lo;                      // padded rows, columns, and the smaller of them
+    int64_t x_bytes, s_bytes;                // one matrix
+    int nparts;
+    int64_t off_x0, off_x1, off_s, off_q, off_parts, off_fac, total;
+};
+
+Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
+    Plan p;
+    p.rp = up(rows); p.cp = up(cols);
+    p.lo = rows <= cols ? p.rp : p.cp;
+    p.x_bytes = 2 * p.rp * p.cp;
+    p.s_bytes = 2 * p.lo * p.lo;
+    const int64_t want = (rows * cols + 16383) / 16384;
+    p.nparts = (int)(want < MAX_PARTS ? (want > 0 ? want : 1) : MAX_PARTS);
+    p.off_x0 = 0;
+    p.off_x1 = p.off_x0 + batch * p.x_bytes;
+    p.off_s = p.off_x1 + batch * p.x_bytes;
+    p.off_q = p.off_s + batch * p.s_bytes;
+    p.off_parts = p.off_q + batch * p.s_bytes;
+    p.off_fac = p.off_parts + (batch * p.nparts * 8 + 15) / 16 * 16;
+    p.total = p.off_fac + (batch * 8 + 15) / 16 * 16;
+    return p;
+}
+
+template <int EPI> int run_product(bool ak, bool bk, const Product &p, hipStream_t st) {
+    // the cost model of the dense products (gnk_api.hip): us per round of workgroups, one 256 x 256 or two 128 x 128 per CU; a step is 64 k
+    const double cus = (double)gnk_num_cus(), ks = (double)p.K / 64.0;
+    const double t256 = ceil((double)(((p.ext_a + 255) / 256) * ((p.ext_b + 255) / 256) * p.batch) / cus) * (12.0 + 1.08 * ks);
+    const double t128 = ceil((double)((p.ext_a / 128) * (p.ext_b / 128) * p.batch) / (2.0 * cus)) * (6.0 + 1.0 * ks);
+    const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1 and 5 choose between the two here as well
+    if (forced != 1 && (forced == 5 || t256 <= t128)) {
+        if (ak) return bk ? launch<256, true, true, EPI>(p, st) : launch<256, true, false, EPI>(p, st);
+        return launch<256, false, false, EPI>(p, st);
+    }
+    if (ak) return bk ? launch<128, true, true, EPI>(p, st) : launch<128, true, false, EPI>(p, st);
+    return launch<128, false, false, EPI>(p, st);
+}
+
+}  // namespace
+
+extern "C" int64_t gnk_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
+    if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    return make_plan(batch, rows, cols).total;
+}
+
+extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
+                                 float eps, void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *name = "orthogonalize";
+    if (batch < 0 || rows < 0 || cols < 0) return gnk_fail(GNK_ERR_BAD_ARG, "%s: negative dimension", name);
+    if (!gnk_is_float_dtype(g_dtype) || !gnk_is_float_dtype(out_dtype)) return gnk_fail(GNK_ERR_BAD_ARG, "%s: dtype codes %d, %d are not bf16/f16/f32", name, g_dtype, out_dtype);
+    if (steps < 1 || steps > 100) return gnk_fail(GNK_ERR_BAD_ARG, "%s: %d steps", name, steps);
+    const float cmax = fabsf(a) + 2.0f * fabsf(b) + 4.0f * fabsf(c);
+    if (!(cmax < 1.0e4f) || !(eps >= 0.0f)) return gnk_fail(GNK_ERR_BAD_ARG, "%s: coefficients (%g, %g, %g), eps %g", name, a, b, c, eps);
+    if (batch > 65535 || rows > (1 << 20) || cols > (1 << 20)) return gnk_fail(GNK_ERR_UNSUPPORTED, "%s: %lld matrices of %lld x %lld", name, (long long)batch, (long long)rows, (long long)cols);
+    if (batch == 0 || rows == 0 || cols == 0) return GNK_OK;
+    if (!G || !out) return gnk_fail(GNK_ERR_BAD_ARG, "%s: null pointer", name);
+    const Plan pl = make_plan(batch, rows, cols);
+    if (!workspace || workspace_bytes < pl.total || ((uintptr_t)workspace & 15) != 0)
+        return gnk_fail(GNK_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %lld bytes", name, (long long)pl.total);
+    int rc = gnk_init();
+    if (rc) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    char *const ws = (char *)workspace;
+    double *const parts = (double *)(ws + pl.off_parts);
+    float *const fac = (float *)(ws + pl.off_fac);
+    char *X = ws + pl.off_x0, *Xn = ws + pl.off_x1;
+    char *const S = ws + pl.off_s, *const Q = ws + pl.off_q;
+    const dim3 g1((unsigned)pl.nparts, (unsigned)batch);
+    const int64_t quads = pl.rp * pl.cp / 4, wantb = (quads + 255) / 256;
+    const dim3 g2((unsigned)(wantb < 512 ? wantb : 512), (unsigned)batch);
+#define GNK_ORTHO_IN(DT)                                                                                                                              \
+    do {                                                                                                                                              \
+        hipLaunchKernelGGL((square_sum_kernel<DT>), g1, dim3(256), 0, st, G, parts, rows * cols, pl.nparts);                                          \
+        hipLaunchKernelGGL((convert_kernel<DT>), g2, dim3(256), 0, st, G, (unsigned short *)X, parts, fac, rows, cols, pl.rp, pl.cp, pl.nparts, eps); \
+    } while (0)
+    if (g_dtype == GNK_BF16) GNK_ORTHO_IN(GNK_BF16);
+    else if (g_dtype == GNK_F16) GNK_ORTHO_IN(GNK_F16);
+    else GNK_ORTHO_IN(GNK_F32);
+#undef GNK_ORTHO_IN
+    rc = gnk_check_launch(name);
+    if (rc) return rc;
+
+    const bool wide = rows <= cols;
+    float sq = 32768.0f;                     // scale of Q: |Q| <= |a| + 2 |b| + 4 |c| while the singular values stay below sqrt 2
+    while (sq * cmax >= 32768.0f) sq *= 0.5f;
+    const int64_t lo = pl.lo, ldx = 2 * pl.cp, lds = 2 * lo;
+    for (int it = 0; it < steps; ++it) {
+        Product p;
+        memset(&p, 0, sizeof(p));
+        p.batch = (int)batch;
+        p.fstride = 2;
+        // S
+        p.A = p.B = X; p.ba = p.bb = pl.x_bytes; p.lda = p.ldb = ldx;
+        p.C = S; p.bc = pl.s_bytes;
+        p.M = p.N = p.ext_a = p.ext_b = lo;
+        p.K = wide ? pl.cp : pl.rp;
+        p.f = it == 0 ? SS : SS / (SX * SX);
+        p.fdev = it == 0 ? fac : nullptr;
+        p.out_dtype = GNK_F16;
+        rc = run_product<SCALE>(wide, wide, p, st);
+        if (rc) return rc;
+        // Q = a I + b S + c S^2
+        p.A = p.B = S; p.ba = p.bb = pl.s_bytes; p.lda = p.ldb = lds;
+        p.C = Q; p.bc = pl.s_bytes;
+        p.D = S; p.bd = pl.s_bytes; p.ldd = lds;
+        p.K = lo;
+        p.f = c * sq / (SS * SS); p.g = b * sq / SS; p.h = a * sq;
+        p.fdev = nullptr;
+        rc = run_product<POLY>(true, true, p, st);
+        if (rc) return rc;
+        // X <- Q X or X Q
+        const bool last = it + 1 == steps;
+        p.A = wide ? Q : X; p.ba = wide ? pl.s_bytes : pl.x_bytes; p.lda = wide ? lds : ldx;
+        p.B = wide ? X : Q; p.bb = wide ? pl.x_bytes : pl.s_bytes; p.ldb = wide ? ldx : lds;
+        p.C = last ? out : (void *)Xn;
+        p.bc = last ? rows * cols * gnk_dtype_size(out_dtype) : pl.x_bytes;
+        p.ext_a = pl.rp; p.ext_b = pl.cp;
+        p.M = last ? rows : pl.rp; p.N = last ? cols : pl.cp;
+        p.K = lo;
+        p.out_dtype = last ? out_dtype : GNK_F16;
+        p.f = (last ? 1.0f : SX) / (it == 0 ? sq : sq * SX);
+        p.fdev = it == 0 ? fac + 1 : nullptr;
+        rc = run_product<SCALE>(true, !wide, p, st);
+        if (rc) return rc;
+        char *const t = X; X = Xn; Xn = t;
+    }
+    return GNK_OK;
+}

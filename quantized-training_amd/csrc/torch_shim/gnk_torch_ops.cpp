@@ -261,6 +261,24 @@ std::tuple<at::Tensor, at::Tensor> quantize_int8_grouped(const at::Tensor &x, co
     return {q, scale};
 }
 
+at::Tensor orthogonalize(const at::Tensor &G_in, int64_t steps, double a, double b, double c, double eps) {
+    const char *op = "orthogonalize";
+    TORCH_CHECK(is_float(G_in.scalar_type()) && G_in.dim() >= 2, "gn_kernels::", op, ": unsupported input (shape ", G_in.sizes(), ", dtype ", G_in.scalar_type(), ")");
+    const at::Tensor G = G_in.contiguous();
+    const int64_t rows = G.size(-2), cols = G.size(-1);
+    int64_t batch = 1;
+    for (int64_t d = 0; d < G.dim() - 2; ++d) batch *= G.size(d);
+    at::Tensor out = at::empty(G.sizes(), G.options());
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(G.device());
+    const int64_t nws = gnk_orthogonalize_workspace_bytes(batch, rows, cols);
+    const at::Tensor ws = workspace_for(G, nws);
+    const int code = dtype_code(G.scalar_type(), op);
+    check(gnk_orthogonalize(G.data_ptr(), code, out.data_ptr(), code, batch, rows, cols, (int)steps, (float)a, (float)b, (float)c, (float)eps,
+                            nws > 0 ? ws.data_ptr() : nullptr, nws, stream_of(G)),
+          op);
+    return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_IMPL(gn_kernels, CUDA, m) {
@@ -274,4 +292,5 @@ TORCH_LIBRARY_IMPL(gn_kernels, CUDA, m) {
     m.impl("grouped_scaled_mm", &grouped_scaled_mm);
     m.impl("grouped_scaled_mm_depth", &grouped_scaled_mm_depth);
     m.impl("quantize_int8_grouped", &quantize_int8_grouped);
+    m.impl("orthogonalize", &orthogonalize);
 }

@@ -8,6 +8,7 @@ from .fp8 import fp8_mm, scaled_fp8_mm
 from .grouped import grouped_scaled_mm, quantize_int8_grouped
 from .mm import _triton_mm, int8_mm, scaled_mm, scaled_mm_t
 from .mx import dequantize_mxfp4, mxfp4_mm, mxfp8_mm, pack_block_scales_nv, quantize_mx
+from .ortho import orthogonalize
 from .quantize import quantize_int8
 
 
@@ -44,6 +45,7 @@ __all__ = [
     "scaled_mm",
     "scaled_mm_t",
     "grouped_scaled_mm",
+    "orthogonalize",
     "quantize_int8",
     "quantize_int8_grouped",
     "quantize_mx",

@@ -11,7 +11,7 @@ import torch
 
 # GNK_LIBRARY: tuning only (an A/B build of the same sources, e.g. `make ABLATE=1 OUT=...`); the shipped library is the default
 _LIB_PATH = Path(os.environ.get("GNK_LIBRARY") or Path(__file__).resolve().parent / "libgnk_hip.so")
-ABI_VERSION = 3   # include/gnk.h GNK_ABI_VERSION
+ABI_VERSION = 4   # include/gnk.h GNK_ABI_VERSION
 
 BF16, F16, F32, I8, E4M3, E5M2, I32 = range(7)
 DTYPE_CODE = {
@@ -31,7 +31,7 @@ _lib = None
 # GNK_NO_TORCH_SHIM=1 keeps the Python implementations (A/B timing of the host path, and the tests' second leg).
 _SHIM_PATH = Path(__file__).resolve().parent / "libgnk_torch_ops.so"
 _SHIM_OPS = ("int8_mm", "scaled_mm", "scaled_mm_t", "tile_scaled_mm", "quantize_int8", "quantize_int8_rowwise_colmax", "quantize_int8_colwise_given",
-             "grouped_scaled_mm", "grouped_scaled_mm_depth", "quantize_int8_grouped")
+             "grouped_scaled_mm", "grouped_scaled_mm_depth", "quantize_int8_grouped", "orthogonalize")
 _shim_loaded = None
 
 
@@ -115,6 +115,9 @@ def load() -> ctypes.CDLL:
     L.gnk_quantize_int8_grouped_workspace_bytes.argtypes = [i64] * 3
     L.gnk_quantize_int8_grouped_workspace_bytes.restype = i64
     L.gnk_quantize_int8_grouped.argtypes = [vp, ci, vp] + [i64] * 5 + [vp, vp, f32, ci, u64, u64, vp, i64, vp]
+    L.gnk_orthogonalize_workspace_bytes.argtypes = [i64] * 3
+    L.gnk_orthogonalize_workspace_bytes.restype = i64
+    L.gnk_orthogonalize.argtypes = [vp, ci, vp, ci, i64, i64, i64, ci, f32, f32, f32, f32, vp, i64, vp]
     if L.gnk_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libgnk_hip.so ABI {L.gnk_abi_version()} != expected {ABI_VERSION}; rebuild it")
     _lib = L

@@ -1,0 +1,174 @@
+"""orthogonalize against the iteration in 64 bits.
+
+Tolerance, in the norm of the result.  The kernels round S, Q and X once each per step to fp16 (as S 2^10, Q 2^s, X 2^10) and the result to its type;
+sums are fp32, K * 2^-24 of sum |a b| off at most, which moves some of those roundings to the neighbouring fp16 value and nothing else.  So the
+same iteration in 64 bits with the same roundings (`rounded`) has errors of the same size, drawn anew where a sum lay next to a border: the kernels'
+error may be at most twice the emulation's, plus half a step of the result's type, plus 2^-11 |X|, one fp16 rounding of X, for matrices so small
+that there is nothing to average over."""
+import math
+
+import pytest
+import torch
+
+import gn_kernels
+from gn_kernels import _cabi
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+COEFFS = (3.4445, -4.7750, 2.0315)
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def iterate(G, steps, co, eps, rounded):
+    a, b, c = co
+    X = G.double().cpu()
+    sq = 32768.0
+    while sq * (abs(a) + 2 * abs(b) + 4 * abs(c)) >= 32768:
+        sq /= 2
+
+    def q(t, scale):
+        return (t * scale).half().double() / scale if rounded else t
+
+    norm = X.norm().item()
+    if G.dtype is torch.float32 and norm > 0:        # X_0 of bf16 and fp16 inputs is exact
+        X = q(X, 2.0 ** (14 - math.floor(math.log2(norm))))
+    X = X / max(norm, eps)
+    tall = X.shape[0] > X.shape[1]
+    X = X.T if tall else X
+    for i in range(steps):
+        S = q(X @ X.T, 1024.0)
+        X = q(a * torch.eye(S.shape[0], dtype=S.dtype) + b * S + c * S @ S, sq) @ X
+        X = q(X, 1024.0) if i + 1 < steps else X
+    return X.T if tall else X
+
+
+def reference(G, steps=5, co=COEFFS, eps=1e-7):
+    """The result in 64 bits, and the tolerance of the module's comment for the norm of the difference."""
+    X = iterate(G, steps, co, eps, False)
+    own = (iterate(G, steps, co, eps, True) - X).norm().item()
+    return X, 2 * own + (torch.finfo(G.dtype).eps / 2 + 2.0 ** -11) * X.norm().item()
+
+
+def matrix(m, n, dt, seed=0, kind="momentum"):
+    g = torch.Generator().manual_seed(seed)
+    if kind == "gauss":
+        return torch.randn(m, n, generator=g).to(DT[dt])
+    r = max(1, min(m, n) // 8)
+    return ((torch.randn(m, r, generator=g) @ torch.randn(r, n, generator=g)) / r ** 0.5 + 0.3 * torch.randn(m, n, generator=g)).mul(1e-3).to(DT[dt])
+
+
+def compare(got, G, **kw):
+    want, tol = reference(G, **kw)
+    assert got.dtype is G.dtype and got.shape == G.shape and torch.isfinite(got).all()
+    err = (got.double().cpu() - want).norm().item()
+    assert err <= tol, f"{err:.3e} off, tolerance {tol:.3e}, norm {want.norm():.3e}"
+
+
+@pytest.fixture(params=[-1, 1, 5], ids=["auto", "tile128", "tile256w4"])
+def forced(request):
+    L = _cabi.load()
+    old = L.gnk_set_gemm_variant(request.param)
+    yield
+    L.gnk_set_gemm_variant(old)
+
+
+@pytest.mark.parametrize("m,n", [(1, 1), (1, 70), (70, 1), (2, 3), (16, 16), (127, 129), (128, 128), (129, 127), (255, 300), (300, 257), (333, 999), (999, 333), (640, 384)])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_shapes(forced, m, n, dt):
+    G = matrix(m, n, dt, seed=m + n)
+    compare(gn_kernels.orthogonalize(G.to(DEV)), G)
+
+
+@pytest.mark.parametrize("m,n", [(96, 200), (200, 96), (256, 256)])
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("kind", ["gauss", "momentum"])
+def test_types(m, n, dt, kind):
+    G = matrix(m, n, dt, kind=kind)
+    compare(gn_kernels.orthogonalize(G.to(DEV)), G)
+
+
+@pytest.mark.parametrize("lead", [(3,), (2, 2), (17,)])
+@pytest.mark.parametrize("m,n", [(40, 150), (150, 40)])
+def test_stacks(forced, lead, m, n):
+    G = torch.stack([matrix(m, n, "bf16", seed=i) * 4.0 ** (i - 4) for i in range(torch.Size(lead).numel())]).view(*lead, m, n)
+    got = gn_kernels.orthogonalize(G.to(DEV))
+    for x, g in zip(got.view(-1, m, n), G.view(-1, m, n)):
+        compare(x, g)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1e-4, 1.0, 1e4, 1e30])
+def test_scale_of_the_input(scale):
+    """Any magnitude that bf16 holds: the norm is taken in 64 bits, below eps the input is divided by eps."""
+    G = (matrix(48, 80, "f32") * 1e3 * scale).bfloat16()
+    compare(gn_kernels.orthogonalize(G.to(DEV)), G)
+
+
+@pytest.mark.parametrize("steps,co", [(1, COEFFS), (2, COEFFS), (10, (2.0, -1.5, 0.5)), (6, (1.875, -1.25, 0.375))])
+def test_steps_and_coefficients(steps, co):
+    G = matrix(64, 130, "bf16")
+    compare(gn_kernels.orthogonalize(G.to(DEV), steps=steps, coefficients=co), G, steps=steps, co=co)
+
+
+def test_special_values():
+    """Zeros stay zeros; a NaN or Inf poisons its own matrix only."""
+    G = torch.stack([matrix(30, 50, "bf16", seed=i) for i in range(4)])
+    G[0] = 0
+    G[1, 3, 4], G[2, 7, 0] = float("nan"), float("inf")
+    got = gn_kernels.orthogonalize(G.to(DEV)).cpu()
+    assert (got[0] == 0).all() and got[1].isnan().all() and got[2].isnan().all()
+    compare(got[3], G[3])
+
+
+def test_strides():
+    base = matrix(70, 140, "bf16")
+    for view in (base.T, base[:, ::2], base[3:60, 5:]):
+        d = base.to(DEV)
+        dv = d.T if view.shape == (140, 70) and view.stride() == (1, 140) else d[:, ::2] if view.stride() == (140, 2) else d[3:60, 5:]
+        got = gn_kernels.orthogonalize(dv)
+        assert got.is_contiguous()
+        compare(got, view.contiguous())
+
+
+def test_orthogonal_result():
+    """What it is for: with the default coefficients every singular value above 1e-2 of the norm ends in [0.6, 1.3], as in 64 bits."""
+    G = matrix(120, 200, "bf16", kind="gauss")
+    s = torch.linalg.svdvals(gn_kernels.orthogonalize(G.to(DEV)).double().cpu())
+    assert s.min() > 0.6 and s.max() < 1.3
+
+
+def test_graph_and_streams():
+    G = torch.stack([matrix(100, 180, "bf16", seed=i) for i in range(2)]).to(DEV)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = gn_kernels.orthogonalize(G)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gn_kernels.orthogonalize(G)
+    for k in range(3):
+        G.mul_(1.0 + k).add_(1e-4 * k)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = gn_kernels.orthogonalize(G)
+        assert torch.equal(out, want)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    outs = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            outs += [gn_kernels.orthogonalize(G) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_refusals():
+    with pytest.raises(RuntimeError):
+        torch.ops.gn_kernels.orthogonalize(torch.zeros(4, 4, dtype=torch.float64, device=DEV), 5, *COEFFS, 1e-7)
+    with pytest.raises(RuntimeError):
+        torch.ops.gn_kernels.orthogonalize(torch.zeros(4, 4, device=DEV), 0, *COEFFS, 1e-7)
+    with pytest.raises(RuntimeError):
+        torch.ops.gn_kernels.orthogonalize(torch.zeros(4, 4, device=DEV), 5, 1e6, 0.0, 0.0, 1e-7)
+    assert gn_kernels.orthogonalize(torch.zeros(0, 4, 5, device=DEV)).shape == (0, 4, 5)
+    assert gn_kernels.orthogonalize(torch.zeros(3, 0, 5, device=DEV)).shape == (3, 0, 5)
