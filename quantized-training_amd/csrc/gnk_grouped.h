@@ -46,62 +46,59 @@ struct Tile {
 __device__ __forceinline__ int64_t clamp_end(int v, int64_t T) { return v < 0 ? 0 : (v < T ? v : T); }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int64_t uniform64(int64_t v) {
-    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)((uint64_t)v >> 32));
-    return (int64_t)(((uint64_t)hi << 32) | lo);
-}
 
-// inclusive prefix sum over the wave
-__device__ __forceinline__ int wave_prefix(int v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int o = __shfl_up(v, d, 64);
-        v += lane >= d ? o : 0;
-    }
+// inclusive prefix sum over the wave: row shifts, then the two row broadcasts (no LDS round trips)
+__device__ __forceinline__ int wave_prefix(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);      // lane 15 of a row into the next row: rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);      // lane 31 into rows 2 and 3
     return v;
 }
 
-// Group and rows of lane `lane` in the 64-group step that starts at group g0: group E takes the rows behind the last end.
-__device__ __forceinline__ void lane_group(const int *ends, int64_t E, int64_t T, int64_t g0, int lane, int64_t &lo, int64_t &hi) {
+// Rows [lo, hi) of group g0 + lane; group E takes the rows behind the last end, groups beyond it none.  (T < 2^31.)
+__device__ __forceinline__ void lane_group(const int *ends, int64_t E, int64_t T, int64_t g0, int lane, int &lo, int &hi) {
     const int64_t e = g0 + lane;
-    lo = e > 0 && e <= E ? clamp_end(ends[e - 1], T) : 0;
-    hi = e < E ? clamp_end(ends[e], T) : (e == E ? T : lo);
+    lo = e > 0 && e <= E ? (int)clamp_end(ends[e - 1], T) : 0;
+    hi = e < E ? (int)clamp_end(ends[e], T) : (e == E ? (int)T : lo);
     if (hi < lo) hi = lo;
 }
 
 // Every group (and the rows behind the last one) is cut into pieces of 1 << sh rows, numbered in group order.
-__device__ __forceinline__ int pieces_of(int64_t rows, int sh) { return (int)((rows + (1LL << sh) - 1) >> sh); }
+__device__ __forceinline__ int pieces_of(int rows, int sh) { return (int)(((unsigned)rows + ((1u << sh) - 1)) >> sh); }
 
 __device__ __forceinline__ int count_pieces(const int *ends, int64_t E, int64_t T, int lane, int sh) {
     int total = 0;
     for (int64_t g0 = 0; g0 <= E; g0 += 64) {
-        int64_t lo, hi;
+        int lo, hi;
         lane_group(ends, E, T, g0, lane, lo, hi);
-        total += uniform(__shfl(wave_prefix(pieces_of(hi - lo, sh), lane), 63, 64));
+        total += __builtin_amdgcn_readlane(wave_prefix(pieces_of(hi - lo, sh)), 63);
     }
     return total;
 }
 
-// piece number `want`: its group e (E: rows of no group; -1: there are fewer pieces), its number within the group and the group's rows
-__device__ __forceinline__ void find_piece(const int *ends, int64_t E, int64_t T, int lane, int sh, int want, int &e, int &idx, int64_t &lo, int64_t &hi) {
-    int before = 0;
+// Piece number `want`: its group e (E: rows of no group; -1: there are fewer pieces), its number within the group, the group's rows, and the
+// number of pieces of 1 << sh2 rows in the groups in front of it.
+struct Piece { int e, idx, lo, hi, first2; };
+__device__ __forceinline__ Piece find_piece(const int *ends, int64_t E, int64_t T, int lane, int sh, int want, int sh2) {
+    int before = 0, before2 = 0;
     for (int64_t g0 = 0; g0 <= E; g0 += 64) {
-        int64_t l, h;
+        int l, h;
         lane_group(ends, E, T, g0, lane, l, h);
-        const int n = pieces_of(h - l, sh), incl = wave_prefix(n, lane) + before;
+        const int n = pieces_of(h - l, sh), n2 = pieces_of(h - l, sh2);
+        const int incl = wave_prefix(n) + before, incl2 = wave_prefix(n2) + before2;
         const unsigned long long hit = __ballot(incl > want);
         if (hit) {
             const int src = __builtin_ctzll(hit);
-            e = (int)g0 + src;
-            idx = want - (__shfl(incl, src, 64) - __shfl(n, src, 64));
-            lo = __shfl((long long)l, src, 64);
-            hi = __shfl((long long)h, src, 64);
-            e = uniform(e); idx = uniform(idx); lo = uniform64(lo); hi = uniform64(hi);
-            return;
+            return {(int)g0 + src, want - __builtin_amdgcn_readlane(incl - n, src), __builtin_amdgcn_readlane(l, src), __builtin_amdgcn_readlane(h, src),
+                    __builtin_amdgcn_readlane(incl2 - n2, src)};
         }
-        before = uniform(__shfl(incl, 63, 64));
+        before = __builtin_amdgcn_readlane(incl, 63);
+        before2 = __builtin_amdgcn_readlane(incl2, 63);
     }
-    e = -1; idx = 0; lo = hi = 0;
+    return {-1, 0, 0, 0, 0};
 }
 
 // rows form: tiles are counted on the device, then given to the XCDs in contiguous runs and walked in strips as tile_of_block does
@@ -115,7 +112,8 @@ __device__ __forceinline__ Tile rows_tile(const GroupedParams &p, int grid_n, in
     if (!t.work) return t;
     int tm, tn;
     tile_of_block(grid_m, grid_n, tm, tn);
-    find_piece(p.ends, p.E, p.T, lane, SH, tm, t.e, t.tm, t.lo, t.hi);
+    const Piece pc = find_piece(p.ends, p.E, p.T, lane, SH, tm, SH);
+    t.e = pc.e; t.tm = pc.idx; t.lo = pc.lo; t.hi = pc.hi;
     t.tn = tn;
     return t;
 }
@@ -247,6 +245,72 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cf
                       wm * Cfg::WTM, wn * Cfg::WTN);
 }
 
+// ------------------------------------------------------------------------------ 64 x 64, ring of four stages (few rows: latency and the weights' bytes)
+// Few tiles leave one or two workgroups on a CU, and a group of a few rows is bound by the bytes of its weights: what counts is how much is in
+// flight.  Three 128-k stages of 16 KiB are, behind the one being read (2 workgroups per CU: ~50 KiB of weights in flight per CU), one barrier per
+// stage.  Stage t lands before the barrier of step t (vmcnt leaves the pieces of t + 1 and t + 2 in flight); the buffer of stage t - 1, which every
+// wave has read by then, takes stage t + 3 behind it.  Towards the end nothing is left to issue and the wait is for everything.
+template <class Cfg, bool DEPTH>
+__global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(2))) ring_kernel(const GroupedParams gp) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int MT = Cfg::MT, NTL = Cfg::NTL, NST = 4, STAGE = Cfg::A_BYTES + Cfg::B_BYTES;
+    constexpr int PIECES = (Cfg::BM + Cfg::BN) / 8 / Cfg::NW;      // LDS-DMA instructions per wave and stage
+    typedef typename AccT<Cfg::OP>::type acc_t;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
+    if (!tile.work) return;
+    const int64_t m0 = (int64_t)tile.tm * Cfg::BM, n0 = (int64_t)tile.tn * Cfg::BN;
+    if (!DEPTH && tile.e == gp.E) {
+        zero_tile<Cfg::BM, Cfg::BN, Cfg::NT>((char *)gp.g.C + tile.lo * gp.g.N * gp.out_bytes, tile.hi - tile.lo, gp.g.N, m0, n0, gp.out_bytes);
+        return;
+    }
+    int64_t ext_a, ext_b;
+    const GemmParams p = tile_params<DEPTH>(gp, tile, ext_a, ext_b);
+    ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, EPI_ROWCOL> spf;
+    spf.issue(p, m0, n0);
+    Stager<Cfg::A_KMAJOR, Cfg::BM, Cfg::NW> sa;
+    Stager<Cfg::B_KMAJOR, Cfg::BN, Cfg::NW> sb;
+    sa.init(p.A, p.lda, m0, ext_a, wave, lane);
+    sb.init(p.B, p.ldb, n0, ext_b, wave, lane);
+    acc_t acc[MT][NTL];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) acc[i][j] = (acc_t){0, 0, 0, 0};
+    const int nk = (int)((p.K + GNK_BK - 1) / GNK_BK), ktail = (int)(p.K % GNK_BK);
+    auto fetch = [&](int t) {
+        char *const As = smem + (t % NST) * STAGE, *const Bs = As + Cfg::A_BYTES;
+        if (ktail && t + 1 == nk) {
+            sa.issue_tail(As, p.lda, m0, ext_a, wave, lane, ktail);
+            sb.issue_tail(Bs, p.ldb, n0, ext_b, wave, lane, ktail);
+        } else {
+            sa.issue(As, wave);
+            sb.issue(Bs, wave);
+        }
+    };
+    for (int t = 0; t < NST - 1 && t < nk; ++t) fetch(t);
+    for (int t = 0; t < nk; ++t) {
+        static_assert(2 * PIECES <= 63, "vmcnt holds 6 bits");
+        if (t + NST - 2 < nk) asm volatile("s_waitcnt vmcnt(%0)" : : "i"((NST - 2) * PIECES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        char *const As = smem + (t % NST) * STAGE, *const Bs = As + Cfg::A_BYTES;
+        if (ktail && t + 1 == nk) {
+            zero_tail<Cfg::A_KMAJOR, Cfg::BM, Cfg::NT>(As, ktail);
+            zero_tail<Cfg::B_KMAJOR, Cfg::BN, Cfg::NT>(Bs, ktail);
+            __syncthreads();
+        }
+        if (t + NST - 1 < nk) fetch(t + NST - 1);
+        compute_step<Cfg, false>(As, Bs, acc, wm, wn, lane);
+    }
+    float *const lsc = (float *)(smem + NST * STAGE);
+    spf.park(p, (char *)lsc);
+    __syncthreads();
+    run_epilogue<Cfg>(p, acc, nullptr, smem, wave, lane, m0 + wm * Cfg::WTM, n0 + wn * Cfg::WTN, lsc, wm * Cfg::WTM, wn * Cfg::WTN);
+}
+
 // ------------------------------------------------------------------------------ 256 x 256, one wave per SIMD (gnk_gemm_w4.h)
 // rows: K % 256 == 0, the dense loop on the group's tile.  depth: the contraction ends where the group does, so the loop reads through buffer
 // descriptors that end there too: k-rows past the end are out of range and arrive in LDS as zeros, which add nothing in int8 and fp8; the loop
@@ -343,37 +407,38 @@ template <class Kernel> static int reserve_lds(Kernel k, int bytes, std::atomic<
     return GNK_OK;
 }
 
-template <class Cfg, bool DEPTH> int launch_two_buffer(const GroupedParams &p0, hipStream_t st) {
-    constexpr int LDS_TOTAL = Cfg::LDS_BYTES + ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, EPI_ROWCOL>::BYTES;
+// Tile sizes of a launch over the whole grid; KERNEL with its LDS.
+template <class Kernel> int launch_tiles(Kernel kernel, std::atomic<bool> (&done)[64], int lds, int threads, bool depth, int bm, int bn, const GroupedParams &p0, hipStream_t st) {
     GroupedParams p = p0;
-    p.g.grid_n = (int)((p.g.N + Cfg::BN - 1) / Cfg::BN);
-    p.g.grid_m = DEPTH ? (int)((p.g.M + Cfg::BM - 1) / Cfg::BM) : 0;
-    const int64_t blocks = (DEPTH ? p.E * p.g.grid_m : max_row_tiles(p.T, p.E, Cfg::BM)) * p.g.grid_n;
+    p.g.grid_n = (int)((p.g.N + bn - 1) / bn);
+    p.g.grid_m = depth ? (int)((p.g.M + bm - 1) / bm) : 0;
+    const int64_t blocks = (depth ? p.E * p.g.grid_m : max_row_tiles(p.T, p.E, bm)) * p.g.grid_n;
     if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "grouped mm: too many tiles");
-    static std::atomic<bool> attr_set[64];
-    const int rc = reserve_lds(two_buffer_kernel<Cfg, DEPTH>, LDS_TOTAL, attr_set);
+    const int rc = reserve_lds(kernel, lds, done);
     if (rc) return rc;
-    hipLaunchKernelGGL((two_buffer_kernel<Cfg, DEPTH>), dim3((unsigned)blocks), dim3(Cfg::NT), LDS_TOTAL, st, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), lds, st, p);
     return gnk_check_launch("grouped mm");
 }
 
-template <class Cfg, bool DEPTH> int launch_w4(const GroupedParams &p0, hipStream_t st) {
-    constexpr int LDS_TOTAL = Cfg::LDS_BYTES + 2048;
-    GroupedParams p = p0;
-    p.g.grid_n = (int)((p.g.N + 255) / 256);
-    p.g.grid_m = DEPTH ? (int)((p.g.M + 255) / 256) : 0;
-    const int64_t blocks = (DEPTH ? p.E * p.g.grid_m : max_row_tiles(p.T, p.E, 256)) * p.g.grid_n;
-    if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "grouped mm: too many tiles");
-    static std::atomic<bool> attr_set[64];
-    const int rc = reserve_lds(w4_kernel<Cfg, DEPTH>, LDS_TOTAL, attr_set);
-    if (rc) return rc;
-    hipLaunchKernelGGL((w4_kernel<Cfg, DEPTH>), dim3((unsigned)blocks), dim3(256), LDS_TOTAL, st, p);
-    return gnk_check_launch("grouped mm (one wave per SIMD)");
+template <class Cfg, bool DEPTH> int launch_two_buffer(const GroupedParams &p, hipStream_t st) {
+    static std::atomic<bool> done[64];
+    return launch_tiles(two_buffer_kernel<Cfg, DEPTH>, done, Cfg::LDS_BYTES + ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, EPI_ROWCOL>::BYTES, Cfg::NT, DEPTH, Cfg::BM,
+                        Cfg::BN, p, st);
 }
 
-// Tile choice, by the cost model of the dense products (gnk_api.hip: us per round of workgroups, one 256 x 256 or two 128 x 128 per CU) on
-// the sizes that the host knows: groups of T / E rows, half a tile of edge each.
-static inline bool prefer_w4(const GroupedParams &p, bool depth) {
+template <class Cfg, bool DEPTH> int launch_ring(const GroupedParams &p, hipStream_t st) {
+    static std::atomic<bool> done[64];
+    return launch_tiles(ring_kernel<Cfg, DEPTH>, done, 4 * (Cfg::A_BYTES + Cfg::B_BYTES) + (Cfg::BM + Cfg::BN) * 4, Cfg::NT, DEPTH, Cfg::BM, Cfg::BN, p, st);
+}
+
+template <class Cfg, bool DEPTH> int launch_w4(const GroupedParams &p, hipStream_t st) {
+    static std::atomic<bool> done[64];
+    return launch_tiles(w4_kernel<Cfg, DEPTH>, done, Cfg::LDS_BYTES + 2048, 256, DEPTH, 256, 256, p, st);
+}
+
+// Tile choice, by the cost model of the dense products (gnk_api.hip: us per round of workgroups; one 256 x 256 or two 128 x 128 per CU) on the
+// sizes that the host knows: groups of T / E rows, half a tile of edge each.
+static inline int choose_variant(const GroupedParams &p, bool depth, bool can_w4) {
     const double cus = (double)gnk_num_cus();
     const double groups = (double)(p.E < p.T ? p.E : p.T), rows = (double)p.T;
     auto tiles = [&](double bm) {
@@ -385,16 +450,26 @@ static inline bool prefer_w4(const GroupedParams &p, bool depth) {
     const double ks = depth ? rows / (double)p.E / 128.0 : (double)p.g.K / 128.0;
     const double edge = depth ? 1.0 : 0.0;       // a 256-k step of the ragged loop is half empty on average
     const double t256 = ceil(tiles(256) / cus) * (12.0 + 1.08 * (ks + edge)), t128 = ceil(tiles(128) / (2.0 * cus)) * (6.0 + 1.0 * ks);
-    return t256 <= t128;
+    const double t64 = ceil(tiles(64) / (2.0 * cus)) * (5.0 + 0.45 * ks);
+    if (t64 <= t128 && (t64 <= t256 || !can_w4)) return GNK_VARIANT_64X128;
+    return can_w4 && t256 <= t128 ? GNK_VARIANT_256_W4 : GNK_VARIANT_128;
 }
 
 template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st) {
     const bool can_w4 = depth ? p.T * (p.g.lda > p.g.ldb ? p.g.lda : p.g.ldb) < (1LL << 32) : p.g.K >= 256 && p.g.K % 256 == 0;
-    const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1 and 5 choose between the two here as well
-    if (can_w4 && forced != GNK_VARIANT_128 && (forced == GNK_VARIANT_256_W4 || prefer_w4(p, depth))) {
+    // gnk_set_gemm_variant: 1, 5 and 6 force the 128 x 128, the 256 x 256 (where it can run) and the 64 x 64 kernel
+    int variant = gnk_forced_variant_get();
+    if ((variant != GNK_VARIANT_128 && variant != GNK_VARIANT_64X128 && variant != GNK_VARIANT_256_W4) || (variant == GNK_VARIANT_256_W4 && !can_w4))
+        variant = choose_variant(p, depth, can_w4);
+    if (variant == GNK_VARIANT_256_W4) {
         if (depth) return launch_w4<PP2Cfg<false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
         if (b_kmajor) return launch_w4<PP2Cfg<true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
         return launch_w4<PP2Cfg<true, false, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
+    }
+    if (variant == GNK_VARIANT_64X128) {
+        if (depth) return launch_ring<GemmCfg<64, 64, 4, 1, false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
+        if (b_kmajor) return launch_ring<GemmCfg<64, 64, 4, 1, true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
+        return launch_ring<GemmCfg<64, 64, 4, 1, true, false, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
     }
     if (depth) return launch_two_buffer<GemmCfg<128, 128, 2, 2, false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
     if (b_kmajor) return launch_two_buffer<GemmCfg<128, 128, 2, 2, true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);

@@ -212,21 +212,23 @@ int partial_shift(int64_t T) {
     return sh;
 }
 
-template <int DT, int VEC> __device__ __forceinline__ void load_vec(const char *p, float (&f)[VEC]) {
+// VEC adjacent elements as loaded (one 16-byte word, or the bits of a single element) and as floats
+template <int DT, int VEC> __device__ __forceinline__ v4i load_vec(const char *p) {
+    if constexpr (VEC == 1) return (v4i){(int)gnk_load_raw<DT>(p, 0), 0, 0, 0};
+    else return *(const v4i *)p;
+}
+template <int DT, int VEC> __device__ __forceinline__ void floats_of(const v4i &raw, float (&f)[VEC]) {
     if constexpr (VEC == 1) {
-        f[0] = gnk_load_scalar<DT>(p, 0);
+        f[0] = gnk_raw_to_f32<DT>((unsigned)raw[0]);
+    } else if constexpr (DT == GNK_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = __int_as_float(raw[i]);
     } else {
-        const v4i raw = *(const v4i *)p;
-        if constexpr (DT == GNK_F32) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[i] = __int_as_float(raw[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const unsigned w = (unsigned)raw[i];
-                f[2 * i] = gnk_raw_to_f32<DT>(w & 0xffffu);
-                f[2 * i + 1] = gnk_raw_to_f32<DT>(w >> 16);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const unsigned w = (unsigned)raw[i];
+            f[2 * i] = gnk_raw_to_f32<DT>(w & 0xffffu);
+            f[2 * i + 1] = gnk_raw_to_f32<DT>(w >> 16);
         }
     }
 }
@@ -235,39 +237,38 @@ template <int DT, int VEC, int CL>
 __global__ void __launch_bounds__(256)
 group_absmax_kernel(const char *__restrict__ x, unsigned *__restrict__ partial, const int *__restrict__ ends, int64_t T, int64_t E, int64_t C, int64_t row_bytes,
                     int64_t col_bytes, int sh) {
-    constexpr int RL = 256 / CL, U = 8;
+    constexpr int RL = 256 / CL, U = 16;
     const int lane = threadIdx.x & 63;
-    int e, idx;
-    int64_t lo, hi;
-    find_piece(ends, E, T, lane, sh, (int)blockIdx.y, e, idx, lo, hi);
-    if (e < 0 || e == E) return;
-    const int64_t r0 = lo + ((int64_t)idx << sh), r1 = r0 + (1LL << sh) < hi ? r0 + (1LL << sh) : hi;
+    const Piece pc = find_piece(ends, E, T, lane, sh, (int)blockIdx.y, sh);
+    if (pc.e < 0 || pc.e == E) return;
+    const int64_t r0 = pc.lo + ((int64_t)pc.idx << sh), r1 = r0 + (1LL << sh) < pc.hi ? r0 + (1LL << sh) : pc.hi;
     const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
     const int64_t col0 = ((int64_t)blockIdx.x * CL + cl) * VEC;
-    unsigned m[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) m[j] = 0u;
+    unsigned mw[4] = {0u, 0u, 0u, 0u};                    // per loaded word: two packed 16-bit patterns, or one fp32 pattern
     if (col0 < C) {
         const char *src = x + col0 * col_bytes;
         for (int64_t r = r0 + rl; r < r1; r += RL * U) {
-            float f[U][VEC];
+            v4i raw[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {       // a row past the piece repeats its last row: the same maximum
-                const int64_t row = r + RL * u < r1 ? r + RL * u : r1 - 1;
-                load_vec<DT, VEC>(src + row * row_bytes, f[u]);
+            for (int u = 0; u < U; ++u) {                  // 16 loads in flight; a row past the piece counts for nothing
+                raw[u] = (v4i){0, 0, 0, 0};
+                if (r + RL * u < r1) raw[u] = load_vec<DT, VEC>(src + (r + RL * u) * row_bytes);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    const unsigned a = __float_as_uint(f[u][j]) & 0x7fffffffu;
-                    m[j] = a > m[j] ? a : m[j];
+                for (int j = 0; j < (VEC == 1 ? 1 : 4); ++j) {
+                    if constexpr (DT == GNK_F32) { const unsigned a = (unsigned)raw[u][j] & 0x7fffffffu; mw[j] = a > mw[j] ? a : mw[j]; }
+                    else mw[j] = gnk_pk_max_u16(mw[j], (unsigned)raw[u][j] & 0x7fff7fffu);
                 }
         }
     }
+    const v4i most = {(int)mw[0], (int)mw[1], (int)mw[2], (int)mw[3]};
+    float m[VEC];
+    floats_of<DT, VEC>(most, m);
     __shared__ unsigned red[RL][CL * VEC + 1];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) red[rl][cl * VEC + j] = m[j];
+    for (int j = 0; j < VEC; ++j) red[rl][cl * VEC + j] = __float_as_uint(m[j]);
     __syncthreads();
     for (int c = threadIdx.x; c < CL * VEC; c += 256) {
         unsigned v = red[0][c];
@@ -278,51 +279,60 @@ group_absmax_kernel(const char *__restrict__ x, unsigned *__restrict__ partial, 
     }
 }
 
-template <int DT, int VEC, int CL, bool SR>
+template <int DT, int VEC, int CL, bool SR, int ROWS_SH>
 __global__ void __launch_bounds__(256)
 group_quant_kernel(const char *__restrict__ x, int8_t *__restrict__ q, void *__restrict__ scale, const unsigned *__restrict__ partial,
                    const int *__restrict__ ends, int64_t T, int64_t E, int64_t C, int64_t row_bytes, int64_t col_bytes, int sh, float eps,
                    unsigned long long seed, unsigned long long offset) {
-    constexpr int RL = 256 / CL;
+    constexpr int RL = 256 / CL, NIT = (1 << ROWS_SH) / RL, U = NIT < 16 ? NIT : 16;
     const int lane = threadIdx.x & 63;
     const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
     const int64_t col0 = ((int64_t)blockIdx.x * CL + cl) * VEC;
     if (blockIdx.y == 0) {                       // groups without rows have no piece: their scale (0) is written here
-        for (int64_t g = 0; g < E; ++g) {
-            const int64_t a = g > 0 ? clamp_end(ends[g - 1], T) : 0, b = clamp_end(ends[g], T);
-            if (b <= a && rl == 0 && col0 < C)
-                for (int j = 0; j < VEC; ++j) gnk_store_scalar_rt(scale, DT, g * C + col0 + j, 0.0f);
+        for (int64_t g0 = 0; g0 < E; g0 += 64) {
+            int l, h;
+            lane_group(ends, E, T, g0, lane, l, h);
+            unsigned long long none = __ballot(g0 + lane < E && h == l);
+            while (none) {
+                const int64_t g = g0 + __builtin_ctzll(none);
+                none &= none - 1;
+                if (rl == 0 && col0 < C)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) gnk_store_scalar_rt(scale, DT, g * C + col0 + j, 0.0f);
+            }
         }
     }
-    int e, idx;
-    int64_t lo, hi;
-    find_piece(ends, E, T, lane, GQ_ROWS_SH, (int)blockIdx.y, e, idx, lo, hi);
-    if (e < 0) return;
-    const int64_t r0 = lo + ((int64_t)idx << GQ_ROWS_SH), r1 = r0 + (1LL << GQ_ROWS_SH) < hi ? r0 + (1LL << GQ_ROWS_SH) : hi;
-    if (e == E) {                                // rows of no group
+    const Piece pc = find_piece(ends, E, T, lane, ROWS_SH, (int)blockIdx.y, sh);
+    if (pc.e < 0) return;
+    const int64_t r0 = pc.lo + ((int64_t)pc.idx << ROWS_SH), r1 = r0 + (1LL << ROWS_SH) < pc.hi ? r0 + (1LL << ROWS_SH) : pc.hi;
+    if (pc.e == E) {                             // rows of no group
         if (col0 < C)
             for (int64_t r = r0 + rl; r < r1; r += RL)
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) q[r * C + col0 + j] = 0;
         return;
     }
-    // the partial rows of this group start behind those of the groups in front of it
-    int first = 0;
-    for (int64_t g0 = 0; g0 < e; g0 += 64) {
-        int64_t l, h;
-        lane_group(ends, E, T, g0, lane, l, h);
-        const int n = g0 + lane < e ? pieces_of(h - l, sh) : 0;
-        first += uniform(__shfl(wave_prefix(n, lane), 63, 64));
+    // The first 16 rows of this thread are loaded before the partial maxima are waited for.
+    const char *src = x + (col0 < C ? col0 : 0) * col_bytes;
+    v4i raw[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t r = r0 + rl + RL * u;
+        raw[u] = (v4i){0, 0, 0, 0};
+        if (r < r1) raw[u] = load_vec<DT, VEC>(src + r * row_bytes);
     }
-    const int nparts = pieces_of(hi - lo, sh);
+    const int nparts = pieces_of(pc.hi - pc.lo, sh);
     __shared__ unsigned cm[CL * VEC];
     for (int c = threadIdx.x; c < CL * VEC; c += 256) {
         const int64_t col = (int64_t)blockIdx.x * CL * VEC + c;
         unsigned v = 0u;
         if (col < C)
-            for (int k = 0; k < nparts; ++k) {
-                const unsigned w = partial[(int64_t)(first + k) * C + col];
-                v = w > v ? w : v;
+            for (int k0 = 0; k0 < nparts; k0 += 8) {
+                unsigned w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) w[k] = k0 + k < nparts ? partial[(int64_t)(pc.first2 + k0 + k) * C + col] : 0u;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) v = w[k] > v ? w[k] : v;
             }
         cm[c] = v;
     }
@@ -335,11 +345,11 @@ group_quant_kernel(const char *__restrict__ x, int8_t *__restrict__ q, void *__r
         const float s = __fmul_rn(__uint_as_float(cm[cl * VEC + j]), GQ_INV127);
         dv[j].set(gnk_clamp_min_nan(s, eps));
         fast = fast && dv[j].ok();
-        if (idx == 0 && rl == 0) gnk_store_scalar_rt(scale, DT, (int64_t)e * C + col0 + j, s);
+        if (pc.idx == 0 && rl == 0) gnk_store_scalar_rt(scale, DT, (int64_t)pc.e * C + col0 + j, s);
     }
-    for (int64_t r = r0 + rl; r < r1; r += RL) {
+    auto emit = [&](const v4i &word, int64_t r) {
         float f[VEC];
-        load_vec<DT, VEC>(x + r * row_bytes + col0 * col_bytes, f);
+        floats_of<DT, VEC>(word, f);
         int qi[VEC];
         float u[VEC];
         if constexpr (SR) {
@@ -357,11 +367,12 @@ group_quant_kernel(const char *__restrict__ x, int8_t *__restrict__ q, void *__r
                 for (int j = 0; j < VEC; ++j) u[j] = gnk_sr_uniform(seed, offset, idx0 + j);
             }
         }
+        if (fast) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float v = fast ? dv[j].quot(f[j]) : f[j] / dv[j].d;
-            if constexpr (SR) qi[j] = gnk_sr_clip_i8(v, u[j]);
-            else qi[j] = gnk_rne_clip_i8_any(v);
+            for (int j = 0; j < VEC; ++j) qi[j] = SR ? gnk_sr_clip_i8(dv[j].quot(f[j]), u[j]) : gnk_rne_clip_i8(dv[j].quot(f[j]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) qi[j] = SR ? gnk_sr_clip_i8(f[j] / dv[j].d, u[j]) : gnk_rne_clip_i8_any(f[j] / dv[j].d);
         }
         int8_t *dst = q + r * C + col0;
         if constexpr (VEC == 8) {
@@ -369,13 +380,19 @@ group_quant_kernel(const char *__restrict__ x, int8_t *__restrict__ q, void *__r
 #pragma unroll
             for (int h = 0; h < 2; ++h)
                 o[h] = (qi[4 * h] & 0xff) | ((qi[4 * h + 1] & 0xff) << 8) | ((qi[4 * h + 2] & 0xff) << 16) | (int)((unsigned)(qi[4 * h + 3] & 0xff) << 24);
-            *(v2i *)dst = o;
+            __builtin_nontemporal_store(o, (v2i *)dst);
         } else if constexpr (VEC == 4) {
             *(int *)dst = (qi[0] & 0xff) | ((qi[1] & 0xff) << 8) | ((qi[2] & 0xff) << 16) | (int)((unsigned)(qi[3] & 0xff) << 24);
         } else {
             dst[0] = (int8_t)qi[0];
         }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t r = r0 + rl + RL * u;
+        if (r < r1) emit(raw[u], r);
     }
+    for (int64_t r = r0 + rl + RL * U; r < r1; r += RL) emit(load_vec<DT, VEC>(src + r * row_bytes), r);
 }
 
 template <int DT, bool VECTOR>
@@ -384,16 +401,23 @@ int launch_group_quant(const void *x, int8_t *q, void *scale, const int *ends, i
     constexpr int ES = DT == GNK_F32 ? 4 : 2, VEC = VECTOR ? 16 / ES : 1, CL = VECTOR ? 32 : 64;
     const int sh = partial_shift(T);
     const unsigned gx = (unsigned)((C + CL * VEC - 1) / (CL * VEC));
-    const int64_t p1 = max_row_tiles(T, E, 1LL << sh), p2 = max_row_tiles(T, E, 1LL << GQ_ROWS_SH);
+    // 128-row pieces once they fill the chip; below that a thread's 16 rows of arithmetic (~5 us) are the kernel's length, and 32-row ones quarter it
+    const int rows_sh = max_row_tiles(T, E, 128) * (int64_t)gx * 2 >= 3 * (int64_t)gnk_num_cus() || max_row_tiles(T, E, 32) > 65535 ? GQ_ROWS_SH : 5;
+    const int64_t p1 = max_row_tiles(T, E, 1LL << sh), p2 = max_row_tiles(T, E, 1LL << rows_sh);
     // gridDim.y carries the pieces
     const dim3 g1(gx, (unsigned)(p1 > 0 ? p1 : 1)), g2(gx, (unsigned)(p2 > 0 ? p2 : 1));
     hipLaunchKernelGGL((group_absmax_kernel<DT, VEC, CL>), g1, dim3(256), 0, st, (const char *)x, partial, ends, T, E, C, sxt * ES, sxc * ES, sh);
-    if (sr)
-        hipLaunchKernelGGL((group_quant_kernel<DT, VEC, CL, true>), g2, dim3(256), 0, st, (const char *)x, q, scale, partial, ends, T, E, C, sxt * ES, sxc * ES,
-                           sh, eps, seed, offset);
-    else
-        hipLaunchKernelGGL((group_quant_kernel<DT, VEC, CL, false>), g2, dim3(256), 0, st, (const char *)x, q, scale, partial, ends, T, E, C, sxt * ES, sxc * ES,
-                           sh, eps, seed, offset);
+#define GNK_GQ_RUN(SR, SH)                                                                                                                             \
+    hipLaunchKernelGGL((group_quant_kernel<DT, VEC, CL, SR, SH>), g2, dim3(256), 0, st, (const char *)x, q, scale, partial, ends, T, E, C, sxt * ES,      \
+                       sxc * ES, sh, eps, seed, offset)
+    if (sr) {
+        if (rows_sh == 5) GNK_GQ_RUN(true, 5);
+        else GNK_GQ_RUN(true, GQ_ROWS_SH);
+    } else {
+        if (rows_sh == 5) GNK_GQ_RUN(false, 5);
+        else GNK_GQ_RUN(false, GQ_ROWS_SH);
+    }
+#undef GNK_GQ_RUN
     return gnk_check_launch("quantize_int8_grouped");
 }
 

@@ -371,7 +371,7 @@ def test_refusals_on_device():
 
 
 # ------------------------------------------------------------------------------------------------ tile variants
-@pytest.fixture(params=[1, 5], ids=["tile128", "tile256w4"])
+@pytest.fixture(params=[1, 5, 6], ids=["tile128", "tile256w4", "tile64"])
 def forced(request):
     L = _cabi.load()
     old = L.gnk_set_gemm_variant(request.param)
