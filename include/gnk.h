@@ -293,11 +293,11 @@ int gnk_grouped_scaled_mm_depth(const void *A, int a_dtype, const void *B, int b
                                 int64_t N, int64_t sam, int64_t sat, int64_t sbt, int64_t sbn, void *workspace, int64_t workspace_bytes, void *stream);
 
 /*
- * gnk_quantize_int8 along the rows of every group (the quantization in front of gnk_grouped_scaled_mm_depth; with ends = N, 2 N, ... also the
- * column-wise one of a stack of weights):  scale[e,c] = max_{t in e} |x[t,c]| * fl(1 / 127) (fp32, stored as x_dtype; 0 for a group without
+ * gnk_quantize_int8 along the rows of every group (the quantization in front of gnk_grouped_scaled_mm_depth):  scale[e,c] = max_{t in e} |x[t,c]| * fl(1 / 127) (fp32, stored as x_dtype; 0 for a group without
  * rows; eager torch's `amax / 127` on a device, within 1.5 fp32 steps of gnk_quantize_int8's quotient),
  * q[t,c] = clip(round_half_even(x[t,c] / max(scale[e,c], eps)), -128, 127) with the unrounded scale, 0 for rows of no group.
- * x (T, C) with strides (sxt, sxc); q (T, C) and scale (E, C) contiguous; `ends` as above.  sr, seed, offset as in gnk_quantize_int8 with
+ * x (T, C) with strides (sxt, sxc); q (T, C) and scale (E, C) contiguous; `ends` as above, or NULL for groups of T / E rows each (a stack of
+ * matrices of that many rows).  sr, seed, offset as in gnk_quantize_int8 with
  * e = t * C + c + offset.  workspace: gnk_quantize_int8_grouped_workspace_bytes() bytes, 4-byte aligned, need not be cleared.
  */
 int64_t gnk_quantize_int8_grouped_workspace_bytes(int64_t T, int64_t E, int64_t C);

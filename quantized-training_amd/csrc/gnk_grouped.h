@@ -58,9 +58,15 @@ __device__ __forceinline__ int wave_prefix(int v) {
     return v;
 }
 
-// Rows [lo, hi) of group g0 + lane; group E takes the rows behind the last end, groups beyond it none.  (T < 2^31.)
+// Rows [lo, hi) of group g0 + lane; group E takes the rows behind the last end, groups beyond it none.  (T < 2^31.)  ends == NULL: equal groups.
 __device__ __forceinline__ void lane_group(const int *ends, int64_t E, int64_t T, int64_t g0, int lane, int &lo, int &hi) {
     const int64_t e = g0 + lane;
+    if (!ends) {
+        const int each = E > 0 ? (int)((unsigned)T / (unsigned)E) : 0;
+        lo = e <= E ? (int)e * each : 0;
+        hi = e < E ? lo + each : (e == E ? (int)T : lo);
+        return;
+    }
     lo = e > 0 && e <= E ? (int)clamp_end(ends[e - 1], T) : 0;
     hi = e < E ? (int)clamp_end(ends[e], T) : (e == E ? (int)T : lo);
     if (hi < lo) hi = lo;

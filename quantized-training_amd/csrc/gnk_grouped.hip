@@ -438,7 +438,7 @@ extern "C" int gnk_quantize_int8_grouped(const void *x, int x_dtype, const int32
     const int64_t pieces = max_row_tiles(T, E, 1LL << GQ_ROWS_SH);
     if (pieces > 65535) return gnk_fail(GNK_ERR_UNSUPPORTED, "%s: %lld rows in %lld groups are too many", name, (long long)T, (long long)E);
     if (C == 0 || (T == 0 && E == 0)) return GNK_OK;
-    if ((T > 0 && (!x || !q)) || (E > 0 && (!ends || !scale))) return gnk_fail(GNK_ERR_BAD_ARG, "%s: null pointer", name);
+    if ((T > 0 && (!x || !q)) || (E > 0 && !scale)) return gnk_fail(GNK_ERR_BAD_ARG, "%s: null pointer", name);
     const int64_t need = gnk_quantize_int8_grouped_workspace_bytes(T, E, C);
     if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 3) != 0))
         return gnk_fail(GNK_ERR_WORKSPACE, "%s: needs a workspace of %lld bytes", name, (long long)need);

@@ -261,6 +261,101 @@ std::tuple<at::Tensor, at::Tensor> quantize_int8_grouped(const at::Tensor &x, co
     return {q, scale};
 }
 
+// F.grouped_mm on a mixed-precision weight (subclasses/mixed_precision.py), forward and backward as one call each: seven quantizations and three products
+// whose host path would otherwise cost more than the kernels of a small layer.  w: (E, K, N) as grouped_mm takes it, usually a view of (E, N, K) weights.
+// Temporaries are carved out of one allocation.
+struct Carver {
+    at::Tensor buf;
+    int64_t used = 0;
+    static int64_t up(int64_t n) { return (n + 255) / 256 * 256; }
+    char *take(int64_t n) {
+        char *const p = (char *)buf.data_ptr() + used;
+        used += up(n);
+        return p;
+    }
+};
+
+void grouped_linear_args(const at::Tensor &x, const at::Tensor &w, const at::Tensor &ends, const char *op) {
+    TORCH_CHECK(x.dim() == 2 && w.dim() == 3 && w.size(1) == x.size(1) && is_float(x.scalar_type()) && w.scalar_type() == x.scalar_type(), "gn_kernels::", op,
+                ": x ", x.sizes(), " ", x.scalar_type(), " and weight ", w.sizes(), " ", w.scalar_type(), " do not go together");
+    TORCH_CHECK(ends.scalar_type() == at::kInt && ends.dim() == 1 && ends.is_contiguous() && ends.size(0) == w.size(0), "gn_kernels::", op,
+                ": offs must be a contiguous 1-D int32 tensor with one end per expert");
+    TORCH_CHECK(w.device() == x.device() && ends.device() == x.device(), "gn_kernels::", op, ": all tensors must be on one device");
+}
+
+void quant_rows(const at::Tensor &x, int code, int64_t R, int64_t C, int64_t sr, char *q, char *s, void *st, const char *op) {
+    if (R == 0) return;
+    check(gnk_quantize_int8(x.data_ptr(), code, R, C, sr, 1, (int8_t *)q, C, 1, s, 1e-12f, 0, 0, 0, nullptr, 0, st), op);
+}
+
+at::Tensor grouped_linear_int8(const at::Tensor &x_in, const at::Tensor &w, const at::Tensor &ends) {
+    const char *op = "grouped_linear_int8";
+    grouped_linear_args(x_in, w, ends, op);
+    const at::Tensor x = x_in.stride(1) == 1 || x_in.size(1) == 1 ? x_in : x_in.contiguous();
+    const at::Tensor wt = w.transpose(1, 2).contiguous();                       // (E, N, K): no copy in the usual call
+    const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(2), es = x.element_size();
+    const int code = dtype_code(x.scalar_type(), op);
+    at::Tensor y = at::empty({T, N}, x.options());
+    if (K == 0) return y.zero_();
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    void *const st = stream_of(x);
+    // the operand copies' size depends on alignment only through the base, which the carver aligns
+    const int64_t nws = gnk_grouped_scaled_mm_rows_workspace_bytes(nullptr, nullptr, T, E, N, K, K, 1, N * K, 1, K);
+    Carver c{at::empty({Carver::up(T * K) + Carver::up(T * es) + Carver::up(E * N * K) + Carver::up(E * N * es) + nws + 256}, x.options().dtype(at::kByte))};
+    char *const xq = c.take(T * K), *const xs = c.take(T * es), *const wq = c.take(E * N * K), *const ws = c.take(E * N * es), *const scratch = c.take(nws);
+    quant_rows(x, code, T, K, x.stride(0), xq, xs, st, op);
+    quant_rows(wt, code, E * N, K, K, wq, ws, st, op);
+    check(gnk_grouped_scaled_mm_rows(xq, GNK_I8, wq, GNK_I8, y.data_ptr(), code, xs, ws, code, 0, (const int32_t *)ends.data_ptr(), T, E, N, K, K, 1, N * K, 1, K,
+                                     nws > 0 ? scratch : nullptr, nws, st),
+          op);
+    return y;
+}
+
+std::tuple<at::Tensor, at::Tensor> grouped_linear_int8_backward(const at::Tensor &g_in, const at::Tensor &x_in, const at::Tensor &w, const at::Tensor &ends, bool need_x,
+                                                                bool need_w) {
+    const char *op = "grouped_linear_int8_backward";
+    grouped_linear_args(x_in, w, ends, op);
+    TORCH_CHECK(g_in.dim() == 2 && g_in.size(0) == x_in.size(0) && g_in.size(1) == w.size(2) && g_in.scalar_type() == x_in.scalar_type() && g_in.device() == x_in.device(),
+                "gn_kernels::", op, ": gradient ", g_in.sizes(), " ", g_in.scalar_type(), " does not fit");
+    const at::Tensor g = g_in.contiguous(), x = x_in.contiguous();
+    const int64_t T = x.size(0), K = x.size(1), E = w.size(0), N = w.size(2), es = x.element_size();
+    const int code = dtype_code(x.scalar_type(), op);
+    const int32_t *const end = (const int32_t *)ends.data_ptr();
+    at::Tensor gx = at::empty({need_x ? T : 0, K}, x.options()), gw = at::empty({need_w ? E : 0, N, K}, x.options());
+    const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(x.device());
+    void *const st = stream_of(x);
+    auto quant_cols = [&](const at::Tensor &t, const int32_t *e, int64_t rows, int64_t cols, char *q, char *s, char *scratch, int64_t bytes) {
+        check(gnk_quantize_int8_grouped(t.data_ptr(), code, e, rows, E, cols, cols, 1, (int8_t *)q, s, 1e-12f, 0, 0, 0, bytes > 0 ? scratch : nullptr, bytes, st), op);
+    };
+    if (need_x && N == 0) gx.zero_();
+    if (need_x && N > 0) {
+        const at::Tensor wt = w.transpose(1, 2).contiguous();
+        const int64_t qws = gnk_quantize_int8_grouped_workspace_bytes(E * N, E, K);
+        const int64_t nws = gnk_grouped_scaled_mm_rows_workspace_bytes(nullptr, nullptr, T, E, K, N, N, 1, N * K, K, 1);
+        Carver c{at::empty({Carver::up(T * N) + Carver::up(T * es) + Carver::up(E * N * K) + Carver::up(E * K * es) + Carver::up(qws) + nws + 256}, x.options().dtype(at::kByte))};
+        char *const gq = c.take(T * N), *const gs = c.take(T * es), *const wq = c.take(E * N * K), *const ws = c.take(E * K * es), *const part = c.take(qws);
+        char *const scratch = c.take(nws);
+        quant_rows(g, code, T, N, N, gq, gs, st, op);
+        quant_cols(wt, nullptr, E * N, K, wq, ws, part, qws);                   // an expert's N rows are a group
+        check(gnk_grouped_scaled_mm_rows(gq, GNK_I8, wq, GNK_I8, gx.data_ptr(), code, gs, ws, code, 0, end, T, E, K, N, N, 1, N * K, K, 1,
+                                         nws > 0 ? scratch : nullptr, nws, st),
+              op);
+    }
+    if (need_w) {
+        const int64_t qg = gnk_quantize_int8_grouped_workspace_bytes(T, E, N), qx = gnk_quantize_int8_grouped_workspace_bytes(T, E, K);
+        const int64_t nws = gnk_grouped_scaled_mm_depth_workspace_bytes(nullptr, nullptr, T, N, K, 1, N, K, 1);
+        Carver c{at::empty({Carver::up(T * N) + Carver::up(E * N * es) + Carver::up(T * K) + Carver::up(E * K * es) + Carver::up(std::max(qg, qx)) + nws + 256},
+                           x.options().dtype(at::kByte))};
+        char *const gq = c.take(T * N), *const gs = c.take(E * N * es), *const xq = c.take(T * K), *const xs = c.take(E * K * es), *const part = c.take(std::max(qg, qx));
+        char *const scratch = c.take(nws);
+        quant_cols(g, end, T, N, gq, gs, part, qg);
+        quant_cols(x, end, T, K, xq, xs, part, qx);
+        check(gnk_grouped_scaled_mm_depth(gq, GNK_I8, xq, GNK_I8, gw.data_ptr(), code, gs, xs, code, 0, end, T, E, N, K, 1, N, K, 1, nws > 0 ? scratch : nullptr, nws, st),
+              op);
+    }
+    return {gx, gw};
+}
+
 at::Tensor orthogonalize(const at::Tensor &G_in, int64_t steps, double a, double b, double c, double eps) {
     const char *op = "orthogonalize";
     TORCH_CHECK(is_float(G_in.scalar_type()) && G_in.dim() >= 2, "gn_kernels::", op, ": unsupported input (shape ", G_in.sizes(), ", dtype ", G_in.scalar_type(), ")");
@@ -292,5 +387,7 @@ TORCH_LIBRARY_IMPL(gn_kernels, CUDA, m) {
     m.impl("grouped_scaled_mm", &grouped_scaled_mm);
     m.impl("grouped_scaled_mm_depth", &grouped_scaled_mm_depth);
     m.impl("quantize_int8_grouped", &quantize_int8_grouped);
+    m.impl("grouped_linear_int8", &grouped_linear_int8);
+    m.impl("grouped_linear_int8_backward", &grouped_linear_int8_backward);
     m.impl("orthogonalize", &orthogonalize);
 }

@@ -31,7 +31,8 @@ _lib = None
 # GNK_NO_TORCH_SHIM=1 keeps the Python implementations (A/B timing of the host path, and the tests' second leg).
 _SHIM_PATH = Path(__file__).resolve().parent / "libgnk_torch_ops.so"
 _SHIM_OPS = ("int8_mm", "scaled_mm", "scaled_mm_t", "tile_scaled_mm", "quantize_int8", "quantize_int8_rowwise_colmax", "quantize_int8_colwise_given",
-             "grouped_scaled_mm", "grouped_scaled_mm_depth", "quantize_int8_grouped", "orthogonalize")
+             "grouped_scaled_mm", "grouped_scaled_mm_depth", "quantize_int8_grouped", "grouped_linear_int8",
+             "grouped_linear_int8_backward", "orthogonalize")
 _shim_loaded = None
 
 

@@ -19,6 +19,11 @@ lib.define("grouped_scaled_mm(Tensor A, Tensor B, Tensor scale_A, Tensor scale_B
 lib.define("grouped_scaled_mm_depth(Tensor A, Tensor B, Tensor scale_A, Tensor scale_B, Tensor offs) -> Tensor")
 lib.define("quantize_int8_grouped(Tensor x, Tensor offs, bool stochastic_rounding, float eps, Tensor? rng=None) -> (Tensor, Tensor)")
 
+# `F.grouped_mm` on a mixed-precision weight (subclasses/mixed_precision.py) without stochastic rounding, one call per direction: x (T, K), w (E, K, N),
+# offs -> y, and grad_y -> (grad_x, grad_w (E, N, K)); a gradient that is not asked for comes back with no rows.
+lib.define("grouped_linear_int8(Tensor x, Tensor w, Tensor offs) -> Tensor")
+lib.define("grouped_linear_int8_backward(Tensor grad_y, Tensor x, Tensor w, Tensor offs, bool need_x, bool need_w) -> (Tensor, Tensor)")
+
 
 def grouped_scaled_mm(A: Tensor, B: Tensor, scale_A: Tensor, scale_B: Tensor, offs: Tensor) -> Tensor:
     """`scaled_mm` for every group of rows; group e holds rows offs[e - 1] .. offs[e] - 1 (offs[-1] = 0).
@@ -73,6 +78,17 @@ def _depth_meta(A: Tensor, B: Tensor, scale_A: Tensor, scale_B: Tensor, offs: Te
 @torch.library.impl(lib, "quantize_int8_grouped", "Meta")
 def _quantize_meta(x: Tensor, offs: Tensor, stochastic_rounding: bool, eps: float, rng: Tensor | None = None):
     return torch.empty(x.shape, dtype=torch.int8, device=x.device), x.new_empty((offs.shape[0], 1, x.shape[1]))
+
+
+@torch.library.impl(lib, "grouped_linear_int8", "Meta")
+def _linear_meta(x: Tensor, w: Tensor, offs: Tensor):
+    return x.new_empty((x.shape[0], w.shape[2]))
+
+
+@torch.library.impl(lib, "grouped_linear_int8_backward", "Meta")
+def _linear_backward_meta(grad_y: Tensor, x: Tensor, w: Tensor, offs: Tensor, need_x: bool, need_w: bool):
+    E, K, N = w.shape
+    return x.new_empty((x.shape[0] if need_x else 0, K)), x.new_empty((E if need_w else 0, N, K))
 
 
 def _check(op: str, A: Tensor, *others: Tensor) -> None:
@@ -130,3 +146,37 @@ def _quantize_hip(x: Tensor, offs: Tensor, stochastic_rounding: bool, eps: float
                                          int(stochastic_rounding), seed, offset, ws.data_ptr() if nws else None, nws, _cabi.stream_of(x))
     _cabi.check(rc, "quantize_int8_grouped")
     return q, scale
+
+
+def linear_forward(x: Tensor, w: Tensor, offs: Tensor, sr: bool) -> Tensor:
+    """y (T, N) of x (T, K) and w (E, K, N): x per row and w per (expert, n) in int8."""
+    E, K, N = w.shape
+    xq, xs = lib_ops.quantize_int8(x, 1, sr, 1e-12, draw_rng(sr))
+    wq, ws = lib_ops.quantize_int8(w.transpose(1, 2).reshape(E * N, K), 1, sr, 1e-12, draw_rng(sr))
+    return lib_ops.grouped_scaled_mm(xq, wq.view(E, N, K).transpose(1, 2), xs, ws.view(E, 1, N), offs)
+
+
+def linear_backward(grad_y: Tensor, x: Tensor, w: Tensor, offs: Tensor, need_x: bool, need_w: bool, sr: bool):
+    """(grad_x (T, K), grad_w (E, N, K)): grad_y per row with w per (expert, k); grad_y and x per (group, column)."""
+    E, K, N = w.shape
+    gx, gw = x.new_empty((0, K)), x.new_empty((0, N, K))
+    if need_x:
+        gq, gs = lib_ops.quantize_int8(grad_y, 1, sr, 1e-12, draw_rng(sr))
+        ends = torch.arange(1, E + 1, dtype=torch.int32, device=w.device) * N      # an expert's N rows are a group
+        wq, ws = lib_ops.quantize_int8_grouped(w.transpose(1, 2).reshape(E * N, K), ends, sr, 1e-12, draw_rng(sr))
+        gx = lib_ops.grouped_scaled_mm(gq, wq.view(E, N, K), gs, ws, offs)
+    if need_w:
+        xq, xs = lib_ops.quantize_int8_grouped(x, offs, sr, 1e-12, draw_rng(sr))
+        gq, gs = lib_ops.quantize_int8_grouped(grad_y, offs, sr, 1e-12, draw_rng(sr))
+        gw = lib_ops.grouped_scaled_mm_depth(gq.T, xq, gs.view(E, N, 1), xs, offs)
+    return gx, gw
+
+
+@_cabi.device_impl(lib, "grouped_linear_int8")
+def _linear_hip(x: Tensor, w: Tensor, offs: Tensor):
+    return linear_forward(x, w, offs, False)
+
+
+@_cabi.device_impl(lib, "grouped_linear_int8_backward")
+def _linear_backward_hip(grad_y: Tensor, x: Tensor, w: Tensor, offs: Tensor, need_x: bool, need_w: bool):
+    return linear_backward(grad_y, x, w, offs, need_x, need_w, False)

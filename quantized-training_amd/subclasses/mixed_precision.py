@@ -24,8 +24,10 @@ import torch.nn.functional as F
 import torch.utils._pytree as pytree
 from torch import Tensor, nn
 
-from gn_kernels import grouped_scaled_mm, quantize_int8_grouped, scaled_mm, scaled_mm_t
+from gn_kernels import grouped as _gop
 from gn_kernels import quantize as _qop
+from gn_kernels import scaled_mm, scaled_mm_t
+from gn_kernels._lib import lib_ops
 
 from .int8 import quantize_int8
 
@@ -56,6 +58,8 @@ _REWRAP_OPS = frozenset({
     aten.clone.default,
 })
 
+_VIEW_OPS = frozenset({aten.detach.default, aten.transpose.int})
+
 
 class MixedPrecisionLinearWeight(Tensor):
     """bf16 master weight whose F.linear runs in INT8."""
@@ -69,6 +73,13 @@ class MixedPrecisionLinearWeight(Tensor):
     def __init__(self, data: Tensor, config: MixedPrecisionConfig):
         self._data = data
         self.config = config
+
+    @classmethod
+    def _wrap(cls, data: Tensor, config: MixedPrecisionConfig):
+        """The constructor without its compiler guards."""
+        out = Tensor._make_wrapper_subclass(cls, data.shape, dtype=data.dtype, device=data.device)
+        out._data, out.config = data, config
+        return out
 
     def __tensor_flatten__(self):
         return ["_data"], [self.config]
@@ -109,6 +120,9 @@ class MixedPrecisionLinearWeight(Tensor):
 
     @classmethod
     def __torch_dispatch__(cls, func, types, args, kwargs):
+        # the two ops that every call of F.grouped_mm makes on its weight, without the tree walk (15 us each)
+        if func in _VIEW_OPS and not torch.compiler.is_compiling() and isinstance(args[0], cls) and args[0].ndim == 3 and not kwargs:
+            return cls._wrap(func(args[0]._data, *args[1:]), args[0].config)
         seen: list[MixedPrecisionConfig] = []
 
         def unwrap(w):
@@ -342,31 +356,22 @@ _GROUPED_MM = {f for f in (getattr(F, "grouped_mm", None), getattr(torch, "_grou
 class _Int8MixedPrecisionGroupedMM(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input: Tensor, weight: MixedPrecisionLinearWeight, offs: Tensor):
-        cfg, w = weight.config, weight._data
-        E, K, N = w.shape
-        wt = w.transpose(1, 2)                                    # (E, N, K), contiguous in the usual call
-        xq, xs = quantize_int8(input, cfg.stochastic_rounding, dim=1)
-        wq, ws = quantize_int8(wt.reshape(E * N, K), cfg.stochastic_rounding, dim=1)
+        w = weight._data
+        ctx.sr = weight.config.stochastic_rounding
         ctx.save_for_backward(input, w, offs)
-        ctx.config = cfg
-        return grouped_scaled_mm(xq, wq.view(E, N, K).transpose(1, 2), xs, ws.view(E, 1, N), offs)
+        if ctx.sr:
+            return _gop.linear_forward(input, w, offs, True)
+        return lib_ops.grouped_linear_int8(input, w, offs)
 
     @staticmethod
     def backward(ctx, grad_output):
         input, w, offs = ctx.saved_tensors
-        sr = ctx.config.stochastic_rounding
-        E, K, N = w.shape
-        grad_input = grad_weight = None
-        if ctx.needs_input_grad[0]:
-            gq, gs = quantize_int8(grad_output, sr, dim=1)
-            ends = torch.arange(N, E * N + 1, max(N, 1), dtype=torch.int32, device=w.device) if N else offs.new_zeros(E)
-            wq, ws = quantize_int8_grouped(w.transpose(1, 2).reshape(E * N, K), ends, sr)
-            grad_input = grouped_scaled_mm(gq, wq.view(E, N, K), gs, ws, offs)
-        if ctx.needs_input_grad[1]:
-            xq, xs = quantize_int8_grouped(input, offs, sr)
-            gq, gs = quantize_int8_grouped(grad_output, offs, sr)
-            grad_weight = grouped_scaled_mm(gq.T, xq, gs.view(E, N, 1), xs, offs).transpose(1, 2)      # stored (E, N, K), as the weight is
-        return grad_input, grad_weight, None
+        need_x, need_w, _ = ctx.needs_input_grad
+        if ctx.sr:
+            gx, gw = _gop.linear_backward(grad_output, input, w, offs, need_x, need_w, True)
+        else:
+            gx, gw = lib_ops.grouped_linear_int8_backward(grad_output, input, w, offs, need_x, need_w)
+        return gx if need_x else None, gw.transpose(1, 2) if need_w else None, None      # gw is stored (E, N, K), as the weight is
 
 
 def _grouped_mm(mat_a: Tensor, mat_b: Tensor, *, offs: Tensor | None = None, bias: Tensor | None = None, out_dtype: torch.dtype | None = None) -> Tensor:
