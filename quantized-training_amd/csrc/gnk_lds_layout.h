@@ -104,14 +104,19 @@ GNK_HD int gnk_mn64_frag16_offset(int rb, int t, int lane) {
 
 // =============================================================================================
 // 16-bit elements.  A K-major tile is byte for byte the 8-bit one (a lane's 16 bytes are 8 consecutive k of its row).  An MN-major tile is
-// [k][L bytes], L = 256 (128 columns, two-buffer kernel: 64 k-rows) or 512 (256 columns, one wave per SIMD: 32 k-rows per stage), read with
+// [k][L bytes], L = 128 or 256 (64 / 128 columns: 64 k-rows per step) or 512 (256 columns, one wave per SIMD: 32 k-rows per stage), read with
 // ds_read_b64_tr_b16: 16 lanes take 4 k-rows x 16 columns, so a half-wave (lane groups g, g + 1) touches k-rows 8 g + 0..3 and 8 g + 8..11 with
-// 32 bytes each; bits 0, 1 and 3 of k pick eight different 32-byte slots of the 256-byte bank window.  16-byte chunk c of k-row k at c ^ swz(k).
-GNK_HD int gnk_mn16_swz(int k) { return ((k & 3) << 1) | (((k >> 3) & 1) << 3); }
-template <int L> GNK_HD int gnk_mn16_offset(int k, int c) { return k * L + ((c ^ gnk_mn16_swz(k)) << 4); }
+// 32 bytes each; bits 0, 1 and 3 of k pick eight different 32-byte slots of the 256-byte bank window (L = 128: bit 0 does by itself, two k-rows
+// share a window).  16-byte chunk c of k-row k at c ^ swz(k).
+template <int L> GNK_HD int gnk_mn16_swz(int k) {
+    static_assert(L == 128 || L == 256 || L == 512, "16-bit MN-major tiles are 64, 128 or 256 columns wide");
+    if (L == 128) return (k & 2) | (((k >> 3) & 1) << 2);
+    return ((k & 3) << 1) | (((k >> 3) & 1) << 3);
+}
+template <int L> GNK_HD int gnk_mn16_offset(int k, int c) { return k * L + ((c ^ gnk_mn16_swz<L>(k)) << 4); }
 template <int L> GNK_HD void gnk_mn16_stage_src(int p, int &k, int &c) {
     k = p / (L / 16);
-    c = (p % (L / 16)) ^ gnk_mn16_swz(k);
+    c = (p % (L / 16)) ^ gnk_mn16_swz<L>(k);
 }
 // first of the two reads of the 16-column fragment at column rb, k-rows 32 ks + 8 (l >> 4) + 0..3; the second (+ 4..7) is 4 L further
 template <int L> GNK_HD int gnk_mn16_frag_offset(int rb, int ks, int lane) {

@@ -28,7 +28,7 @@ typedef short v4s __attribute__((ext_vector_type(4)));
 
 constexpr int PAD = 128;                     // rows and columns of every intermediate are padded to this
 constexpr float SX = 1024.0f, SS = 1024.0f;  // scales of X (after step 0) and S
-constexpr int MAX_PARTS = 64;                // partial sums of squares per matrix
+constexpr int MAX_PARTS = 256;               // partial sums of squares per matrix
 
 enum { SCALE = 0, POLY = 1 };                // epilogues: acc * f;  acc * f + D * g + (diagonal) h
 
@@ -48,15 +48,24 @@ struct Product {
 };
 
 // Tile of a workgroup: the XCDs take contiguous runs of tiles (matrices one after the other), each walked in strips of four tile rows.
-__device__ __forceinline__ void batch_tile(const Product &p, int &b, int &tm, int &tn) {
-    const int per = p.grid_m * p.grid_n, nwg = per * p.batch;
+// SYM: only the tiles on and above the diagonal, row by row; the others are their mirror images (store_mirror).
+template <bool SYM> __host__ __device__ __forceinline__ int tiles_of(const Product &p) { return SYM ? p.grid_m * (p.grid_m + 1) / 2 : p.grid_m * p.grid_n; }
+
+template <bool SYM> __device__ __forceinline__ void batch_tile(const Product &p, int &b, int &tm, int &tn) {
+    const int per = tiles_of<SYM>(p), nwg = per * p.batch;
     const int xcd = (int)blockIdx.x & 7, idx = (int)blockIdx.x >> 3, q = nwg >> 3, r = nwg & 7;
     const int wg = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
     b = wg / per;
-    const int in = wg - b * per;
-    const int width = 4 * p.grid_n, strip = in / width, first = strip * 4, gsz = min(p.grid_m - first, 4), rest = in - strip * width;
-    tm = first + rest % gsz;
-    tn = rest / gsz;
+    int in = wg - b * per;
+    if constexpr (SYM) {
+        tm = 0;
+        while (in >= p.grid_m - tm) in -= p.grid_m - tm++;
+        tn = tm + in;
+    } else {
+        const int width = 4 * p.grid_n, strip = in / width, first = strip * 4, gsz = min(p.grid_m - first, 4), rest = in - strip * width;
+        tm = first + rest % gsz;
+        tn = rest / gsz;
+    }
 }
 
 // acc (lane: row m, columns n .. n + 3) -> the stored value
@@ -84,98 +93,166 @@ __device__ __forceinline__ GemmParams store_params(const Product &p, int b) {
 
 __device__ __forceinline__ float factor(const Product &p, int b) { return p.fdev ? p.f * p.fdev[(int64_t)b * p.fstride] : p.f; }
 
-// ------------------------------------------------------------------------------ 128 x 128 tiles, two buffers
-template <bool KMAJOR> struct Stager16 {
+// The transpose of a wave's 16 MT x 64 results (fp16 output, rows m0 .., columns n0 ..; both inside the padded matrix), through its slice of LDS:
+// image [64 n][16 MT m], 16-byte chunk c of row n at c ^ 2 ((n >> 2) & 3), so that the four lane groups of a write land in different banks; rows of
+// 32 MT bytes go out whole.
+template <int MT> __device__ __forceinline__ void store_mirror(const Product &p, int b, const v4f (&acc)[MT][4], char *region, int lane, int64_t m0, int64_t n0) {
+    constexpr int PITCH = 32 * MT, CHUNKS = 2 * MT;
+    static_assert(MT >= 4, "the swizzle needs eight chunks per row");
+    if (m0 + 16 * MT > p.ext_a || n0 + 64 > p.ext_b) return;                  // padding tiles beyond the matrix (extents are multiples of 128)
+    const int g = lane >> 4, ml = lane & 15;
+    asm volatile("" ::: "memory");           // behind the wave's earlier reads of the slice
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int n = 16 * j + 4 * g + r, c = (2 * i + (ml >> 3)) ^ (2 * g);
+                *(GNK_LDS _Float16 *)(GNK_LDS char *)(region + n * PITCH + 16 * c + 2 * (ml & 7)) = (_Float16)acc[i][j][r];
+            }
+    char *const C = (char *)p.C + b * p.bc;
+#pragma unroll
+    for (int u = 0; u < CHUNKS; ++u) {                                         // 64 rows x CHUNKS chunks over 64 lanes
+        const int e = u * 64 + lane, n = e / CHUNKS, c = e % CHUNKS;
+        const v4i v = *(const GNK_LDS v4i *)(const GNK_LDS char *)(region + n * PITCH + 16 * (c ^ (2 * ((n >> 2) & 3))));
+        gnk_store16_out(C + 2 * ((n0 + n) * p.N + m0) + 16 * c, v);
+    }
+}
+
+// ------------------------------------------------------------------------------ tiles of 128 or 64 with a ring of LDS stages
+// This wave's pieces of one operand's 64-k step (BM rows x 128 bytes, or 64 k-rows x 2 BM bytes)
+template <bool KMAJOR, int BM> struct Stager16 {
+    static constexpr int NP = BM / 32;
     const char *base;
-    unsigned off[4];
+    unsigned off[NP];
     int64_t step;
     __device__ __forceinline__ void init(const char *ptr, int64_t ld, int64_t r0, int wave, int lane) {
         base = KMAJOR ? ptr + r0 * ld : ptr + 2 * r0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < NP; ++i) {
             const int p = (i * 4 + wave) * 64 + lane;
             int r, c;
             if constexpr (KMAJOR) gnk_kmaj_stage_src(p, r, c);
-            else gnk_mn16_stage_src<256>(p, r, c);
+            else gnk_mn16_stage_src<2 * BM>(p, r, c);
             off[i] = (unsigned)(r * ld + 16 * c);
         }
         step = KMAJOR ? 128 : 64 * ld;
     }
     __device__ __forceinline__ void issue(char *tile, int wave) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < NP; ++i)
             __builtin_amdgcn_global_load_lds((const GNK_GLOBAL void *)(base + off[i]), (GNK_LDS void *)(tile + (i * 4 + wave) * 1024), 16, 0, 0);
         base += step;
     }
 };
 
-template <bool KMAJOR> __device__ __forceinline__ v8h frag16(const char *tile, int rb, int ks, int lane) {
+template <bool KMAJOR, int BM> __device__ __forceinline__ v8h frag16(const char *tile, int rb, int ks, int lane) {
     v4i v;
     if constexpr (KMAJOR) {
         v = *(const GNK_LDS v4i *)(const GNK_LDS char *)(tile + gnk_kmaj_frag_offset(rb, ks, lane));
     } else {
-        const int o = gnk_mn16_frag_offset<256>(rb, ks, lane);
+        const int o = gnk_mn16_frag_offset<2 * BM>(rb, ks, lane);
         const v2i lo = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((GNK_LDS v4s *)(tile + o)));
-        const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((GNK_LDS v4s *)(tile + o + 4 * 256)));
+        const v2i hi = __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((GNK_LDS v4s *)(tile + o + 8 * BM)));
         v = (v4i){lo[0], lo[1], hi[0], hi[1]};
     }
     return __builtin_bit_cast(v8h, v);
 }
 
-template <bool AK, bool BK, int EPI>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) product128_kernel(const Product p) {
+// BM = 128: 2 x 2 waves of 64 x 64, two stages (64 KiB: two workgroups per CU).  BM = 64: 2 x 2 waves of 32 x 32 would halve the fragment reads, but the
+// stores want 64 columns per wave: 4 x 1 waves of 16 x 64; four stages (64 KiB) because few tiles are bound by the latency of a step, not by its work.
+template <int BM> struct RingShape {
+    static constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1, MT = BM / WM / 16, NST = BM == 128 ? 2 : 4, OPER = BM * 128, STAGE = 2 * OPER;
+    static constexpr int LDS = NST * STAGE;
+};
+
+template <int BM, bool AK, bool BK, int EPI, bool SYM>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) product_ring_kernel(const Product p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    typedef GemmCfg<128, 128, 2, 2, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;     // fp32 accumulators and the epilogue's maps
-    constexpr int TILE = 128 * 128;                                          // bytes of one operand's 64-k step
+    typedef RingShape<BM> R;
+    typedef GemmCfg<BM, BM, R::WM, R::WN, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;     // fp32 accumulators and the epilogue's maps
+    constexpr int MT = R::MT, NST = R::NST, PIECES = 2 * BM / 32;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave >> 1, wn = wave & 1;
+    const int wm = wave / R::WN, wn = wave % R::WN;
     int b, tm, tn;
-    batch_tile(p, b, tm, tn);
-    const int64_t m0 = (int64_t)tm * 128, n0 = (int64_t)tn * 128;
-    Stager16<AK> sa;
-    Stager16<BK> sb;
+    batch_tile<SYM>(p, b, tm, tn);
+    const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BM;
+    Stager16<AK, BM> sa;
+    Stager16<BK, BM> sb;
     sa.init(p.A + b * p.ba, p.lda, m0, wave, lane);
     sb.init(p.B + b * p.bb, p.ldb, n0, wave, lane);
-    v4f acc[4][4];
+    v4f acc[MT][4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-    char *const As = smem, *const Bs = smem + 2 * TILE;
     const int nk = (int)(p.K / 64);
-    sa.issue(As, wave);
-    sb.issue(Bs, wave);
+    for (int t = 0; t < NST - 1 && t < nk; ++t) {
+        sa.issue(smem + t * R::STAGE, wave);
+        sb.issue(smem + t * R::STAGE + R::OPER, wave);
+    }
     for (int t = 0; t < nk; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        // stage t has landed; t + 1 .. t + NST - 2 may stay in flight
+        if (t + NST - 2 < nk) asm volatile("s_waitcnt vmcnt(%0)" : : "i"((NST - 2) * PIECES) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        const int cur = (t & 1) * TILE, nxt = TILE - cur;
-        if (t + 1 < nk) {
-            sa.issue(As + nxt, wave);
-            sb.issue(Bs + nxt, wave);
+        char *const As = smem + (t % NST) * R::STAGE, *const Bs = As + R::OPER;
+        if (t + NST - 1 < nk) {                                        // into the buffer of stage t - 1, which every wave has read
+            char *const next = smem + ((t + NST - 1) % NST) * R::STAGE;
+            sa.issue(next, wave);
+            sb.issue(next + R::OPER, wave);
         }
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
-            v8h fa[4], fb[4];
+            v8h fa[MT], fb[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) fb[j] = frag16<BK>(Bs + cur, wn * 64 + 16 * j, ks, lane);
+            for (int j = 0; j < 4; ++j) fb[j] = frag16<BK, BM>(Bs, wn * 64 + 16 * j, ks, lane);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fa[i] = frag16<AK>(As + cur, wm * 64 + 16 * i, ks, lane);
+            for (int i = 0; i < MT; ++i) fa[i] = frag16<AK, BM>(As, wm * 16 * MT + 16 * i, ks, lane);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < MT; ++i)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[j], fa[i], acc[i][j], 0, 0, 0);
         }
     }
     const float f = factor(p, b);
     const char *D = p.D + b * p.bd;
+    const int64_t mw = m0 + wm * 16 * MT, nw = n0 + wn * 64;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, D, f, acc[i][j], m0 + wm * 64 + 16 * i + (lane & 15), n0 + wn * 64 + 16 * j + 4 * (lane >> 4));
+        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, D, f, acc[i][j], mw + 16 * i + (lane & 15), nw + 16 * j + 4 * (lane >> 4));
     __syncthreads();
     const GemmParams g = store_params(p, b);
-    run_epilogue<Cfg>(g, acc, nullptr, smem, wave, lane, m0 + wm * 64, n0 + wn * 64);
+    run_epilogue<Cfg>(g, acc, nullptr, smem, wave, lane, mw, nw);
+    if constexpr (SYM) {
+        if (tm != tn) {
+            if constexpr (MT >= 4) {
+                store_mirror<MT>(p, b, acc, smem + R::LDS / 2 + wave * (64 * 32 * MT), lane, mw, nw);
+            } else {
+                // 16 rows per wave: transposed rows of 32 bytes would waste the stores; the four waves put theirs side by side first
+                char *const T = smem + R::LDS / 2;                     // [64 n][64 m] fp16, rows of 128 bytes, 16-byte chunk c at c ^ (n & 7)
+                const int gq = lane >> 4, ml = lane & 15;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int n = 16 * j + 4 * gq + r, c = (2 * wave + (ml >> 3)) ^ (n & 7);
+                        *(GNK_LDS _Float16 *)(GNK_LDS char *)(T + n * 128 + 16 * c + 2 * (ml & 7)) = (_Float16)acc[0][j][r];
+                    }
+                __syncthreads();
+                char *const C = (char *)p.C + b * p.bc;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int e = u * 256 + (int)threadIdx.x, n = e >> 3, c = e & 7;
+                    const v4i v = *(const GNK_LDS v4i *)(const GNK_LDS char *)(T + n * 128 + 16 * (c ^ (n & 7)));
+                    gnk_store16_out(C + 2 * ((n0 + n) * p.N + m0) + 16 * c, v);
+                }
+            }
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------ 256 x 256 tiles, one wave per SIMD (gnk_gemm_w4.h)
@@ -215,7 +292,7 @@ template <int H, int I> __device__ __forceinline__ void fetch_row(v4f (&acc)[8][
 
 // columns 64 H .. 64 H + 63 of the wave tile: accumulators -> values -> memory
 template <class Cfg, int EPI, int H>
-__device__ __forceinline__ void finish_half(const Product &p, const GemmParams &g, const char *D, float f, char *smem, int wave, int lane, int64_t mw, int64_t nw) {
+__device__ __forceinline__ void finish_half(const Product &p, const GemmParams &g, int b, bool mirror, const char *D, float f, char *smem, int wave, int lane, int64_t mw, int64_t nw) {
     v4f acc[8][4];
     fetch_row<H, 0>(acc); fetch_row<H, 1>(acc); fetch_row<H, 2>(acc); fetch_row<H, 3>(acc);
     fetch_row<H, 4>(acc); fetch_row<H, 5>(acc); fetch_row<H, 6>(acc); fetch_row<H, 7>(acc);
@@ -224,9 +301,10 @@ __device__ __forceinline__ void finish_half(const Product &p, const GemmParams &
 #pragma unroll
         for (int j = 0; j < 4; ++j) finish_value<EPI>(p, D, f, acc[i][j], mw + 16 * i + (lane & 15), nw + 64 * H + 16 * j + 4 * (lane >> 4));
     run_epilogue<Cfg>(g, acc, nullptr, smem, wave * 2 + H, lane, mw, nw + 64 * H);
+    if (mirror) store_mirror<8>(p, b, acc, smem + (wave * 2 + H) * 16384, lane, mw, nw + 64 * H);     // the same slice: a wave's LDS accesses stay in order
 }
 
-template <bool AK, bool BK, int EPI>
+template <bool AK, bool BK, int EPI, bool SYM>
 __global__ void __launch_bounds__(256) product256_kernel(const Product p) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmCfg<256, 256, 2, 4, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;      // the epilogue's maps: 128 x 64 halves of a wave's 128 x 128
@@ -234,7 +312,7 @@ __global__ void __launch_bounds__(256) product256_kernel(const Product p) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
     int b, tm, tn;
-    batch_tile(p, b, tm, tn);
+    batch_tile<SYM>(p, b, tm, tn);
     const int64_t m0 = (int64_t)tm * 256, n0 = (int64_t)tn * 256;
     StagerW4H<AK> sa;
     StagerW4H<BK> sb;
@@ -265,41 +343,76 @@ __global__ void __launch_bounds__(256) product256_kernel(const Product p) {
     const char *D = p.D + b * p.bd;
     const GemmParams g = store_params(p, b);
     const int64_t mw = m0 + wm * 128, nw = n0 + wn * 128;
-    finish_half<Cfg, EPI, 0>(p, g, D, f, smem, wave, lane, mw, nw);
-    finish_half<Cfg, EPI, 1>(p, g, D, f, smem, wave, lane, mw, nw);
+    const bool mirror = SYM && tm != tn;
+    finish_half<Cfg, EPI, 0>(p, g, b, mirror, D, f, smem, wave, lane, mw, nw);
+    finish_half<Cfg, EPI, 1>(p, g, b, mirror, D, f, smem, wave, lane, mw, nw);
 }
 
 // ------------------------------------------------------------------------------ sums of squares, conversion
-template <int DT> __device__ __forceinline__ float load1(const void *p, int64_t i) { return gnk_load_scalar<DT>(p, i); }
-
-template <int DT>
-__global__ void __launch_bounds__(256) square_sum_kernel(const void *__restrict__ G, double *__restrict__ parts, int64_t numel, int nparts) {
-    // fp64: the squares of any fp32 fit, and nothing is lost on the way
-    const int64_t b = blockIdx.y, per = (numel + nparts - 1) / nparts, i0 = (int64_t)blockIdx.x * per, i1 = i0 + per < numel ? i0 + per : numel;
-    double s = 0.0;
-    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256) {
-        const double v = load1<DT>(G, b * numel + i);
-        s += v * v;
-    }
+// V consecutive elements as floats: one 16-byte load, or a single element
+template <int DT, int V> __device__ __forceinline__ void load_floats(const void *p, int64_t i, float (&f)[V]) {
+    if constexpr (V == 1) {
+        f[0] = gnk_load_scalar<DT>(p, i);
+    } else if constexpr (DT == GNK_F32) {
+        const v4f v = *(const v4f *)((const float *)p + i);
+        f[0] = v[0]; f[1] = v[1]; f[2] = v[2]; f[3] = v[3];
+    } else {
+        const v4i v = *(const v4i *)((const unsigned short *)p + i);
 #pragma unroll
-    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+        for (int k = 0; k < 4; ++k) {
+            const unsigned w = (unsigned)v[k];
+            f[2 * k] = gnk_raw_to_f32<DT>(w & 0xffffu);
+            f[2 * k + 1] = gnk_raw_to_f32<DT>(w >> 16);
+        }
+    }
+}
+template <int DT> constexpr int VEC = DT == GNK_F32 ? 4 : 8;
+
+// Partial sums of squares: HBM-bound.  fp64: the squares of any fp32 fit, and nothing is lost on the way.
+template <int DT, int V>
+__global__ void __launch_bounds__(256) square_sum_kernel(const void *__restrict__ G, double *__restrict__ parts, int64_t numel, int nparts) {
+    const int64_t b = blockIdx.y, words = numel / V, per = (words + nparts - 1) / nparts, i0 = (int64_t)blockIdx.x * per, i1 = i0 + per < words ? i0 + per : words;
+    double s[4] = {0.0, 0.0, 0.0, 0.0};
+    for (int64_t i = i0 + threadIdx.x; i < i1; i += 256 * 4) {
+        float f[4][V];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {                                 // four loads in flight; past the end zeros
+#pragma unroll
+            for (int k = 0; k < V; ++k) f[u][k] = 0.0f;
+            if (i + 256 * u < i1) load_floats<DT, V>(G, b * numel + (i + 256 * u) * V, f[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int k = 0; k < V; ++k) s[u] = fma((double)f[u][k], (double)f[u][k], s[u]);
+    }
+    double t = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+    for (int d = 32; d; d >>= 1) t += __shfl_xor(t, d, 64);
     __shared__ double red[4];
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
     __syncthreads();
     if (threadIdx.x == 0) parts[b * nparts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// fac[b] = {factor of step 0's S, factor of step 0's update}: what takes G 2^p back to X_0
-template <int DT>
+// G 2^p as fp16, padded; fac[b] = {factor of step 0's S, factor of step 0's update}: what takes G 2^p back to X_0.  HBM-bound.
+template <int DT, int V>
 __global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G, unsigned short *__restrict__ X, const double *__restrict__ parts, float *__restrict__ fac,
                                                       int64_t rows, int64_t cols, int64_t rows_p, int64_t cols_p, int nparts, float eps) {
     const int64_t b = blockIdx.y;
-    double sum = 0.0;
-    for (int k = 0; k < nparts; ++k) sum += parts[b * nparts + k];      // every block adds in the same order
-    const double norm = sqrt(sum);
+    __shared__ double total;
+    if (threadIdx.x < 64) {                                           // every block adds in the same order
+        double t = 0.0;
+        for (int k = threadIdx.x; k < nparts; k += 64) t += parts[b * nparts + k];
+#pragma unroll
+        for (int d = 32; d; d >>= 1) t += __shfl_xor(t, d, 64);
+        if (threadIdx.x == 0) total = t;
+    }
+    __syncthreads();
+    const double norm = sqrt(total);
     int p = 0;
     double inv = 1.0 / (norm > (double)eps ? norm : (double)eps);
-    const bool finite = norm < 1.0e300;                                  // false for NaN and Inf: every output becomes NaN through the factors
+    const bool finite = norm < 1.0e300;                                // false for NaN and Inf: every output becomes NaN through the factors
     if (finite && norm > 0.0) p = 14 - ilogb(norm);
     if (!finite) inv = __builtin_nan("");
     if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -307,23 +420,42 @@ __global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G
         fac[2 * b] = (float)(x0 * x0);
         fac[2 * b + 1] = (float)x0;
     }
-    const int64_t quads = rows_p * cols_p / 4;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < quads; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / (cols_p / 4), c = (i - r * (cols_p / 4)) * 4;
-        float v[4];
+    const int64_t per_row = cols_p / 8, octets = rows_p * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < octets; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+        float v[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            v[k] = finite && r < rows && c + k < cols ? load1<DT>(G, (b * rows + r) * cols + c + k) : 0.0f;
-            v[k] = ldexpf(v[k], p);
+        for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+        if (finite && r < rows && c < cols) {
+            const int64_t at = (b * rows + r) * cols + c;
+            if constexpr (V > 1) {                                     // cols is a multiple of V
+#pragma unroll
+                for (int h = 0; h < 8 / V; ++h) {
+                    if (c + h * V < cols) {
+                        float w[V];
+                        load_floats<DT, V>(G, at + h * V, w);
+#pragma unroll
+                        for (int k = 0; k < V; ++k) v[h * V + k] = w[k];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    if (c + k < cols) v[k] = gnk_load_scalar<DT>(G, at + k);
+            }
         }
-        const v2i o = {(int)gnk_pack2_f16(v[0], v[1]), (int)gnk_pack2_f16(v[2], v[3])};
-        *(v2i *)(X + (b * rows_p + r) * cols_p + c) = o;
+        v4i o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = (int)gnk_pack2_f16(ldexpf(v[2 * k], p), ldexpf(v[2 * k + 1], p));
+        *(v4i *)(X + (b * rows_p + r) * cols_p + c) = o;
     }
 }
 
-template <int BM, bool AK, bool BK, int EPI> int launch(const Product &p0, hipStream_t st) {
-    constexpr int LDS_TOTAL = BM == 256 ? 131072 : 65536;
-    auto *const kernel = BM == 256 ? product256_kernel<AK, BK, EPI> : product128_kernel<AK, BK, EPI>;
+template <int BM, bool AK, bool BK, int EPI, bool SYM> int launch(const Product &p0, hipStream_t st) {
+    constexpr int LDS_TOTAL = BM == 256 ? 131072 : RingShape<BM == 256 ? 128 : BM>::LDS;
+    void (*kernel)(const Product);
+    if constexpr (BM == 256) kernel = product256_kernel<AK, BK, EPI, SYM>;
+    else kernel = product_ring_kernel<BM, AK, BK, EPI, SYM>;
     Product p = p0;
     p.grid_m = (int)((p.ext_a + BM - 1) / BM);
     p.grid_n = (int)((p.ext_b + BM - 1) / BM);
@@ -335,7 +467,7 @@ template <int BM, bool AK, bool BK, int EPI> int launch(const Product &p0, hipSt
             return gnk_fail(GNK_ERR_LAUNCH, "orthogonalize: cannot reserve LDS");
         attr_set[dev].store(true, std::memory_order_release);
     }
-    const int64_t blocks = (int64_t)p.grid_m * p.grid_n * p.batch;
+    const int64_t blocks = (int64_t)tiles_of<SYM>(p) * p.batch;
     if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), LDS_TOTAL, st, p);
     return gnk_check_launch("orthogonalize");
@@ -368,18 +500,33 @@ Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
     return p;
 }
 
-template <int EPI> int run_product(bool ak, bool bk, const Product &p, hipStream_t st) {
-    // the cost model of the dense products (gnk_api.hip): us per round of workgroups, one 256 x 256 or two 128 x 128 per CU; a step is 64 k
+template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p, hipStream_t st) {
+    // the cost model of the dense products (gnk_api.hip): us per round of workgroups, one 256 x 256 or two smaller ones per CU; a step is 64 k
     const double cus = (double)gnk_num_cus(), ks = (double)p.K / 64.0;
-    const double t256 = ceil((double)(((p.ext_a + 255) / 256) * ((p.ext_b + 255) / 256) * p.batch) / cus) * (12.0 + 1.08 * ks);
-    const double t128 = ceil((double)((p.ext_a / 128) * (p.ext_b / 128) * p.batch) / (2.0 * cus)) * (6.0 + 1.0 * ks);
-    const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1 and 5 choose between the two here as well
-    if (forced != 1 && (forced == 5 || t256 <= t128)) {
-        if (ak) return bk ? launch<256, true, true, EPI>(p, st) : launch<256, true, false, EPI>(p, st);
-        return launch<256, false, false, EPI>(p, st);
+    auto tiles = [&](int64_t bm) {
+        const double gm = (double)((p.ext_a + bm - 1) / bm), gn = (double)((p.ext_b + bm - 1) / bm);
+        return (SYM ? gm * (gm + 1) / 2 : gm * gn) * (double)p.batch;
+    };
+    const double t256 = ceil(tiles(256) / cus) * (12.0 + 1.3 * ks), t128 = ceil(tiles(128) / (2.0 * cus)) * (6.0 + 1.0 * ks);
+    const double t64 = ceil(tiles(64) / (2.0 * cus)) * (4.0 + 0.4 * ks);
+    const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1, 5 and 6 force the 128, 256 and 64 tiles here as well
+    if (forced == 6 || (forced != 1 && forced != 5 && t64 <= t128 && t64 <= t256)) return launch<64, AK, BK, EPI, SYM>(p, st);
+    if (forced == 5 || (forced != 1 && t256 <= t128)) return launch<256, AK, BK, EPI, SYM>(p, st);
+    return launch<128, AK, BK, EPI, SYM>(p, st);
+}
+
+template <int DT> int read_input(const void *G, char *X, double *parts, float *fac, int64_t batch, int64_t rows, int64_t cols, const Plan &pl, float eps, hipStream_t st) {
+    const dim3 g1((unsigned)pl.nparts, (unsigned)batch);
+    const int64_t octets = pl.rp * pl.cp / 8, want = (octets + 255) / 256;
+    const dim3 g2((unsigned)(want < 1024 ? want : 1024), (unsigned)batch);
+    if (cols % VEC<DT> == 0 && ((uintptr_t)G & 15) == 0) {
+        hipLaunchKernelGGL((square_sum_kernel<DT, VEC<DT>>), g1, dim3(256), 0, st, G, parts, rows * cols, pl.nparts);
+        hipLaunchKernelGGL((convert_kernel<DT, VEC<DT>>), g2, dim3(256), 0, st, G, (unsigned short *)X, parts, fac, rows, cols, pl.rp, pl.cp, pl.nparts, eps);
+    } else {
+        hipLaunchKernelGGL((square_sum_kernel<DT, 1>), g1, dim3(256), 0, st, G, parts, rows * cols, pl.nparts);
+        hipLaunchKernelGGL((convert_kernel<DT, 1>), g2, dim3(256), 0, st, G, (unsigned short *)X, parts, fac, rows, cols, pl.rp, pl.cp, pl.nparts, eps);
     }
-    if (ak) return bk ? launch<128, true, true, EPI>(p, st) : launch<128, true, false, EPI>(p, st);
-    return launch<128, false, false, EPI>(p, st);
+    return gnk_check_launch("orthogonalize");
 }
 
 }  // namespace
@@ -411,19 +558,9 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
     float *const fac = (float *)(ws + pl.off_fac);
     char *X = ws + pl.off_x0, *Xn = ws + pl.off_x1;
     char *const S = ws + pl.off_s, *const Q = ws + pl.off_q;
-    const dim3 g1((unsigned)pl.nparts, (unsigned)batch);
-    const int64_t quads = pl.rp * pl.cp / 4, wantb = (quads + 255) / 256;
-    const dim3 g2((unsigned)(wantb < 512 ? wantb : 512), (unsigned)batch);
-#define GNK_ORTHO_IN(DT)                                                                                                                              \
-    do {                                                                                                                                              \
-        hipLaunchKernelGGL((square_sum_kernel<DT>), g1, dim3(256), 0, st, G, parts, rows * cols, pl.nparts);                                          \
-        hipLaunchKernelGGL((convert_kernel<DT>), g2, dim3(256), 0, st, G, (unsigned short *)X, parts, fac, rows, cols, pl.rp, pl.cp, pl.nparts, eps); \
-    } while (0)
-    if (g_dtype == GNK_BF16) GNK_ORTHO_IN(GNK_BF16);
-    else if (g_dtype == GNK_F16) GNK_ORTHO_IN(GNK_F16);
-    else GNK_ORTHO_IN(GNK_F32);
-#undef GNK_ORTHO_IN
-    rc = gnk_check_launch(name);
+    rc = g_dtype == GNK_BF16 ? read_input<GNK_BF16>(G, X, parts, fac, batch, rows, cols, pl, eps, st)
+         : g_dtype == GNK_F16 ? read_input<GNK_F16>(G, X, parts, fac, batch, rows, cols, pl, eps, st)
+                              : read_input<GNK_F32>(G, X, parts, fac, batch, rows, cols, pl, eps, st);
     if (rc) return rc;
 
     const bool wide = rows <= cols;
@@ -443,7 +580,7 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.f = it == 0 ? SS : SS / (SX * SX);
         p.fdev = it == 0 ? fac : nullptr;
         p.out_dtype = GNK_F16;
-        rc = run_product<SCALE>(wide, wide, p, st);
+        rc = wide ? run_product<true, true, SCALE, true>(p, st) : run_product<false, false, SCALE, true>(p, st);
         if (rc) return rc;
         // Q = a I + b S + c S^2
         p.A = p.B = S; p.ba = p.bb = pl.s_bytes; p.lda = p.ldb = lds;
@@ -452,7 +589,7 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.K = lo;
         p.f = c * sq / (SS * SS); p.g = b * sq / SS; p.h = a * sq;
         p.fdev = nullptr;
-        rc = run_product<POLY>(true, true, p, st);
+        rc = run_product<true, true, POLY, true>(p, st);
         if (rc) return rc;
         // X <- Q X or X Q
         const bool last = it + 1 == steps;
@@ -466,7 +603,7 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.out_dtype = last ? out_dtype : GNK_F16;
         p.f = (last ? 1.0f : SX) / (it == 0 ? sq : sq * SX);
         p.fdev = it == 0 ? fac + 1 : nullptr;
-        rc = run_product<SCALE>(true, !wide, p, st);
+        rc = wide ? run_product<true, false, SCALE, false>(p, st) : run_product<true, true, SCALE, false>(p, st);
         if (rc) return rc;
         char *const t = X; X = Xn; Xn = t;
     }

@@ -64,7 +64,7 @@ def compare(got, G, **kw):
     assert err <= tol, f"{err:.3e} off, tolerance {tol:.3e}, norm {want.norm():.3e}"
 
 
-@pytest.fixture(params=[-1, 1, 5], ids=["auto", "tile128", "tile256w4"])
+@pytest.fixture(params=[-1, 1, 5, 6], ids=["auto", "tile128", "tile256w4", "tile64"])
 def forced(request):
     L = _cabi.load()
     old = L.gnk_set_gemm_variant(request.param)
@@ -72,7 +72,7 @@ def forced(request):
     L.gnk_set_gemm_variant(old)
 
 
-@pytest.mark.parametrize("m,n", [(1, 1), (1, 70), (70, 1), (2, 3), (16, 16), (127, 129), (128, 128), (129, 127), (255, 300), (300, 257), (333, 999), (999, 333), (640, 384)])
+@pytest.mark.parametrize("m,n", [(1, 1), (1, 70), (70, 1), (2, 3), (16, 16), (127, 129), (128, 128), (129, 127), (255, 300), (300, 257), (333, 999), (999, 333), (640, 384), (520, 900), (1100, 700)])
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 def test_shapes(forced, m, n, dt):
     G = matrix(m, n, dt, seed=m + n)
