@@ -233,6 +233,130 @@ template <int DT, int VEC> __device__ __forceinline__ void floats_of(const v4i &
     }
 }
 
+// divisors of VEC columns from their maxima (fp32 bit patterns), and the scales
+template <int DT, int VEC>
+__device__ __forceinline__ bool divisors(const unsigned *amax, float eps, GnkDivisor (&dv)[VEC], void *scale, int64_t at, bool write) {
+    bool fast = true;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const float s = __fmul_rn(__uint_as_float(amax[j]), GQ_INV127);
+        dv[j].set(gnk_clamp_min_nan(s, eps));
+        fast = fast && dv[j].ok();
+        if (write) gnk_store_scalar_rt(scale, DT, at + j, s);
+    }
+    return fast;
+}
+
+// VEC elements of row r from column col0 on: quantized and stored
+template <int DT, int VEC, bool SR>
+__device__ __forceinline__ void quant_store(const v4i &word, int64_t r, int64_t col0, int64_t C, const GnkDivisor (&dv)[VEC], bool fast, int8_t *__restrict__ q,
+                                            unsigned long long seed, unsigned long long offset) {
+    float f[VEC];
+    floats_of<DT, VEC>(word, f);
+    int qi[VEC];
+    float u[VEC];
+    if constexpr (SR) {
+        const unsigned long long idx0 = (unsigned long long)(r * C + col0);
+        if (VEC > 1 && ((idx0 + offset) & 3ull) == 0) {      // one Philox block per four elements
+#pragma unroll
+            for (int h = 0; h < VEC / 4; ++h) {
+                float w[4];
+                gnk_sr_uniform4(seed, offset, idx0 + 4 * h, w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) u[4 * h + k] = w[k];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) u[j] = gnk_sr_uniform(seed, offset, idx0 + j);
+        }
+    }
+    if (fast) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) qi[j] = SR ? gnk_sr_clip_i8(dv[j].quot(f[j]), u[j]) : gnk_rne_clip_i8(dv[j].quot(f[j]));
+    } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) qi[j] = SR ? gnk_sr_clip_i8(f[j] / dv[j].d, u[j]) : gnk_rne_clip_i8_any(f[j] / dv[j].d);
+    }
+    int8_t *dst = q + r * C + col0;
+    if constexpr (VEC == 8) {
+        v2i o;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            o[h] = (qi[4 * h] & 0xff) | ((qi[4 * h + 1] & 0xff) << 8) | ((qi[4 * h + 2] & 0xff) << 16) | (int)((unsigned)(qi[4 * h + 3] & 0xff) << 24);
+        __builtin_nontemporal_store(o, (v2i *)dst);
+    } else if constexpr (VEC == 4) {
+        *(int *)dst = (qi[0] & 0xff) | ((qi[1] & 0xff) << 8) | ((qi[2] & 0xff) << 16) | (int)((unsigned)(qi[3] & 0xff) << 24);
+    } else {
+        dst[0] = (int8_t)qi[0];
+    }
+}
+
+// Small calls (T <= GQ_ONCE_ROWS): one workgroup takes a group's CL * VEC columns from the maximum to the last store -- one launch, no partial maxima, no
+// search for its rows.  A thread keeps its first eight rows in registers; a group with more is read again from L2.
+constexpr int64_t GQ_ONCE_ROWS = 2048;
+
+template <int DT, int VEC, int CL, bool SR>
+__global__ void __launch_bounds__(256)
+group_quant_once_kernel(const char *__restrict__ x, int8_t *__restrict__ q, void *__restrict__ scale, const int *__restrict__ ends, int64_t T, int64_t E, int64_t C,
+                        int64_t row_bytes, int64_t col_bytes, float eps, unsigned long long seed, unsigned long long offset) {
+    constexpr int RL = 256 / CL, KEEP = 8;
+    const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
+    const int64_t col0 = ((int64_t)blockIdx.x * CL + cl) * VEC, e = blockIdx.y;
+    int lo, hi;
+    lane_group(ends, E, T, e, 0, lo, hi);
+    if (e == E) {                                // rows of no group
+        if (col0 < C)
+            for (int64_t r = lo + rl; r < hi; r += RL)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) q[r * C + col0 + j] = 0;
+        return;
+    }
+    const char *src = x + (col0 < C ? col0 : 0) * col_bytes;
+    unsigned mw[4] = {0u, 0u, 0u, 0u};
+    v4i keep[KEEP];
+    for (int64_t r0 = lo + rl; r0 < hi; r0 += RL * KEEP) {
+        v4i raw[KEEP];
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u) {
+            raw[u] = (v4i){0, 0, 0, 0};
+            if (r0 + RL * u < hi) raw[u] = load_vec<DT, VEC>(src + (r0 + RL * u) * row_bytes);
+        }
+#pragma unroll
+        for (int u = 0; u < KEEP; ++u) {
+#pragma unroll
+            for (int j = 0; j < (VEC == 1 ? 1 : 4); ++j) {
+                if constexpr (DT == GNK_F32) { const unsigned a = (unsigned)raw[u][j] & 0x7fffffffu; mw[j] = a > mw[j] ? a : mw[j]; }
+                else mw[j] = gnk_pk_max_u16(mw[j], (unsigned)raw[u][j] & 0x7fff7fffu);
+            }
+            if (r0 == lo + rl) keep[u] = raw[u];
+        }
+    }
+    const v4i most = {(int)mw[0], (int)mw[1], (int)mw[2], (int)mw[3]};
+    float m[VEC];
+    floats_of<DT, VEC>(most, m);
+    __shared__ unsigned red[RL][CL * VEC + 1];
+    __shared__ unsigned cm[CL * VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) red[rl][cl * VEC + j] = __float_as_uint(m[j]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < CL * VEC; c += 256) {
+        unsigned v = red[0][c];
+#pragma unroll
+        for (int i = 1; i < RL; ++i) v = red[i][c] > v ? red[i][c] : v;
+        cm[c] = v;
+    }
+    __syncthreads();
+    if (col0 >= C) return;
+    GnkDivisor dv[VEC];
+    const bool fast = divisors<DT, VEC>(cm + cl * VEC, eps, dv, scale, e * C + col0, rl == 0);
+#pragma unroll
+    for (int u = 0; u < KEEP; ++u) {
+        const int64_t r = lo + rl + RL * u;
+        if (r < hi) quant_store<DT, VEC, SR>(keep[u], r, col0, C, dv, fast, q, seed, offset);
+    }
+    for (int64_t r = lo + rl + RL * KEEP; r < hi; r += RL) quant_store<DT, VEC, SR>(load_vec<DT, VEC>(src + r * row_bytes), r, col0, C, dv, fast, q, seed, offset);
+}
+
 template <int DT, int VEC, int CL>
 __global__ void __launch_bounds__(256)
 group_absmax_kernel(const char *__restrict__ x, unsigned *__restrict__ partial, const int *__restrict__ ends, int64_t T, int64_t E, int64_t C, int64_t row_bytes,
@@ -339,66 +463,28 @@ group_quant_kernel(const char *__restrict__ x, int8_t *__restrict__ q, void *__r
     __syncthreads();
     if (col0 >= C) return;
     GnkDivisor dv[VEC];
-    bool fast = true;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        const float s = __fmul_rn(__uint_as_float(cm[cl * VEC + j]), GQ_INV127);
-        dv[j].set(gnk_clamp_min_nan(s, eps));
-        fast = fast && dv[j].ok();
-        if (pc.idx == 0 && rl == 0) gnk_store_scalar_rt(scale, DT, (int64_t)pc.e * C + col0 + j, s);
-    }
-    auto emit = [&](const v4i &word, int64_t r) {
-        float f[VEC];
-        floats_of<DT, VEC>(word, f);
-        int qi[VEC];
-        float u[VEC];
-        if constexpr (SR) {
-            const unsigned long long idx0 = (unsigned long long)(r * C + col0);
-            if (VEC > 1 && ((idx0 + offset) & 3ull) == 0) {      // one Philox block per four elements
-#pragma unroll
-                for (int h = 0; h < VEC / 4; ++h) {
-                    float w[4];
-                    gnk_sr_uniform4(seed, offset, idx0 + 4 * h, w);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) u[4 * h + k] = w[k];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) u[j] = gnk_sr_uniform(seed, offset, idx0 + j);
-            }
-        }
-        if (fast) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) qi[j] = SR ? gnk_sr_clip_i8(dv[j].quot(f[j]), u[j]) : gnk_rne_clip_i8(dv[j].quot(f[j]));
-        } else {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) qi[j] = SR ? gnk_sr_clip_i8(f[j] / dv[j].d, u[j]) : gnk_rne_clip_i8_any(f[j] / dv[j].d);
-        }
-        int8_t *dst = q + r * C + col0;
-        if constexpr (VEC == 8) {
-            v2i o;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-                o[h] = (qi[4 * h] & 0xff) | ((qi[4 * h + 1] & 0xff) << 8) | ((qi[4 * h + 2] & 0xff) << 16) | (int)((unsigned)(qi[4 * h + 3] & 0xff) << 24);
-            __builtin_nontemporal_store(o, (v2i *)dst);
-        } else if constexpr (VEC == 4) {
-            *(int *)dst = (qi[0] & 0xff) | ((qi[1] & 0xff) << 8) | ((qi[2] & 0xff) << 16) | (int)((unsigned)(qi[3] & 0xff) << 24);
-        } else {
-            dst[0] = (int8_t)qi[0];
-        }
-    };
+    const bool fast = divisors<DT, VEC>(cm + cl * VEC, eps, dv, scale, (int64_t)pc.e * C + col0, pc.idx == 0 && rl == 0);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t r = r0 + rl + RL * u;
-        if (r < r1) emit(raw[u], r);
+        if (r < r1) quant_store<DT, VEC, SR>(raw[u], r, col0, C, dv, fast, q, seed, offset);
     }
-    for (int64_t r = r0 + rl + RL * U; r < r1; r += RL) emit(load_vec<DT, VEC>(src + r * row_bytes), r);
+    for (int64_t r = r0 + rl + RL * U; r < r1; r += RL) quant_store<DT, VEC, SR>(load_vec<DT, VEC>(src + r * row_bytes), r, col0, C, dv, fast, q, seed, offset);
 }
 
 template <int DT, bool VECTOR>
 int launch_group_quant(const void *x, int8_t *q, void *scale, const int *ends, int64_t T, int64_t E, int64_t C, int64_t sxt, int64_t sxc, float eps, int sr,
                        uint64_t seed, uint64_t offset, unsigned *partial, hipStream_t st) {
     constexpr int ES = DT == GNK_F32 ? 4 : 2, VEC = VECTOR ? 16 / ES : 1, CL = VECTOR ? 32 : 64;
+    if (T <= GQ_ONCE_ROWS && E < 65535) {
+        constexpr int CLO = VECTOR ? 8 : 32;
+        const dim3 g((unsigned)((C + CLO * VEC - 1) / (CLO * VEC)), (unsigned)(E + 1));
+        if (sr)
+            hipLaunchKernelGGL((group_quant_once_kernel<DT, VEC, CLO, true>), g, dim3(256), 0, st, (const char *)x, q, scale, ends, T, E, C, sxt * ES, sxc * ES, eps, seed, offset);
+        else
+            hipLaunchKernelGGL((group_quant_once_kernel<DT, VEC, CLO, false>), g, dim3(256), 0, st, (const char *)x, q, scale, ends, T, E, C, sxt * ES, sxc * ES, eps, seed, offset);
+        return gnk_check_launch("quantize_int8_grouped");
+    }
     const int sh = partial_shift(T);
     const unsigned gx = (unsigned)((C + CL * VEC - 1) / (CL * VEC));
     // 128-row pieces once they fill the chip; below that a thread's 16 rows of arithmetic (~5 us) are the kernel's length, and 32-row ones quarter it
@@ -424,7 +510,7 @@ int launch_group_quant(const void *x, int8_t *q, void *scale, const int *ends, i
 }  // namespace
 
 extern "C" int64_t gnk_quantize_int8_grouped_workspace_bytes(int64_t T, int64_t E, int64_t C) {
-    if (T <= 0 || E <= 0 || C <= 0) return 0;
+    if (T <= 0 || E <= 0 || C <= 0 || (T <= GQ_ONCE_ROWS && E < 65535)) return 0;
     return max_row_tiles(T, E, 1LL << partial_shift(T)) * C * 4;
 }
 

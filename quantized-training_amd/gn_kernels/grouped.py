@@ -38,20 +38,21 @@ def grouped_scaled_mm(A: Tensor, B: Tensor, scale_A: Tensor, scale_B: Tensor, of
     form).  Others are copied first.  scales are contiguous, the result has their dtype.  offs: int32 on the same device, not decreasing,
     at most T (not checked: that would wait for the device).
     """
-    assert (A.dtype == B.dtype == torch.int8) or (A.dtype in _FP8 and B.dtype in _FP8)
-    assert scale_A.dtype == scale_B.dtype
-    assert A.ndim == 2 and B.ndim in (2, 3)
+    dt, E = A.dtype, offs.shape[0]
+    assert (dt is torch.int8 and B.dtype is torch.int8) or (dt in _FP8 and B.dtype in _FP8)
+    assert scale_A.dtype is scale_B.dtype
     assert offs.ndim == 1 and offs.dtype is torch.int32 and offs.is_contiguous()
     assert scale_A.is_contiguous() and scale_B.is_contiguous()
-    E = offs.shape[0]
-    assert scale_B.shape in ((E, 1, B.shape[-1]), (E, 1, 1))
-    if B.ndim == 3:
-        assert B.shape[0] == E and A.shape[1] == B.shape[1]
-        assert scale_A.shape == (A.shape[0], 1)
-        return lib_ops.grouped_scaled_mm(A, B, scale_A, scale_B, offs)
-    assert A.shape[1] == B.shape[0]
-    assert scale_A.shape == (E, A.shape[0], 1)
-    return lib_ops.grouped_scaled_mm_depth(A, B, scale_A, scale_B, offs)
+    shape_B = tuple(B.shape)
+    assert tuple(scale_B.shape) in ((E, 1, shape_B[-1]), (E, 1, 1))
+    m, k = A.shape
+    if len(shape_B) == 3:
+        assert shape_B[0] == E and k == shape_B[1]
+        assert tuple(scale_A.shape) == (m, 1)
+        return lib_ops.grouped_scaled_mm.default(A, B, scale_A, scale_B, offs)
+    assert len(shape_B) == 2 and k == shape_B[0]
+    assert tuple(scale_A.shape) == (E, m, 1)
+    return lib_ops.grouped_scaled_mm_depth.default(A, B, scale_A, scale_B, offs)
 
 
 def quantize_int8_grouped(x: Tensor, offs: Tensor, stochastic_rounding: bool = False, *, eps: float = 1e-12):

@@ -256,7 +256,7 @@ def test_quantize_grouped(name, C, dt):
     assert torch.equal(s.cpu().view(torch.int8), ws.view(torch.int8))
 
 
-@pytest.mark.parametrize("sizes,pad", [([5000, 0, 129, 1, 3000], 9), ([1] * 70 + [4097], 0)])
+@pytest.mark.parametrize("sizes,pad", [([5000, 0, 129, 1, 3000], 9), ([1] * 70 + [4097], 0), ([2048], 0), ([2000, 48], 1), ([1500, 0, 300], 5)])
 def test_quantize_grouped_long(sizes, pad):
     """Groups of several partial rows."""
     x = torch.randn(sum(sizes) + pad, 72, generator=torch.Generator().manual_seed(1)).bfloat16()

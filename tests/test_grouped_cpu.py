@@ -80,4 +80,5 @@ def test_workspace_is_only_for_operands_that_cannot_be_read_in_place():
     assert rows(64, 50, 64, 50 * 64, 50, 1) == 3 * 64 * 64         # (E, K, N) with N = 50: rows of 64
     depth = lambda M, N, sat, sbt: L.gnk_grouped_scaled_mm_depth_workspace_bytes(a, b, 100, M, N, 1, sat, sbt, 1)  # noqa: E731
     assert depth(64, 48, 64, 48) == 0 and depth(64, 50, 64, 50) == 100 * 64 and depth(63, 48, 64, 48) == 100 * 64
-    assert L.gnk_quantize_int8_grouped_workspace_bytes(1000, 4, 64) == (1000 // 128 + 5) * 64 * 4
+    assert L.gnk_quantize_int8_grouped_workspace_bytes(4000, 4, 64) == (4000 // 128 + 5) * 64 * 4
+    assert L.gnk_quantize_int8_grouped_workspace_bytes(1000, 4, 64) == 0           # small calls keep their maxima on chip
