@@ -162,19 +162,23 @@ template <bool KMAJOR, int BM> __device__ __forceinline__ v8h frag16(const char 
 
 // BM = 128: 2 x 2 waves of 64 x 64, two stages (64 KiB: two workgroups per CU).  BM = 64: 2 x 2 waves of 32 x 32 would halve the fragment reads, but the
 // stores want 64 columns per wave: 4 x 1 waves of 16 x 64; four stages (64 KiB) because few tiles are bound by the latency of a step, not by its work.
+// KG = 2 (BM = 64, at most one workgroup per CU): a second set of four waves with a ring of its own takes every other step of the contraction; the two
+// halves meet in LDS, in the same order on both sides, and then one set stores the tile and the other its mirror image.
 template <int BM> struct RingShape {
     static constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1, MT = BM / WM / 16, NST = BM == 128 ? 2 : 4, OPER = BM * 128, STAGE = 2 * OPER;
     static constexpr int LDS = NST * STAGE;
 };
 
-template <int BM, bool AK, bool BK, int EPI, bool SYM>
-__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) product_ring_kernel(const Product p) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
+template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM>
+__global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2))) product_ring_kernel(const Product p) {
+    extern __shared__ __attribute__((aligned(16))) char smem_all[];
     typedef RingShape<BM> R;
+    static_assert(KG == 1 || (KG == 2 && BM == 64), "two sets of waves: 64 x 64 tiles");
     typedef GemmCfg<BM, BM, R::WM, R::WN, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;     // fp32 accumulators and the epilogue's maps
     constexpr int MT = R::MT, NST = R::NST, PIECES = 2 * BM / 32;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = KG == 1 ? 0 : wave_all >> 2, wave = wave_all & 3;
+    char *const smem = smem_all + kg * R::LDS;
     const int wm = wave / R::WN, wn = wave % R::WN;
     int b, tm, tn;
     batch_tile<SYM>(p, b, tm, tn);
@@ -188,12 +192,18 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-    const int nk = (int)(p.K / 64);
+    const int nk = ((int)(p.K / 64) + KG - 1 - kg) / KG, nk_most = KG == 1 ? nk : ((int)(p.K / 64) + KG - 1) / KG;      // steps kg, kg + KG, ...
+    if constexpr (KG > 1) {
+        sa.base += kg * sa.step;
+        sb.base += kg * sb.step;
+        sa.step *= KG;
+        sb.step *= KG;
+    }
     for (int t = 0; t < NST - 1 && t < nk; ++t) {
         sa.issue(smem + t * R::STAGE, wave);
         sb.issue(smem + t * R::STAGE + R::OPER, wave);
     }
-    for (int t = 0; t < nk; ++t) {
+    for (int t = 0; t < nk_most; ++t) {
         // stage t has landed; t + 1 .. t + NST - 2 may stay in flight
         if (t + NST - 2 < nk) asm volatile("s_waitcnt vmcnt(%0)" : : "i"((NST - 2) * PIECES) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -204,6 +214,7 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
             sa.issue(next, wave);
             sb.issue(next + R::OPER, wave);
         }
+        if (KG > 1 && t >= nk) break;                                  // the other set has one step more
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
             v8h fa[MT], fb[4];
@@ -217,6 +228,15 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
                 for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fb[j], fa[i], acc[i][j], 0, 0, 0);
         }
     }
+    if constexpr (KG > 1) {
+        __syncthreads();                                               // both rings are free
+        char *const mine = smem_all + kg * 16384, *const other = smem_all + (1 - kg) * 16384;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *(GNK_LDS v4f *)(GNK_LDS char *)(mine + 16 * ((wave * 4 + j) * 64 + lane)) = acc[0][j];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[0][j] += *(const GNK_LDS v4f *)(const GNK_LDS char *)(other + 16 * ((wave * 4 + j) * 64 + lane));     // a + b = b + a
+    }
     const float f = factor(p, b);
     const char *D = p.D + b * p.bd;
     const int64_t mw = m0 + wm * 16 * MT, nw = n0 + wn * 64;
@@ -226,15 +246,17 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
         for (int j = 0; j < 4; ++j) finish_value<EPI>(p, D, f, acc[i][j], mw + 16 * i + (lane & 15), nw + 16 * j + 4 * (lane >> 4));
     __syncthreads();
     const GemmParams g = store_params(p, b);
-    run_epilogue<Cfg>(g, acc, nullptr, smem, wave, lane, mw, nw);
+    if (kg == 0) run_epilogue<Cfg>(g, acc, nullptr, smem, wave, lane, mw, nw);
     if constexpr (SYM) {
         if (tm != tn) {
             if constexpr (MT >= 4) {
                 store_mirror<MT>(p, b, acc, smem + R::LDS / 2 + wave * (64 * 32 * MT), lane, mw, nw);
             } else {
                 // 16 rows per wave: transposed rows of 32 bytes would waste the stores; the four waves put theirs side by side first
+                // (KG = 2: the second set does, in its own ring's LDS; both pass the barrier)
                 char *const T = smem + R::LDS / 2;                     // [64 n][64 m] fp16, rows of 128 bytes, 16-byte chunk c at c ^ (n & 7)
                 const int gq = lane >> 4, ml = lane & 15;
+                if (kg == KG - 1)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -244,9 +266,10 @@ __global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) p
                     }
                 __syncthreads();
                 char *const C = (char *)p.C + b * p.bc;
+                if (kg == KG - 1)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const int e = u * 256 + (int)threadIdx.x, n = e >> 3, c = e & 7;
+                    const int e = u * 256 + ((int)threadIdx.x & 255), n = e >> 3, c = e & 7;
                     const v4i v = *(const GNK_LDS v4i *)(const GNK_LDS char *)(T + n * 128 + 16 * (c ^ (n & 7)));
                     gnk_store16_out(C + 2 * ((n0 + n) * p.N + m0) + 16 * c, v);
                 }
@@ -451,11 +474,11 @@ __global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G
     }
 }
 
-template <int BM, bool AK, bool BK, int EPI, bool SYM> int launch(const Product &p0, hipStream_t st) {
-    constexpr int LDS_TOTAL = BM == 256 ? 131072 : RingShape<BM == 256 ? 128 : BM>::LDS;
+template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM> int launch(const Product &p0, hipStream_t st) {
+    constexpr int LDS_TOTAL = BM == 256 ? 131072 : KG * RingShape<BM == 256 ? 128 : BM>::LDS;
     void (*kernel)(const Product);
     if constexpr (BM == 256) kernel = product256_kernel<AK, BK, EPI, SYM>;
-    else kernel = product_ring_kernel<BM, AK, BK, EPI, SYM>;
+    else kernel = product_ring_kernel<BM, KG, AK, BK, EPI, SYM>;
     Product p = p0;
     p.grid_m = (int)((p.ext_a + BM - 1) / BM);
     p.grid_n = (int)((p.ext_b + BM - 1) / BM);
@@ -469,7 +492,7 @@ template <int BM, bool AK, bool BK, int EPI, bool SYM> int launch(const Product 
     }
     const int64_t blocks = (int64_t)tiles_of<SYM>(p) * p.batch;
     if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "orthogonalize: too many tiles");
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), LDS_TOTAL, st, p);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256 * KG), LDS_TOTAL, st, p);
     return gnk_check_launch("orthogonalize");
 }
 
@@ -488,7 +511,7 @@ Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
     p.lo = rows <= cols ? p.rp : p.cp;
     p.x_bytes = 2 * p.rp * p.cp;
     p.s_bytes = 2 * p.lo * p.lo;
-    const int64_t want = (rows * cols + 16383) / 16384;
+    const int64_t want = (rows * cols + 4095) / 4096;
     p.nparts = (int)(want < MAX_PARTS ? (want > 0 ? want : 1) : MAX_PARTS);
     p.off_x0 = 0;
     p.off_x1 = p.off_x0 + batch * p.x_bytes;
@@ -510,9 +533,12 @@ template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p,
     const double t256 = ceil(tiles(256) / cus) * (12.0 + 1.3 * ks), t128 = ceil(tiles(128) / (2.0 * cus)) * (6.0 + 1.0 * ks);
     const double t64 = ceil(tiles(64) / (2.0 * cus)) * (4.0 + 0.4 * ks);
     const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1, 5 and 6 force the 128, 256 and 64 tiles here as well
-    if (forced == 6 || (forced != 1 && forced != 5 && t64 <= t128 && t64 <= t256)) return launch<64, AK, BK, EPI, SYM>(p, st);
-    if (forced == 5 || (forced != 1 && t256 <= t128)) return launch<256, AK, BK, EPI, SYM>(p, st);
-    return launch<128, AK, BK, EPI, SYM>(p, st);
+    if (forced == 6 || (forced != 1 && forced != 5 && t64 <= t128 && t64 <= t256)) {
+        if (tiles(64) <= cus && ks >= 4.0) return launch<64, 2, AK, BK, EPI, SYM>(p, st);
+        return launch<64, 1, AK, BK, EPI, SYM>(p, st);
+    }
+    if (forced == 5 || (forced != 1 && t256 <= t128)) return launch<256, 1, AK, BK, EPI, SYM>(p, st);
+    return launch<128, 1, AK, BK, EPI, SYM>(p, st);
 }
 
 template <int DT> int read_input(const void *G, char *X, double *parts, float *fac, int64_t batch, int64_t rows, int64_t cols, const Plan &pl, float eps, hipStream_t st) {
