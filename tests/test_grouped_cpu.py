@@ -1,9 +1,12 @@
 """The grouped products without a GPU: wrapper checks, Meta implementations, the C ABI's refusals, workspace sizes."""
 import pytest
 import torch
+import torch.nn.functional as F
+from torch import nn
 
 import gn_kernels
 from gn_kernels import _cabi
+from subclasses import MixedPrecisionConfig, MixedPrecisionLinearWeight, convert_mixed_precision_experts
 
 
 def i8(*s):
@@ -82,3 +85,134 @@ def test_workspace_is_only_for_operands_that_cannot_be_read_in_place():
     assert depth(64, 48, 64, 48) == 0 and depth(64, 50, 64, 50) == 100 * 64 and depth(63, 48, 64, 48) == 100 * 64
     assert L.gnk_quantize_int8_grouped_workspace_bytes(4000, 4, 64) == (4000 // 128 + 5) * 64 * 4
     assert L.gnk_quantize_int8_grouped_workspace_bytes(1000, 4, 64) == 0           # small calls keep their maxima on chip
+
+
+# ------------------------------------------------------------------------------------------------ F.grouped_mm on a mixed-precision weight
+@pytest.fixture(scope="module")
+def cpu_ops():
+    """The expert projection's two ops on host tensors, unquantized: what is tested is how autograd and the subclass call them."""
+    impl = torch.library.Library("gn_kernels", "IMPL")
+
+    def groups(offs):
+        ends = offs.tolist()
+        return enumerate(zip([0] + ends[:-1], ends))
+
+    def forward(x, w, offs):
+        y = x.new_zeros(x.shape[0], w.shape[2])
+        for e, (lo, hi) in groups(offs):
+            y[lo:hi] = x[lo:hi] @ w[e]
+        return y
+
+    def backward(gy, x, w, offs, need_x, need_w):
+        gx, gw = x.new_zeros(x.shape if need_x else (0, x.shape[1])), x.new_zeros((w.shape[0] if need_w else 0, w.shape[2], w.shape[1]))
+        for e, (lo, hi) in groups(offs):
+            if need_x:
+                gx[lo:hi] = gy[lo:hi] @ w[e].T
+            if need_w:
+                gw[e] = gy[lo:hi].T @ x[lo:hi]
+        return gx, gw
+
+    impl.impl("grouped_linear_int8", forward, "CPU")
+    impl.impl("grouped_linear_int8_backward", backward, "CPU")
+    yield
+
+
+class Experts(nn.Module):
+    def __init__(self, dt=torch.float64):
+        super().__init__()
+        g = torch.Generator().manual_seed(0)
+        self.up = nn.Parameter(torch.randn(3, 12, 8, generator=g, dtype=dt))
+        self.down = nn.Parameter(torch.randn(3, 8, 12, generator=g, dtype=dt))
+        self.conv = nn.Conv1d(2, 2, 3)
+        self.norm = nn.LayerNorm(8)
+
+    def forward(self, x, offs):
+        return F.grouped_mm(torch.tanh(F.grouped_mm(x, self.up.transpose(-2, -1), offs=offs)), self.down.transpose(1, 2), offs=offs)
+
+
+def plain_experts(m, x, sizes):
+    up, down = (getattr(p, "_data", p) for p in (m.up, m.down))
+    return torch.cat([torch.tanh(part @ up[e].T) @ down[e].T for e, part in enumerate(x.split(sizes))])
+
+
+def test_conversion_wraps_stacks_of_experts_only():
+    m = convert_mixed_precision_experts(Experts())
+    assert isinstance(m.up, MixedPrecisionLinearWeight) and isinstance(m.down, MixedPrecisionLinearWeight)
+    assert isinstance(m.up, nn.Parameter) or m.up.requires_grad
+    assert not isinstance(m.conv.weight, MixedPrecisionLinearWeight) and not isinstance(m.norm.weight, MixedPrecisionLinearWeight)
+
+
+@pytest.mark.parametrize("op", [F.grouped_mm, torch._grouped_mm])
+def test_autograd_of_one_projection(cpu_ops, op):
+    """Gradients against the formula and against central differences (exact for a product up to rounding: 2^-52 / h)."""
+    g = torch.Generator().manual_seed(1)
+    sizes, offs = [3, 0, 4], torch.tensor([3, 3, 7], dtype=torch.int32)
+    x, w = torch.randn(7, 8, generator=g, dtype=torch.float64), torch.randn(3, 12, 8, generator=g, dtype=torch.float64)
+    gy = torch.randn(7, 12, generator=g, dtype=torch.float64)
+    xp, wp = x.clone().requires_grad_(), nn.Parameter(MixedPrecisionLinearWeight(w.clone(), MixedPrecisionConfig()))
+    y = op(xp, wp.transpose(-2, -1), offs=offs)
+    y.backward(gy)
+    gw = wp.grad._data if isinstance(wp.grad, MixedPrecisionLinearWeight) else wp.grad
+    want = torch.cat([p @ w[e].T for e, p in enumerate(x.split(sizes))])
+    torch.testing.assert_close(y.detach(), want, rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(xp.grad, torch.cat([p @ w[e] for e, p in enumerate(gy.split(sizes))]), rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(gw, torch.stack([a.T @ b for a, b in zip(gy.split(sizes), x.split(sizes))]), rtol=1e-12, atol=1e-12)
+
+    def loss(x, w):
+        return sum(((p @ w[e].T) * q).sum() for e, (p, q) in enumerate(zip(x.split(sizes), gy.split(sizes))))
+
+    h = 2.0 ** -10
+    for i, j in ((0, 0), (6, 7), (3, 2)):
+        d = torch.zeros_like(x)
+        d[i, j] = h
+        assert abs((loss(x + d, w) - loss(x - d, w)) / (2 * h) - xp.grad[i, j]) < 1e-9
+    d = torch.zeros_like(w)
+    d[2, 5, 1] = h
+    assert abs((loss(x, w + d) - loss(x, w - d)) / (2 * h) - gw[2, 5, 1]) < 1e-9 and (gw[1] == 0).all()
+
+
+@pytest.mark.parametrize("compiled", [False, True])
+@pytest.mark.parametrize("frozen", ["none", "up", "x"])
+def test_module_of_experts(cpu_ops, compiled, frozen):
+    """Eager and traced (the ops stay opaque nodes): outputs and every gradient that is asked for, none that is not."""
+    m = convert_mixed_precision_experts(Experts())
+    sizes, offs = [2, 0, 3], torch.tensor([2, 2, 5], dtype=torch.int32)
+    x = torch.randn(5, 8, generator=torch.Generator().manual_seed(2), dtype=torch.float64).requires_grad_(frozen != "x")
+    if frozen == "up":
+        m.up.requires_grad_(False)
+    call = torch.compile(m, backend="aot_eager") if compiled else m
+    y = call(x, offs)
+    y.square().sum().backward()
+    ref = Experts()
+    xr = x.detach().clone().requires_grad_()
+    yr = plain_experts(ref, xr, sizes)
+    yr.square().sum().backward()
+    torch.testing.assert_close(y.detach(), yr.detach(), rtol=1e-12, atol=1e-12)
+    for p, r in ((m.up, ref.up), (m.down, ref.down), (x, xr)):
+        if not p.requires_grad:
+            assert p.grad is None
+            continue
+        grad = p.grad._data if isinstance(p.grad, MixedPrecisionLinearWeight) else p.grad
+        torch.testing.assert_close(grad, r.grad, rtol=1e-10, atol=1e-12)
+
+
+def test_two_dimensional_weights_are_viewed_as_before():
+    w = MixedPrecisionLinearWeight(torch.randn(4, 6), MixedPrecisionConfig())
+    assert isinstance(w.t(), MixedPrecisionLinearWeight) and not isinstance(w.transpose(0, 1), MixedPrecisionLinearWeight)
+    assert isinstance(w.detach(), MixedPrecisionLinearWeight)
+
+
+@pytest.mark.parametrize("kwargs,error", [
+    (dict(bias=torch.zeros(3, 12)), NotImplementedError),
+    (dict(out_dtype=torch.float32), NotImplementedError),
+    (dict(offs=None), NotImplementedError),
+    (dict(offs=torch.tensor([1, 2], dtype=torch.int32)), RuntimeError),
+])
+def test_grouped_mm_refusals(kwargs, error):
+    w = MixedPrecisionLinearWeight(torch.zeros(3, 12, 8, dtype=torch.bfloat16), MixedPrecisionConfig())
+    args = dict(offs=torch.tensor([1, 2, 4], dtype=torch.int32)) | kwargs
+    with pytest.raises(error):
+        F.grouped_mm(torch.zeros(4, 8, dtype=torch.bfloat16), w.transpose(-2, -1), **args)
+    with pytest.raises(NotImplementedError):
+        part = MixedPrecisionLinearWeight(torch.zeros(3, 12, 8, dtype=torch.bfloat16), MixedPrecisionConfig(grad_input=False))
+        F.grouped_mm(torch.zeros(4, 8, dtype=torch.bfloat16), part.transpose(-2, -1), offs=torch.tensor([1, 2, 4], dtype=torch.int32))

@@ -1,0 +1,123 @@
+"""The optimizer around orthogonalize: its arithmetic against the formula on the host (with the operator's definition as the host's
+implementation), and a training run on the device."""
+import json
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+from torch import nn
+
+import gn_kernels
+from muon import Muon
+from subclasses import MixedPrecisionConfig, MixedPrecisionLinearWeight
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+def newton_schulz(G, steps, a, b, c, eps):
+    X = G.double()
+    X = X / X.flatten(-2).norm(dim=-1)[..., None, None].clamp_min(eps)
+    for _ in range(steps):
+        S = X @ X.mT
+        X = a * X + b * S @ X + c * S @ S @ X
+    return X.to(G.dtype)
+
+
+@pytest.fixture(scope="module")
+def cpu_op():
+    impl = torch.library.Library("gn_kernels", "IMPL")
+    impl.impl("orthogonalize", newton_schulz, "CPU")
+    yield
+
+
+def test_wrapper_refuses_and_infers_shapes():
+    for bad in (lambda: gn_kernels.orthogonalize(torch.zeros(4, device="meta")), lambda: gn_kernels.orthogonalize(torch.zeros(4, 4, device="meta", dtype=torch.float64)),
+                lambda: gn_kernels.orthogonalize(torch.zeros(4, 4, device="meta"), steps=0), lambda: gn_kernels.orthogonalize(torch.zeros(4, 4, device="meta"), eps=-1.0),
+                lambda: gn_kernels.orthogonalize(torch.zeros(4, 4, device="meta"), coefficients=(1.0, 2.0))):
+        with pytest.raises(AssertionError):
+            bad()
+    for dt in (torch.bfloat16, torch.float16, torch.float32):
+        y = gn_kernels.orthogonalize(torch.zeros(2, 3, 4, device="meta", dtype=dt))
+        assert y.shape == (2, 3, 4) and y.dtype is dt
+
+
+def test_cabi_refusals_without_a_gpu():
+    L = gn_kernels._cabi.load()
+    call = lambda *, dt=0, b=1, m=4, n=4, steps=5, a=3.4445, eps=1e-7: L.gnk_orthogonalize(None, dt, None, dt, b, m, n, steps, a, -4.775, 2.0315, eps, None, 0, None)  # noqa: E731
+    assert call() == -1 and b"null pointer" in L.gnk_last_error()
+    assert call(dt=3) == -1 and call(b=-1) == -1 and call(steps=0) == -1 and call(steps=101) == -1 and call(a=1e5) == -1 and call(a=float("nan")) == -1
+    assert call(eps=-1.0) == -1 and call(m=(1 << 20) + 1) == -2 and call(b=1 << 16) == -2
+    assert call(b=0) == 0 and call(m=0) == 0
+    assert L.gnk_orthogonalize_workspace_bytes(0, 4, 4) == 0 and L.gnk_orthogonalize_workspace_bytes(2, 100, 300) >= 2 * 2 * 2 * (128 * 384 + 128 * 128)
+
+
+@pytest.mark.parametrize("nesterov", [True, False])
+@pytest.mark.parametrize("wd", [0.0, 0.1])
+def test_update_rule(cpu_op, nesterov, wd):
+    """Three steps of matrices of two shapes and a stack, against the formula written out."""
+    g = torch.Generator().manual_seed(0)
+    shapes = [(6, 10), (10, 6), (6, 10), (3, 6, 10)]
+    ps = [nn.Parameter(torch.randn(s, generator=g, dtype=torch.float32)) for s in shapes]
+    want = [p.detach().clone() for p in ps]
+    mom = [torch.zeros_like(p) for p in want]
+    opt = Muon(ps, lr=0.1, momentum=0.9, nesterov=nesterov, weight_decay=wd)
+    for _ in range(3):
+        grads = [torch.randn(s, generator=g) for s in shapes]
+        for p, gr in zip(ps, grads):
+            p.grad = gr.clone()
+        opt.step()
+        for i, gr in enumerate(grads):
+            mom[i] = 0.9 * mom[i] + gr
+            u = gr + 0.9 * mom[i] if nesterov else mom[i]
+            u = newton_schulz(u, 5, 3.4445, -4.7750, 2.0315, 1e-7)
+            want[i] = want[i] * (1 - 0.1 * wd) - 0.1 * max(1.0, u.shape[-2] / u.shape[-1]) ** 0.5 * u
+    for p, w in zip(ps, want):
+        # a few fp32 roundings per step, of values around 1, through an iteration that stretches small ones by 3.4 per step: 3.4^5 * 2^-22
+        torch.testing.assert_close(p.detach(), w, rtol=1e-4, atol=2e-4)
+
+
+def test_wrapped_weights_and_missing_gradients(cpu_op):
+    w = torch.randn(8, 4, generator=torch.Generator().manual_seed(1))
+    p = nn.Parameter(MixedPrecisionLinearWeight(w.clone(), MixedPrecisionConfig()))
+    q = nn.Parameter(torch.zeros(4, 4))
+    opt = Muon([p, q], lr=0.1)
+    p.grad = torch.ones(8, 4)
+    opt.step()
+    assert isinstance(p, MixedPrecisionLinearWeight) and not torch.equal(p._data, w) and torch.equal(q.detach(), torch.zeros(4, 4))
+    assert "momentum" not in opt.state[q]
+
+
+def test_refuses_what_it_cannot_update():
+    for bad in (torch.zeros(4), torch.zeros(1, 2, 3, 4)):
+        with pytest.raises(ValueError):
+            Muon([nn.Parameter(bad)])
+    with pytest.raises(ValueError):
+        Muon([nn.Parameter(torch.zeros(4, 4))], lr=-1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("quantize", ["none", "mixed_precision"])
+def test_training_harness_runs_on_the_device(quantize):
+    r = subprocess.run([sys.executable, str(ROOT / "train_bench.py"), "--model", "tiny", "--quantize", quantize, "--batch_size", "2", "--seq_len", "64", "--steps", "2",
+                        "--warmup", "1", "--optimizer", "muon"], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0, r.stderr[-2000:]
+    out = json.loads([l for l in r.stdout.splitlines() if l.startswith("{")][-1])
+    assert out["value"] > 0 and "Muon" in out["config"]["workload"]
+
+
+@pytest.mark.gpu
+def test_update_on_the_device():
+    """One step of a stack of experts and a Linear's weight: the update is lr times the operator's result."""
+    g = torch.Generator().manual_seed(2)
+    ps = [nn.Parameter(torch.randn(s, generator=g).bfloat16().cuda()) for s in ((3, 64, 96), (64, 96), (96, 64))]
+    before = [p.detach().clone() for p in ps]
+    for p in ps:
+        p.grad = torch.randn(p.shape, generator=g).bfloat16().cuda()
+    Muon(ps, lr=0.5, momentum=0.0, nesterov=False).step()
+    for p, b in zip(ps, before):
+        u = gn_kernels.orthogonalize(p.grad)
+        want = b.double() - 0.5 * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5 * u.double()
+        # the stack and the single call round alike; the sum is rounded to bf16 once (the scaled update once more where the factor is no power of two)
+        assert ((p.detach().double() - want).abs() <= 2.0 ** -8 * (want.abs() + u.double().abs())).all()

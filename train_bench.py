@@ -90,6 +90,8 @@ def parse_args(argv=None):
     ap.add_argument("--steps", type=int, default=10)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--lr", type=float, default=3e-4)
+    ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"], help="muon: orthogonalised momentum for the body's matrices (--muon_lr), AdamW for the rest")
+    ap.add_argument("--muon_lr", type=float, default=0.02)
     ap.add_argument("--weight_decay", type=float, default=1e-2)
     ap.add_argument("--activation_checkpointing", action="store_true")
     ap.add_argument("--device", default="cuda")
@@ -155,7 +157,15 @@ def run(args):
 
         # gradient_as_bucket_view: .grad aliases the bucket, which saves one copy of every gradient per step and 2 bytes per parameter
         model = DDP(model, device_ids=[local_rank] if on_gpu else None, bucket_cap_mb=args.ddp_bucket_mb, gradient_as_bucket_view=True)
-    optim = torch.optim.AdamW(model.parameters(), lr=args.lr, weight_decay=args.weight_decay, fused=on_gpu and args.quantize != "int8")
+    matrices = []
+    if args.optimizer == "muon":
+        from muon import Muon
+
+        assert args.quantize != "int8", "muon updates floating-point weights"
+        matrices = [m.weight for m in getattr(model, "module", model).model.modules() if isinstance(m, nn.Linear)]
+        muon = Muon(matrices, lr=args.muon_lr, weight_decay=args.weight_decay)
+    ids = {id(p) for p in matrices}
+    optim = torch.optim.AdamW([p for p in model.parameters() if id(p) not in ids], lr=args.lr, weight_decay=args.weight_decay, fused=on_gpu and args.quantize != "int8")
 
     # --data markov: a LEARNABLE synthetic stream (next token = perm[token] with probability 0.9, else uniform), so that loss curves of
     # the quantized and bf16 runs can be compared while the loss actually falls; uniform random tokens only ever reach log(32000).
@@ -181,6 +191,9 @@ def run(args):
         loss.backward()
         optim.step()
         optim.zero_grad()
+        if matrices:
+            muon.step()
+            muon.zero_grad()
         return loss
 
     def sync():
@@ -217,7 +230,7 @@ def run(args):
                 args.quantize, "bf16 weights/activations; int8 MFMA in the Linear fwd / grad-input / grad-weight"),
             "data": "synthetic tokens, random-init weights",
             "config": {"workload": f"llama-{args.model} {'(ASSUMED 1.1B shape: 2048/5632/22/32)' if args.model == '1b' else ''} global_batch {args.batch_size} x seq_len {args.seq_len}, "
-                                   f"quantize={args.quantize}{' ' + args.quantize_kwargs if qkw else ''}, {'torch.compile(get_loss)' if args.compile else 'eager'}, AdamW, {'DDP x%d (RCCL all-reduce)' % world if world > 1 else 'single GPU'}",
+                                   f"quantize={args.quantize}{' ' + args.quantize_kwargs if qkw else ''}, {'torch.compile(get_loss)' if args.compile else 'eager'}, {'Muon + AdamW' if matrices else 'AdamW'}, {'DDP x%d (RCCL all-reduce)' % world if world > 1 else 'single GPU'}",
                        "params": n_params, "body_linear_weights": lin},
             "body_linear_TOPS": round(6 * args.batch_size * args.seq_len * lin * args.steps / dt * 1e-12, 1),
             "loss_first_last": [round(losses[0], 4), round(losses[-1], 4)],
