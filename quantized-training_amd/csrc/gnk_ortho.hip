@@ -6,7 +6,10 @@
 // is small (by a per step where S is near 0), and with it the rounding of the intermediate matrices; bf16's 8 bits leave 1-5 % in the result, fp16's
 // 11 bits an eighth of that at the same matrix rate.  Ranges: |X| <= 1 element by element while its singular values stay around 1, so
 //   X_0 as G 2^p with |G|_F 2^p in [2^14, 2^15): no rounding at all for bf16 and fp16 inputs (1 / |G|_F goes into the products' factors);
-//   later X as X 2^10, S as S 2^10, Q as Q 2^s with |a| + 2 |b| + 4 |c| < 2^(15 - s): nothing overflows, and what underflows is below 2^-24.
+//   later X as X 2^10, S as S 2^10, Q - mu I as (Q - mu I) 2^s with |a| + 2 |b| + 4 |c| < 2^(14 - s): nothing overflows, and what underflows is
+//   below 2^-24.  mu = p(mean of S's diagonal), p(s) = a + b s + c s^2, is about the mean of Q's diagonal, which otherwise carries most of Q's rounding error:
+//   three quarters of the whole result's for flat matrices (36 x 2230: 2.6e-3 -> 1.1e-3).  mu X is added in fp32 where Q X is stored.  From 512 rows on the
+//   rounding of X is most of the error (512 x 512: 1.4e-3 of 1.6e-3) and the second read of X costs 15 % of that product: mu = 0 there.
 // Shapes are padded with zeros to multiples of 128 in the workspace: zero rows and columns stay zero through every product.
 //
 // The products: `wide` S = X X^T reads both operands along K, Q X reads X as it lies (N-contiguous, transposed on the way out of LDS); `tall` S = X^T X
@@ -26,22 +29,27 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 v4h __attribute__((ext_vector_type(4)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 
+constexpr int64_t MU_ROWS = 512;             // smaller sides below this: Q without its mean diagonal
 constexpr int PAD = 128;                     // rows and columns of every intermediate are padded to this
 constexpr float SX = 1024.0f, SS = 1024.0f;  // scales of X (after step 0) and S
 constexpr int MAX_PARTS = 256;               // partial sums of squares per matrix
 
-enum { SCALE = 0, POLY = 1 };                // epilogues: acc * f;  acc * f + D * g + (diagonal) h
+// Epilogues: GRAM acc * f;  POLY acc * f + D * g + (on the diagonal) (h - mu) k, D = S;  UPDATE (acc + D * k mu) * f, D = X
+enum { GRAM = 0, POLY = 1, UPDATE = 2 };
 
 struct Product {
     const char *A, *B;
     void *C;
-    const char *D;                           // POLY: the matrix S
+    const char *D;                           // POLY: the matrix S; UPDATE: X
     int64_t ba, bb, bc, bd;                  // bytes from one matrix of the stack to the next
     int64_t M, N, K;                         // output extents that are stored; K a multiple of 128
     int64_t lda, ldb, ldd;                   // bytes
     int64_t ext_a, ext_b;                    // staged extents (elements, >= M / N, multiples of 128)
-    float f, g, h;
-    const float *fdev;                       // SCALE: a further factor per matrix (step 0), or NULL
+    float f, g, h, k;
+    float c0, c1, c2;                        // POLY: mu = c0 + c1 s + c2 s^2, s = diag_scale * (sum of D's diagonal)
+    float diag_scale;
+    float *mu;                               // per matrix: written by POLY's first tile, read by UPDATE; NULL: mu = 0
+    const float *fdev;                       // GRAM, UPDATE: a further factor per matrix (step 0), or NULL
     int fstride;
     int out_dtype;
     int batch, grid_m, grid_n;
@@ -68,18 +76,62 @@ template <bool SYM> __device__ __forceinline__ void batch_tile(const Product &p,
     }
 }
 
+// What an epilogue needs beside the accumulators
+struct Finish {
+    const char *D;
+    float f, d, diag;                        // value = acc * f + D * d (+ diag on the diagonal)
+};
+
 // acc (lane: row m, columns n .. n + 3) -> the stored value
 template <int EPI>
-__device__ __forceinline__ void finish_value(const Product &p, const char *D, float f, v4f &acc, int64_t m, int64_t n) {
-    if constexpr (EPI == SCALE) {
+__device__ __forceinline__ void finish_value(const Product &p, const Finish &fin, v4f &acc, int64_t m, int64_t n) {
+    if constexpr (EPI == GRAM) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] *= f;
+        for (int r = 0; r < 4; ++r) acc[r] *= fin.f;
     } else {
         const int64_t mm = m < p.ext_a ? m : p.ext_a - 1, nn = n < p.ext_b ? n : p.ext_b - 4;
-        const v4h d = *(const v4h *)(D + mm * p.ldd + 2 * nn);
+        const v4h d = *(const v4h *)(fin.D + mm * p.ldd + 2 * nn);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = __builtin_fmaf(acc[r], f, __builtin_fmaf((float)d[r], p.g, m == n + r ? p.h : 0.0f));
+        for (int r = 0; r < 4; ++r) {
+            acc[r] = __builtin_fmaf(acc[r], fin.f, (float)d[r] * fin.d);
+            if (EPI == POLY && m == n + r) acc[r] += fin.diag;
+        }
     }
+}
+
+// POLY: this thread's part of the sum of S's diagonal (issued ahead of the products), and the workgroup's sum of them: every workgroup of a matrix adds the
+// same numbers in the same order
+template <int NT> __device__ __forceinline__ float diagonal_part(const Product &p, int b) {
+    const char *D = p.D + b * p.bd;
+    float s = 0.0f;
+    if (!p.mu) return s;
+    for (int64_t i = threadIdx.x; i < p.ext_a; i += NT) s += (float)*(const _Float16 *)(D + i * (p.ldd + 2));
+    return s;
+}
+template <int NT> __device__ __forceinline__ float workgroup_sum(float s, char *lds) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+    if ((threadIdx.x & 63) == 0) *(GNK_LDS float *)(GNK_LDS char *)(lds + 4 * (threadIdx.x >> 6)) = s;
+    __syncthreads();
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) t += *(const GNK_LDS float *)(const GNK_LDS char *)(lds + 4 * w);
+    __syncthreads();                         // the caller goes on using this LDS
+    return t;
+}
+
+template <int EPI> __device__ __forceinline__ Finish make_finish(const Product &p, int b, bool first_tile, float diagonal_sum) {
+    Finish fin = {nullptr, p.f, 0.0f, 0.0f};
+    if constexpr (EPI != POLY) fin.f = p.fdev ? p.f * p.fdev[(int64_t)b * p.fstride] : p.f;
+    if constexpr (EPI != GRAM) fin.D = p.D + b * p.bd;
+    if constexpr (EPI == UPDATE) fin.d = p.mu[b] * p.k * fin.f;
+    if constexpr (EPI == POLY) {
+        const float s = diagonal_sum * p.diag_scale, mu = p.mu ? __builtin_fmaf(s, __builtin_fmaf(s, p.c2, p.c1), p.c0) : 0.0f;
+        fin.d = p.g;
+        fin.diag = (p.h - mu) * p.k;
+        if (p.mu && first_tile && threadIdx.x == 0) p.mu[b] = mu;
+    }
+    return fin;
 }
 
 __device__ __forceinline__ GemmParams store_params(const Product &p, int b) {
@@ -90,8 +142,6 @@ __device__ __forceinline__ GemmParams store_params(const Product &p, int b) {
     g.out_dtype = p.out_dtype;
     return g;
 }
-
-__device__ __forceinline__ float factor(const Product &p, int b) { return p.fdev ? p.f * p.fdev[(int64_t)b * p.fstride] : p.f; }
 
 // The transpose of a wave's 16 MT x 64 results (fp16 output, rows m0 .., columns n0 ..; both inside the padded matrix), through its slice of LDS:
 // image [64 n][16 MT m], 16-byte chunk c of row n at c ^ 2 ((n >> 2) & 3), so that the four lane groups of a write land in different banks; rows of
@@ -187,6 +237,7 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
     Stager16<BK, BM> sb;
     sa.init(p.A + b * p.ba, p.lda, m0, wave, lane);
     sb.init(p.B + b * p.bb, p.ldb, n0, wave, lane);
+    const float diag = EPI == POLY ? diagonal_part<256 * KG>(p, b) : 0.0f;
     v4f acc[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -237,13 +288,17 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[0][j] += *(const GNK_LDS v4f *)(const GNK_LDS char *)(other + 16 * ((wave * 4 + j) * 64 + lane));     // a + b = b + a
     }
-    const float f = factor(p, b);
-    const char *D = p.D + b * p.bd;
+    float diag_sum = 0.0f;
+    if constexpr (EPI == POLY) {
+        __syncthreads();
+        diag_sum = workgroup_sum<256 * KG>(diag, smem_all);
+    }
+    const Finish fin = make_finish<EPI>(p, b, tm == 0 && tn == 0, diag_sum);
     const int64_t mw = m0 + wm * 16 * MT, nw = n0 + wn * 64;
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, D, f, acc[i][j], mw + 16 * i + (lane & 15), nw + 16 * j + 4 * (lane >> 4));
+        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, fin, acc[i][j], mw + 16 * i + (lane & 15), nw + 16 * j + 4 * (lane >> 4));
     __syncthreads();
     const GemmParams g = store_params(p, b);
     if (kg == 0) run_epilogue<Cfg>(g, acc, nullptr, smem, wave, lane, mw, nw);
@@ -315,14 +370,14 @@ template <int H, int I> __device__ __forceinline__ void fetch_row(v4f (&acc)[8][
 
 // columns 64 H .. 64 H + 63 of the wave tile: accumulators -> values -> memory
 template <class Cfg, int EPI, int H>
-__device__ __forceinline__ void finish_half(const Product &p, const GemmParams &g, int b, bool mirror, const char *D, float f, char *smem, int wave, int lane, int64_t mw, int64_t nw) {
+__device__ __forceinline__ void finish_half(const Product &p, const GemmParams &g, int b, bool mirror, const Finish &fin, char *smem, int wave, int lane, int64_t mw, int64_t nw) {
     v4f acc[8][4];
     fetch_row<H, 0>(acc); fetch_row<H, 1>(acc); fetch_row<H, 2>(acc); fetch_row<H, 3>(acc);
     fetch_row<H, 4>(acc); fetch_row<H, 5>(acc); fetch_row<H, 6>(acc); fetch_row<H, 7>(acc);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, D, f, acc[i][j], mw + 16 * i + (lane & 15), nw + 64 * H + 16 * j + 4 * (lane >> 4));
+        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, fin, acc[i][j], mw + 16 * i + (lane & 15), nw + 64 * H + 16 * j + 4 * (lane >> 4));
     run_epilogue<Cfg>(g, acc, nullptr, smem, wave * 2 + H, lane, mw, nw + 64 * H);
     if (mirror) store_mirror<8>(p, b, acc, smem + (wave * 2 + H) * 16384, lane, mw, nw + 64 * H);     // the same slice: a wave's LDS accesses stay in order
 }
@@ -341,6 +396,7 @@ __global__ void __launch_bounds__(256) product256_kernel(const Product p) {
     StagerW4H<BK> sb;
     sa.init(p.A + b * p.ba, p.lda, m0, p.ext_a, wave, lane);
     sb.init(p.B + b * p.bb, p.ldb, n0, p.ext_b, wave, lane);
+    const float diag = EPI == POLY ? diagonal_part<256>(p, b) : 0.0f;
     const unsigned lds0 = (unsigned)(uintptr_t)(GNK_LDS char *)smem;
     const unsigned va = lds0 + (AK ? gnk_kmaj_frag_offset(wm * 128, 0, lane) : gnk_mn16_frag_offset<512>(wm * 128, 0, lane));
     const unsigned vb = lds0 + 65536 + (BK ? gnk_kmaj_frag_offset(wn * 128, 0, lane) : gnk_mn16_frag_offset<512>(wn * 128, 0, lane));
@@ -362,13 +418,14 @@ __global__ void __launch_bounds__(256) product256_kernel(const Product p) {
     else GNK_ORTHO_RUN(GNK_W4_ASM_F16_MM);
 #undef GNK_ORTHO_RUN
     // the asm ends behind vmcnt(0) + a barrier: LDS is free for the epilogue
-    const float f = factor(p, b);
-    const char *D = p.D + b * p.bd;
+    float diag_sum = 0.0f;
+    if constexpr (EPI == POLY) diag_sum = workgroup_sum<256>(diag, smem);
+    const Finish fin = make_finish<EPI>(p, b, tm == 0 && tn == 0, diag_sum);
     const GemmParams g = store_params(p, b);
     const int64_t mw = m0 + wm * 128, nw = n0 + wn * 128;
     const bool mirror = SYM && tm != tn;
-    finish_half<Cfg, EPI, 0>(p, g, b, mirror, D, f, smem, wave, lane, mw, nw);
-    finish_half<Cfg, EPI, 1>(p, g, b, mirror, D, f, smem, wave, lane, mw, nw);
+    finish_half<Cfg, EPI, 0>(p, g, b, mirror, fin, smem, wave, lane, mw, nw);
+    finish_half<Cfg, EPI, 1>(p, g, b, mirror, fin, smem, wave, lane, mw, nw);
 }
 
 // ------------------------------------------------------------------------------ sums of squares, conversion
@@ -502,7 +559,7 @@ struct Plan {
     int64_t rp, cp, lo;                      // padded rows, columns, and the smaller of them
     int64_t x_bytes, s_bytes;                // one matrix
     int nparts;
-    int64_t off_x0, off_x1, off_s, off_q, off_parts, off_fac, total;
+    int64_t off_x0, off_x1, off_s, off_q, off_parts, off_fac, off_mu, total;
 };
 
 Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
@@ -519,7 +576,8 @@ Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
     p.off_q = p.off_s + batch * p.s_bytes;
     p.off_parts = p.off_q + batch * p.s_bytes;
     p.off_fac = p.off_parts + (batch * p.nparts * 8 + 15) / 16 * 16;
-    p.total = p.off_fac + (batch * 8 + 15) / 16 * 16;
+    p.off_mu = p.off_fac + (batch * 8 + 15) / 16 * 16;
+    p.total = p.off_mu + (batch * 4 + 15) / 16 * 16;
     return p;
 }
 
@@ -590,14 +648,16 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
     if (rc) return rc;
 
     const bool wide = rows <= cols;
-    float sq = 32768.0f;                     // scale of Q: |Q| <= |a| + 2 |b| + 4 |c| while the singular values stay below sqrt 2
-    while (sq * cmax >= 32768.0f) sq *= 0.5f;
+    float sq = 32768.0f;                     // scale of Q - mu I: |Q|, |mu| <= |a| + 2 |b| + 4 |c| while the singular values stay below sqrt 2
+    while (sq * cmax >= 16384.0f) sq *= 0.5f;
+    const bool with_mu = (wide ? rows : cols) < MU_ROWS;
     const int64_t lo = pl.lo, ldx = 2 * pl.cp, lds = 2 * lo;
     for (int it = 0; it < steps; ++it) {
         Product p;
         memset(&p, 0, sizeof(p));
         p.batch = (int)batch;
         p.fstride = 2;
+        p.mu = with_mu ? (float *)(ws + pl.off_mu) : nullptr;
         // S
         p.A = p.B = X; p.ba = p.bb = pl.x_bytes; p.lda = p.ldb = ldx;
         p.C = S; p.bc = pl.s_bytes;
@@ -606,18 +666,19 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.f = it == 0 ? SS : SS / (SX * SX);
         p.fdev = it == 0 ? fac : nullptr;
         p.out_dtype = GNK_F16;
-        rc = wide ? run_product<true, true, SCALE, true>(p, st) : run_product<false, false, SCALE, true>(p, st);
+        rc = wide ? run_product<true, true, GRAM, true>(p, st) : run_product<false, false, GRAM, true>(p, st);
         if (rc) return rc;
-        // Q = a I + b S + c S^2
+        // Q - mu I = (a - mu) I + b S + c S^2
         p.A = p.B = S; p.ba = p.bb = pl.s_bytes; p.lda = p.ldb = lds;
         p.C = Q; p.bc = pl.s_bytes;
         p.D = S; p.bd = pl.s_bytes; p.ldd = lds;
         p.K = lo;
-        p.f = c * sq / (SS * SS); p.g = b * sq / SS; p.h = a * sq;
+        p.f = c * sq / (SS * SS); p.g = b * sq / SS; p.h = a; p.k = sq;
+        p.c0 = a; p.c1 = b; p.c2 = c; p.diag_scale = 1.0f / (SS * (float)(wide ? rows : cols));
         p.fdev = nullptr;
         rc = run_product<true, true, POLY, true>(p, st);
         if (rc) return rc;
-        // X <- Q X or X Q
+        // X <- Q X or X Q: the product with Q - mu I, and mu X
         const bool last = it + 1 == steps;
         p.A = wide ? Q : X; p.ba = wide ? pl.s_bytes : pl.x_bytes; p.lda = wide ? lds : ldx;
         p.B = wide ? X : Q; p.bb = wide ? pl.x_bytes : pl.s_bytes; p.ldb = wide ? ldx : lds;
@@ -625,11 +686,13 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.bc = last ? rows * cols * gnk_dtype_size(out_dtype) : pl.x_bytes;
         p.ext_a = pl.rp; p.ext_b = pl.cp;
         p.M = last ? rows : pl.rp; p.N = last ? cols : pl.cp;
+        p.D = X; p.bd = pl.x_bytes; p.ldd = ldx; p.k = sq;
         p.K = lo;
         p.out_dtype = last ? out_dtype : GNK_F16;
         p.f = (last ? 1.0f : SX) / (it == 0 ? sq : sq * SX);
         p.fdev = it == 0 ? fac + 1 : nullptr;
-        rc = wide ? run_product<true, false, SCALE, false>(p, st) : run_product<true, true, SCALE, false>(p, st);
+        if (with_mu) rc = wide ? run_product<true, false, UPDATE, false>(p, st) : run_product<true, true, UPDATE, false>(p, st);
+        else rc = wide ? run_product<true, false, GRAM, false>(p, st) : run_product<true, true, GRAM, false>(p, st);
         if (rc) return rc;
         char *const t = X; X = Xn; Xn = t;
     }

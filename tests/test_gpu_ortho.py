@@ -1,6 +1,6 @@
 """orthogonalize against the iteration in 64 bits.
 
-Tolerance, in the norm of the result.  The kernels round S, Q and X once each per step to fp16 (as S 2^10, Q 2^s, X 2^10) and the result to its type;
+Tolerance, in the norm of the result.  The kernels round S, Q - mu I and X once each per step to fp16 (as S 2^10, (Q - mu I) 2^s, X 2^10; mu = p(mean diagonal of S) below 512 rows, else 0) and the result to its type;
 sums are fp32, K * 2^-24 of sum |a b| off at most, which moves some of those roundings to the neighbouring fp16 value and nothing else.  So the
 same iteration in 64 bits with the same roundings (`rounded`) has errors of the same size, drawn anew where a sum lay next to a border: the kernels'
 error may be at most twice the emulation's, plus half a step of the result's type, plus 2^-11 |X|, one fp16 rounding of X, for matrices so small
@@ -23,7 +23,7 @@ def iterate(G, steps, co, eps, rounded):
     a, b, c = co
     X = G.double().cpu()
     sq = 32768.0
-    while sq * (abs(a) + 2 * abs(b) + 4 * abs(c)) >= 32768:
+    while sq * (abs(a) + 2 * abs(b) + 4 * abs(c)) >= 16384:
         sq /= 2
 
     def q(t, scale):
@@ -37,7 +37,9 @@ def iterate(G, steps, co, eps, rounded):
     X = X.T if tall else X
     for i in range(steps):
         S = q(X @ X.T, 1024.0)
-        X = q(a * torch.eye(S.shape[0], dtype=S.dtype) + b * S + c * S @ S, sq) @ X
+        s = S.diagonal().mean().item()
+        mu = a + b * s + c * s * s if rounded and S.shape[0] < 512 else 0.0
+        X = q((a - mu) * torch.eye(S.shape[0], dtype=S.dtype) + b * S + c * S @ S, sq) @ X + mu * X
         X = q(X, 1024.0) if i + 1 < steps else X
     return X.T if tall else X
 
