@@ -581,22 +581,29 @@ Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
     return p;
 }
 
-template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p, hipStream_t st) {
-    // the cost model of the dense products (gnk_api.hip): us per round of workgroups, one 256 x 256 or two smaller ones per CU; a step is 64 k
-    const double cus = (double)gnk_num_cus(), ks = (double)p.K / 64.0;
+// Tile size of a product over `batch` matrices, and its time by the cost model of the dense products (gnk_api.hip: us per round of workgroups, one
+// 256 x 256 or two smaller ones per CU; a step is 64 k) with whole rounds and without (what is left where another launch fills the last one).
+struct Choice { int bm, kg; double rounds_us, work_us; };
+Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t batch) {
+    const double cus = (double)gnk_num_cus(), ks = (double)K / 64.0;
     auto tiles = [&](int64_t bm) {
-        const double gm = (double)((p.ext_a + bm - 1) / bm), gn = (double)((p.ext_b + bm - 1) / bm);
-        return (SYM ? gm * (gm + 1) / 2 : gm * gn) * (double)p.batch;
+        const double gm = (double)((ext_a + bm - 1) / bm), gn = (double)((ext_b + bm - 1) / bm);
+        return (sym ? gm * (gm + 1) / 2 : gm * gn) * (double)batch;
     };
-    const double t256 = ceil(tiles(256) / cus) * (12.0 + 1.3 * ks), t128 = ceil(tiles(128) / (2.0 * cus)) * (6.0 + 1.0 * ks);
-    const double t64 = ceil(tiles(64) / (2.0 * cus)) * (4.0 + 0.4 * ks);
+    auto priced = [&](int bm, int kg, double slots, double per) { return Choice{bm, kg, ceil(tiles(bm) / slots) * per, tiles(bm) / slots * per}; };
+    const Choice c256 = priced(256, 1, cus, 12.0 + 1.3 * ks), c128 = priced(128, 1, 2.0 * cus, 6.0 + 1.0 * ks);
+    const Choice c64 = priced(64, tiles(64) <= cus && ks >= 4.0 ? 2 : 1, 2.0 * cus, 4.0 + 0.4 * ks);
     const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1, 5 and 6 force the 128, 256 and 64 tiles here as well
-    if (forced == 6 || (forced != 1 && forced != 5 && t64 <= t128 && t64 <= t256)) {
-        if (tiles(64) <= cus && ks >= 4.0) return launch<64, 2, AK, BK, EPI, SYM>(p, st);
-        return launch<64, 1, AK, BK, EPI, SYM>(p, st);
-    }
-    if (forced == 5 || (forced != 1 && t256 <= t128)) return launch<256, 1, AK, BK, EPI, SYM>(p, st);
-    return launch<128, 1, AK, BK, EPI, SYM>(p, st);
+    if (forced == 6 || (forced != 1 && forced != 5 && c64.rounds_us <= c128.rounds_us && c64.rounds_us <= c256.rounds_us)) return c64;
+    if (forced == 5 || (forced != 1 && c256.rounds_us <= c128.rounds_us)) return c256;
+    return c128;
+}
+
+template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p, const Choice &c, hipStream_t st) {
+    if (c.bm == 256) return launch<256, 1, AK, BK, EPI, SYM>(p, st);
+    if (c.bm == 128) return launch<128, 1, AK, BK, EPI, SYM>(p, st);
+    if (c.kg == 2) return launch<64, 2, AK, BK, EPI, SYM>(p, st);
+    return launch<64, 1, AK, BK, EPI, SYM>(p, st);
 }
 
 template <int DT> int read_input(const void *G, char *X, double *parts, float *fac, int64_t batch, int64_t rows, int64_t cols, const Plan &pl, float eps, hipStream_t st) {
@@ -612,6 +619,45 @@ template <int DT> int read_input(const void *G, char *X, double *parts, float *f
     }
     return gnk_check_launch("orthogonalize");
 }
+
+// A second stream for half of a stack.  Its products depend on nothing of the other half, so the two chains fill each other's last, partly empty rounds of
+// workgroups.  One stream per device, made on first use and kept; calls that overlap only queue behind each other on it.  Not used while the caller's
+// stream is being captured (fork() then says no): a captured stream must not be shared.
+struct SideStream {
+    hipStream_t stream = nullptr;
+    hipEvent_t ev = nullptr;
+    bool fork(hipStream_t st) {
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(st, &cs) != hipSuccess || cs != hipStreamCaptureStatusNone) {
+            (void)hipGetLastError();
+            return false;
+        }
+        static std::atomic<hipStream_t> made[64];
+        int dev = 0;
+        if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return false;
+        stream = made[dev].load(std::memory_order_acquire);
+        if (!stream) {
+            hipStream_t fresh = nullptr, none = nullptr;
+            if (hipStreamCreateWithFlags(&fresh, hipStreamNonBlocking) != hipSuccess) return false;
+            if (made[dev].compare_exchange_strong(none, fresh)) stream = fresh;
+            else {
+                (void)hipStreamDestroy(fresh);
+                stream = none;
+            }
+        }
+        if (hipEventCreateWithFlags(&ev, hipEventDisableTiming) != hipSuccess) return false;
+        if (hipEventRecord(ev, st) == hipSuccess && hipStreamWaitEvent(stream, ev, 0) == hipSuccess) return true;
+        (void)hipEventDestroy(ev);
+        return false;
+    }
+    int join(hipStream_t st) {
+        const bool ok = hipEventRecord(ev, stream) == hipSuccess && hipStreamWaitEvent(st, ev, 0) == hipSuccess;
+        (void)hipEventDestroy(ev);               // released by the runtime once it has completed
+        if (ok) return GNK_OK;
+        (void)hipStreamSynchronize(stream);      // never hand the workspace back with work in flight on it
+        return gnk_fail(GNK_ERR_LAUNCH, "orthogonalize: cannot join the second stream");
+    }
+};
 
 }  // namespace
 
@@ -640,11 +686,11 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
     char *const ws = (char *)workspace;
     double *const parts = (double *)(ws + pl.off_parts);
     float *const fac = (float *)(ws + pl.off_fac);
-    char *X = ws + pl.off_x0, *Xn = ws + pl.off_x1;
-    char *const S = ws + pl.off_s, *const Q = ws + pl.off_q;
-    rc = g_dtype == GNK_BF16 ? read_input<GNK_BF16>(G, X, parts, fac, batch, rows, cols, pl, eps, st)
-         : g_dtype == GNK_F16 ? read_input<GNK_F16>(G, X, parts, fac, batch, rows, cols, pl, eps, st)
-                              : read_input<GNK_F32>(G, X, parts, fac, batch, rows, cols, pl, eps, st);
+    char *const X0 = ws + pl.off_x0, *const X1 = ws + pl.off_x1;
+    char *const S_all = ws + pl.off_s, *const Q_all = ws + pl.off_q;
+    rc = g_dtype == GNK_BF16 ? read_input<GNK_BF16>(G, X0, parts, fac, batch, rows, cols, pl, eps, st)
+         : g_dtype == GNK_F16 ? read_input<GNK_F16>(G, X0, parts, fac, batch, rows, cols, pl, eps, st)
+                              : read_input<GNK_F32>(G, X0, parts, fac, batch, rows, cols, pl, eps, st);
     if (rc) return rc;
 
     const bool wide = rows <= cols;
@@ -652,21 +698,28 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
     while (sq * cmax >= 16384.0f) sq *= 0.5f;
     const bool with_mu = (wide ? rows : cols) < MU_ROWS;
     const int64_t lo = pl.lo, ldx = 2 * pl.cp, lds = 2 * lo;
-    for (int it = 0; it < steps; ++it) {
+    // chosen for the whole stack, however it is split below: the results do not depend on the split
+    const Choice c_gram = choose_tile(lo, lo, wide ? pl.cp : pl.rp, true, batch), c_poly = choose_tile(lo, lo, lo, true, batch);
+    const Choice c_next = choose_tile(pl.rp, pl.cp, lo, false, batch);
+    // one step of matrices b0 .. b0 + n - 1 on stream s
+    auto one_step = [&](int it, int64_t b0, int64_t n, hipStream_t s) -> int {
+        const bool last = it + 1 == steps;
+        char *const X = (it & 1 ? X1 : X0) + b0 * pl.x_bytes, *const Xn = (it & 1 ? X0 : X1) + b0 * pl.x_bytes;
+        char *const S = S_all + b0 * pl.s_bytes, *const Q = Q_all + b0 * pl.s_bytes;
         Product p;
         memset(&p, 0, sizeof(p));
-        p.batch = (int)batch;
+        p.batch = (int)n;
         p.fstride = 2;
-        p.mu = with_mu ? (float *)(ws + pl.off_mu) : nullptr;
+        p.mu = with_mu ? (float *)(ws + pl.off_mu) + b0 : nullptr;
         // S
         p.A = p.B = X; p.ba = p.bb = pl.x_bytes; p.lda = p.ldb = ldx;
         p.C = S; p.bc = pl.s_bytes;
         p.M = p.N = p.ext_a = p.ext_b = lo;
         p.K = wide ? pl.cp : pl.rp;
         p.f = it == 0 ? SS : SS / (SX * SX);
-        p.fdev = it == 0 ? fac : nullptr;
+        p.fdev = it == 0 ? fac + 2 * b0 : nullptr;
         p.out_dtype = GNK_F16;
-        rc = wide ? run_product<true, true, GRAM, true>(p, st) : run_product<false, false, GRAM, true>(p, st);
+        int rc = wide ? run_product<true, true, GRAM, true>(p, c_gram, s) : run_product<false, false, GRAM, true>(p, c_gram, s);
         if (rc) return rc;
         // Q - mu I = (a - mu) I + b S + c S^2
         p.A = p.B = S; p.ba = p.bb = pl.s_bytes; p.lda = p.ldb = lds;
@@ -676,25 +729,36 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.f = c * sq / (SS * SS); p.g = b * sq / SS; p.h = a; p.k = sq;
         p.c0 = a; p.c1 = b; p.c2 = c; p.diag_scale = 1.0f / (SS * (float)(wide ? rows : cols));
         p.fdev = nullptr;
-        rc = run_product<true, true, POLY, true>(p, st);
+        rc = run_product<true, true, POLY, true>(p, c_poly, s);
         if (rc) return rc;
         // X <- Q X or X Q: the product with Q - mu I, and mu X
-        const bool last = it + 1 == steps;
         p.A = wide ? Q : X; p.ba = wide ? pl.s_bytes : pl.x_bytes; p.lda = wide ? lds : ldx;
         p.B = wide ? X : Q; p.bb = wide ? pl.x_bytes : pl.s_bytes; p.ldb = wide ? ldx : lds;
-        p.C = last ? out : (void *)Xn;
         p.bc = last ? rows * cols * gnk_dtype_size(out_dtype) : pl.x_bytes;
+        p.C = last ? (char *)out + b0 * p.bc : Xn;
         p.ext_a = pl.rp; p.ext_b = pl.cp;
         p.M = last ? rows : pl.rp; p.N = last ? cols : pl.cp;
         p.D = X; p.bd = pl.x_bytes; p.ldd = ldx; p.k = sq;
         p.K = lo;
         p.out_dtype = last ? out_dtype : GNK_F16;
         p.f = (last ? 1.0f : SX) / (it == 0 ? sq : sq * SX);
-        p.fdev = it == 0 ? fac + 1 : nullptr;
-        if (with_mu) rc = wide ? run_product<true, false, UPDATE, false>(p, st) : run_product<true, true, UPDATE, false>(p, st);
-        else rc = wide ? run_product<true, false, GRAM, false>(p, st) : run_product<true, true, GRAM, false>(p, st);
-        if (rc) return rc;
-        char *const t = X; X = Xn; Xn = t;
+        p.fdev = it == 0 ? fac + 2 * b0 + 1 : nullptr;
+        if (with_mu) return wide ? run_product<true, false, UPDATE, false>(p, c_next, s) : run_product<true, true, UPDATE, false>(p, c_next, s);
+        return wide ? run_product<true, false, GRAM, false>(p, c_next, s) : run_product<true, true, GRAM, false>(p, c_next, s);
+    };
+    // Two chains of half the stack each where that is worth the second stream: large products (below B m^2 n = 1e11 two short chains get in each other's way:
+    // 8 x 1024 x 4096 734 us alone, 966 us as two) whose last rounds are partly empty.  8 x 2048 x 5632: 3.35 -> 2.89 ms, 2 x 4096 x 4096: 2.84 -> 2.36.
+    const double rounds = c_gram.rounds_us + c_poly.rounds_us + c_next.rounds_us, work = c_gram.work_us + c_poly.work_us + c_next.work_us;
+    SideStream side;
+    const bool two = batch > 1 && (double)batch * (double)lo * (double)pl.rp * (double)pl.cp >= 1.0e11 && work <= 0.9 * rounds && side.fork(st);
+    const int64_t half = two ? batch / 2 : batch;
+    for (int it = 0; it < steps && !rc; ++it) {
+        rc = one_step(it, 0, half, st);
+        if (two && !rc) rc = one_step(it, half, batch - half, side.stream);
     }
-    return GNK_OK;
+    if (two) {
+        const int joined = side.join(st);
+        if (!rc) rc = joined;
+    }
+    return rc;
 }

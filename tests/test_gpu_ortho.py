@@ -165,6 +165,38 @@ def test_graph_and_streams():
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_large_stack_takes_two_streams():
+    """A stack that is split over two streams: against the definition (64 bits, on the device), from another stream while its own next call is on the way,
+    and captured (one stream there) with the same bits."""
+    B, n = 2, 4096
+    G = torch.stack([torch.randn(n, n, generator=torch.Generator(device=DEV).manual_seed(i), device=DEV) for i in range(B)]).bfloat16()
+    got = gn_kernels.orthogonalize(G)
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        again = [gn_kernels.orthogonalize(G) for _ in range(3)]
+    here = gn_kernels.orthogonalize(G)
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, got) for x in (*again, here))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gn_kernels.orthogonalize(G)
+    for k in range(2):
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, gn_kernels.orthogonalize(G))
+        assert torch.equal(out, got)
+    X = G[1].double()
+    X = X / X.norm()
+    for _ in range(5):
+        S = X @ X.T
+        X = COEFFS[0] * X + COEFFS[1] * (S @ X) + COEFFS[2] * (S @ (S @ X))
+    # the fp16 roundings leave 1.2e-3 of the norm at 512 x 512 for this kind of matrix (the emulation of the other tests; it does not grow with the
+    # size, every rounding being relative): twice that, and the bf16 result's half step
+    assert (got[1].double() - X).norm() <= (2 * 1.2e-3 + 2.0 ** -8) * X.norm()
+
+
 def test_refusals():
     with pytest.raises(RuntimeError):
         torch.ops.gn_kernels.orthogonalize(torch.zeros(4, 4, dtype=torch.float64, device=DEV), 5, *COEFFS, 1e-7)
