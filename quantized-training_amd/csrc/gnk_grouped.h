@@ -72,8 +72,12 @@ __device__ __forceinline__ void lane_group(const int *ends, int64_t E, int64_t T
     if (hi < lo) hi = lo;
 }
 
-// Every group (and the rows behind the last one) is cut into pieces of 1 << sh rows, numbered in group order.
-__device__ __forceinline__ int pieces_of(int rows, int sh) { return (int)(((unsigned)rows + ((1u << sh) - 1)) >> sh); }
+// Every group (and the rows behind the last one) is cut into pieces of 1 << sh rows (sh = -192: of 192 rows), numbered in group order.
+constexpr int ROWS_192 = -192;
+__device__ __forceinline__ int pieces_of(int rows, int sh) {
+    if (sh == ROWS_192) return (int)(((unsigned)rows + 191u) / 192u);
+    return (int)(((unsigned)rows + ((1u << sh) - 1)) >> sh);
+}
 
 __device__ __forceinline__ int count_pieces(const int *ends, int64_t E, int64_t T, int lane, int sh) {
     int total = 0;
@@ -110,8 +114,8 @@ __device__ __forceinline__ Piece find_piece(const int *ends, int64_t E, int64_t 
 // rows form: tiles are counted on the device, then given to the XCDs in contiguous runs and walked in strips as tile_of_block does
 template <int BM>
 __device__ __forceinline__ Tile rows_tile(const GroupedParams &p, int grid_n, int lane) {
-    constexpr int SH = BM == 256 ? 8 : BM == 128 ? 7 : BM == 64 ? 6 : BM == 32 ? 5 : 4;
-    static_assert(BM == 1 << SH, "row tiles are powers of two");
+    constexpr int SH = BM == 256 ? 8 : BM == 192 ? ROWS_192 : BM == 128 ? 7 : 6;
+    static_assert(BM == 256 || BM == 192 || BM == 128 || BM == 64, "row tiles");
     Tile t;
     const int grid_m = count_pieces(p.ends, p.E, p.T, lane, SH);
     t.work = (int64_t)blockIdx.x < (int64_t)grid_m * grid_n;
@@ -317,22 +321,40 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(2)
     run_epilogue<Cfg>(p, acc, nullptr, smem, wave, lane, m0 + wm * Cfg::WTM, n0 + wn * Cfg::WTN, lsc, wm * Cfg::WTM, wn * Cfg::WTN);
 }
 
+// columns 64 H .. 64 H + 63 of a wave's 96 x 128 results (int8): six accumulator rows of 16, the epilogue of a 192 x 256 tile
+template <class Cfg, int H, int I> __device__ __forceinline__ void fetch_row_192(v4i (&acc)[6][4]) {
+    int r[16];
+    w4_read16<8 * H + I>(r);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[I][j] = (v4i){r[4 * j], r[4 * j + 1], r[4 * j + 2], r[4 * j + 3]};
+}
+template <class Cfg, int H>
+__device__ __forceinline__ void finish_half_192(const GemmParams &p, char *smem, int wave, int lane, int64_t mwave, int64_t nwave, const float *lsc, int mlw, int nlw) {
+    typedef GemmCfg<192, 256, 2, 4, Cfg::A_KMAJOR, Cfg::B_KMAJOR, OP_I8, 0, 0, EPI_ROWCOL> ECfg;
+    v4i acc[6][4];
+    fetch_row_192<Cfg, H, 0>(acc); fetch_row_192<Cfg, H, 1>(acc); fetch_row_192<Cfg, H, 2>(acc);
+    fetch_row_192<Cfg, H, 3>(acc); fetch_row_192<Cfg, H, 4>(acc); fetch_row_192<Cfg, H, 5>(acc);
+    run_epilogue<ECfg>(p, acc, nullptr, smem, wave * 2 + H, lane, mwave, nwave + 64 * H, lsc, mlw, nlw + 64 * H);
+}
+
 // ------------------------------------------------------------------------------ 256 x 256, one wave per SIMD (gnk_gemm_w4.h)
 // rows: K % 256 == 0, the dense loop on the group's tile.  depth: the contraction ends where the group does, so the loop reads through buffer
 // descriptors that end there too: k-rows past the end are out of range and arrive in LDS as zeros, which add nothing in int8 and fp8; the loop
 // runs over ceil(T_e / 256) * 256 of them (a group without rows: once over zeros).  Host-checked: T * pitch < 2^32 (the descriptors' sizes).
-template <class Cfg, bool DEPTH>
+// BM = 192 (rows, int8): the same loop with three quarters of the rows, for tile counts that leave the last round of 256-row tiles nearly empty.
+template <class Cfg, bool DEPTH, int BM = 256>
 __global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef typename W4Select<Cfg, Cfg::OP>::type K;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
-    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n) : rows_tile<256>(gp, gp.g.grid_n, lane);
+    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n) : rows_tile<BM>(gp, gp.g.grid_n, lane);
     if (!tile.work) return;
-    const int64_t m0 = (int64_t)tile.tm * 256, n0 = (int64_t)tile.tn * 256;
+    constexpr int WTM = BM / 2;
+    const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * 256;
     if (!DEPTH && tile.e == gp.E) {
-        zero_tile<256, 256, 256>((char *)gp.g.C + tile.lo * gp.g.N * gp.out_bytes, tile.hi - tile.lo, gp.g.N, m0, n0, gp.out_bytes);
+        zero_tile<BM, 256, 256>((char *)gp.g.C + tile.lo * gp.g.N * gp.out_bytes, tile.hi - tile.lo, gp.g.N, m0, n0, gp.out_bytes);
         return;
     }
     int64_t ext_a, ext_b;
@@ -349,7 +371,7 @@ __global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
     sb.init(p.B, p.ldb, n0, ext_b, wave, lane);
 
     const unsigned lds0 = (unsigned)(uintptr_t)(GNK_LDS char *)smem;
-    const unsigned va = lds0 + K::frag0(Cfg::A_KMAJOR, wm * 128, lane);
+    const unsigned va = lds0 + K::frag0(Cfg::A_KMAJOR, wm * WTM, lane);
     const unsigned vb = lds0 + 4 * Cfg::OPER_BYTES + K::frag0(Cfg::B_KMAJOR, wn * 128, lane);
     const unsigned alo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)sa.base), ahi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)sa.base >> 32));
     const unsigned blo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)sb.base), bhi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)sb.base >> 32));
@@ -378,7 +400,9 @@ __global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
                      [oa7] "v"(sa.off[7]), [ob4] "v"(sb.off[4]), [ob5] "v"(sb.off[5]), [ob6] "v"(sb.off[6]), [ob7] "v"(sb.off[7])     \
                      : GNK_W4_CLOBBERS)
         if constexpr (Cfg::OP == OP_I8) {
-            if constexpr (Cfg::B_KMAJOR) GNK_GROUPED_W4_RUN(GNK_W4_ASM_I8_KK);
+            if constexpr (BM == 192 && Cfg::B_KMAJOR) GNK_GROUPED_W4_RUN(GNK_W4_ASM_I8_KK_192);
+            else if constexpr (BM == 192) GNK_GROUPED_W4_RUN(GNK_W4_ASM_I8_KM_192);
+            else if constexpr (Cfg::B_KMAJOR) GNK_GROUPED_W4_RUN(GNK_W4_ASM_I8_KK);
             else GNK_GROUPED_W4_RUN(GNK_W4_ASM_I8_KM);
         } else {
             if constexpr (Cfg::B_KMAJOR) GNK_GROUPED_W4_RUN(GNK_W4_ASM_F8_KK);
@@ -389,11 +413,16 @@ __global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
 #undef GNK_GROUPED_W4_IN
     // the asm ends behind vmcnt(0) + a barrier: LDS is free for the epilogue
     float *const lsc = (float *)(smem + Cfg::LDS_BYTES);
-    *(GNK_LDS float *)(GNK_LDS char *)((char *)lsc + 4 * threadIdx.x) = gnk_raw_to_f32_rt(raw_r, p.scale_dtype);
-    *(GNK_LDS float *)(GNK_LDS char *)((char *)lsc + 4 * (256 + threadIdx.x)) = gnk_raw_to_f32_rt(raw_c, p.scale_dtype);
+    if (BM == 256 || (int)threadIdx.x < BM) *(GNK_LDS float *)(GNK_LDS char *)((char *)lsc + 4 * threadIdx.x) = gnk_raw_to_f32_rt(raw_r, p.scale_dtype);
+    *(GNK_LDS float *)(GNK_LDS char *)((char *)lsc + 4 * (BM + threadIdx.x)) = gnk_raw_to_f32_rt(raw_c, p.scale_dtype);      // behind the rows' (EpiScales)
     __syncthreads();
-    K::template finish_half<0>(p, smem, wave, lane, m0 + wm * 128, n0 + wn * 128, lsc, wm * 128, wn * 128);
-    K::template finish_half<1>(p, smem, wave, lane, m0 + wm * 128, n0 + wn * 128, lsc, wm * 128, wn * 128);
+    if constexpr (BM == 192) {
+        finish_half_192<Cfg, 0>(p, smem, wave, lane, m0 + wm * WTM, n0 + wn * 128, lsc, wm * WTM, wn * 128);
+        finish_half_192<Cfg, 1>(p, smem, wave, lane, m0 + wm * WTM, n0 + wn * 128, lsc, wm * WTM, wn * 128);
+    } else {
+        K::template finish_half<0>(p, smem, wave, lane, m0 + wm * 128, n0 + wn * 128, lsc, wm * 128, wn * 128);
+        K::template finish_half<1>(p, smem, wave, lane, m0 + wm * 128, n0 + wn * 128, lsc, wm * 128, wn * 128);
+    }
 }
 
 // most row tiles the groups can need: every group wastes less than one tile, and the rows behind the last group are one group more
@@ -437,36 +466,50 @@ template <class Cfg, bool DEPTH> int launch_ring(const GroupedParams &p, hipStre
     return launch_tiles(ring_kernel<Cfg, DEPTH>, done, 4 * (Cfg::A_BYTES + Cfg::B_BYTES) + (Cfg::BM + Cfg::BN) * 4, Cfg::NT, DEPTH, Cfg::BM, Cfg::BN, p, st);
 }
 
-template <class Cfg, bool DEPTH> int launch_w4(const GroupedParams &p, hipStream_t st) {
+template <class Cfg, bool DEPTH, int BM = 256> int launch_w4(const GroupedParams &p, hipStream_t st) {
     static std::atomic<bool> done[64];
-    return launch_tiles(w4_kernel<Cfg, DEPTH>, done, Cfg::LDS_BYTES + 2048, 256, DEPTH, 256, 256, p, st);
+    return launch_tiles(w4_kernel<Cfg, DEPTH, BM>, done, Cfg::LDS_BYTES + 2048, 256, DEPTH, BM, 256, p, st);
 }
 
 // Tile choice, by the cost model of the dense products (gnk_api.hip: us per round of workgroups; one 256 x 256 or two 128 x 128 per CU) on the
 // sizes that the host knows: groups of T / E rows, half a tile of edge each.
-static inline int choose_variant(const GroupedParams &p, bool depth, bool can_w4) {
+constexpr int VARIANT_192 = 100;             // beside gnk_set_gemm_variant's numbers: 192 x 256 (int8, rows form)
+
+static inline int choose_variant(const GroupedParams &p, bool depth, bool can_w4, bool can_192) {
     const double cus = (double)gnk_num_cus();
     const double groups = (double)(p.E < p.T ? p.E : p.T), rows = (double)p.T;
-    auto tiles = [&](double bm) {
-        const double gn = ceil((double)p.g.N / bm);
+    auto tiles = [&](double bm, double bn) {
+        const double gn = ceil((double)p.g.N / bn);
         if (depth) return (double)p.E * ceil((double)p.g.M / bm) * gn;
-        const double m = rows / bm + 0.5 * groups;
-        return (m > groups ? m : groups) * gn;
+        const double m = rows / bm + 0.5 * groups, least = 1.15 * groups;      // sizes spread: some groups of less than a tile on average need two
+        return (m > least ? m : least) * gn;
     };
     const double ks = depth ? rows / (double)p.E / 128.0 : (double)p.g.K / 128.0;
     const double edge = depth ? 1.0 : 0.0;       // a 256-k step of the ragged loop is half empty on average
-    const double t256 = ceil(tiles(256) / cus) * (12.0 + 1.08 * (ks + edge)), t128 = ceil(tiles(128) / (2.0 * cus)) * (6.0 + 1.0 * ks);
-    const double t64 = ceil(tiles(64) / (2.0 * cus)) * (5.0 + 0.45 * ks);
+    // the number of row tiles is an estimate: a last round that it fills to a few percent may as well not be there or be full, so rounds count from
+    // 8 % of one on, and what a tile costs decides
+    auto rounds = [&](double n, double slots) { return n <= slots ? 1.0 : ceil(n / slots - 0.08); };
+    const double t256 = rounds(tiles(256, 256), cus) * (12.0 + 1.08 * (ks + edge)), t128 = ceil(tiles(128, 128) / (2.0 * cus)) * (6.0 + 1.0 * ks);
+    const double t192 = rounds(tiles(192, 256), cus) * (11.0 + 0.86 * ks);
+    const double t64 = ceil(tiles(64, 64) / (2.0 * cus)) * (5.0 + 0.45 * ks);
     if (t64 <= t128 && (t64 <= t256 || !can_w4)) return GNK_VARIANT_64X128;
+    if (can_192 && t192 < 0.98 * t256 && t192 < t128) return VARIANT_192;
     return can_w4 && t256 <= t128 ? GNK_VARIANT_256_W4 : GNK_VARIANT_128;
 }
 
 template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st) {
     const bool can_w4 = depth ? p.T * (p.g.lda > p.g.ldb ? p.g.lda : p.g.ldb) < (1LL << 32) : p.g.K >= 256 && p.g.K % 256 == 0;
-    // gnk_set_gemm_variant: 1, 5 and 6 force the 128 x 128, the 256 x 256 (where it can run) and the 64 x 64 kernel
+    const bool can_192 = OP == OP_I8 && !depth && can_w4;
+    // gnk_set_gemm_variant: 1, 5 and 6 force the 128 x 128, the 256 x 256 (where it can run) and the 64 x 64 kernel, 0 the 192 x 256 one
     int variant = gnk_forced_variant_get();
-    if ((variant != GNK_VARIANT_128 && variant != GNK_VARIANT_64X128 && variant != GNK_VARIANT_256_W4) || (variant == GNK_VARIANT_256_W4 && !can_w4))
-        variant = choose_variant(p, depth, can_w4);
+    if (variant == GNK_VARIANT_256 && can_192) variant = VARIANT_192;
+    else if ((variant != GNK_VARIANT_128 && variant != GNK_VARIANT_64X128 && variant != GNK_VARIANT_256_W4) || (variant == GNK_VARIANT_256_W4 && !can_w4))
+        variant = choose_variant(p, depth, can_w4, can_192);
+    if constexpr (OP == OP_I8) {
+        if (variant == VARIANT_192)
+            return b_kmajor ? launch_w4<PP2Cfg<true, true, OP, FA, FB, EPI_ROWCOL>, false, 192>(p, st)
+                            : launch_w4<PP2Cfg<true, false, OP, FA, FB, EPI_ROWCOL>, false, 192>(p, st);
+    }
     if (variant == GNK_VARIANT_256_W4) {
         if (depth) return launch_w4<PP2Cfg<false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
         if (b_kmajor) return launch_w4<PP2Cfg<true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);

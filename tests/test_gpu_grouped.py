@@ -371,7 +371,7 @@ def test_refusals_on_device():
 
 
 # ------------------------------------------------------------------------------------------------ tile variants
-@pytest.fixture(params=[1, 5, 6], ids=["tile128", "tile256w4", "tile64"])
+@pytest.fixture(params=[1, 5, 6, 0], ids=["tile128", "tile256w4", "tile64", "tile192"])
 def forced(request):
     L = _cabi.load()
     old = L.gnk_set_gemm_variant(request.param)
@@ -394,6 +394,14 @@ def test_variants_depth_ends(forced, sizes):
     for M, N in ((256, 256), (16, 32), (100, 300)):
         run_depth(sizes, 3, M, N, "int8", "f32")
         run_depth(sizes, 3, M, N, "e4m3", "bf16")
+
+
+@pytest.mark.parametrize("sizes", [[191, 192, 193], [95, 96, 97, 1], [385, 0, 383]])
+def test_variants_row_edges(forced, sizes):
+    """Group sizes around the halves and multiples of a 192-row tile."""
+    for K, N in ((256, 256), (768, 300), (1024, 16)):
+        for order in ((0, 2, 1), (0, 1, 2)):
+            run_rows(sizes, 3, K, N, "int8", "f32", order)
 
 
 @pytest.mark.parametrize("out", list(OUT))

@@ -54,8 +54,10 @@ def rng(r, n):
 
 
 class Gen:
-    def __init__(self, op, ak, bk, ragged=False):
+    def __init__(self, op, ak, bk, ragged=False, rows=256):
         self.op = op
+        self.rows = rows                 # of the tile: 256, or 192 (int8, A K-major: three quarters of A's fragments, pieces and super-stage)
+        assert rows == 256 or (rows == 192 and op == "i8" and ak)
         self.ragged = ragged
         assert not ragged or not (ak or bk)
         self.kmaj = {"a": ak, "b": bk}
@@ -65,6 +67,8 @@ class Gen:
         self.wide = op == "f8"
         self.fw = 8 if self.wide else 4
         self.nf = 4 if self.wide else 8
+        self.frags = {"a": self.nf * rows // 256, "b": self.nf}
+        self.ss_bytes = {"a": SS_BYTES * rows // 256, "b": SS_BYTES}
         self.vm, self.vm_prologue = self.waits()
 
     def e(self, s):
@@ -76,10 +80,10 @@ class Gen:
         for operand in ("b", "a"):
             o = OPERANDS[operand]
             abase = o["abase"]
-            for f in range(self.nf):
+            for f in range(self.frags[operand]):
                 r = frag_reg(cset, operand, f, self.fw)
                 if self.kmaj[operand]:
-                    off, ks = ((t >> 1) & 1) * SS_BYTES, t & 1
+                    off, ks = ((t >> 1) & 1) * self.ss_bytes[operand], t & 1
                     if not self.wide:     # 16 rows x 128 B per fragment: + 2 f KiB; address register ks
                         out.append(f"ds_read_b128 v{rng(r, 4)}, v{abase + ks} offset:{off + f * 2048}")
                     else:                 # 32 rows x 128 B per fragment: + 4 f KiB; chunks (h, 2 + h) of the 64-k half: registers 2 ks, 2 ks + 1
@@ -105,7 +109,8 @@ class Gen:
 
     def pieces_km(self, operand, ss):
         o = OPERANDS[operand]
-        return [(operand, o["ring"] + (ss & 1) * SS_BYTES + i * 4096, i, 2 * ss - 1) for i in range(8)]
+        size = self.ss_bytes[operand]
+        return [(operand, o["ring"] + (ss & 1) * size + i * 4096, i, 2 * ss - 1) for i in range(size // 4096)]
 
     def issue_group(self, mn_stage=None, km_ss=None):
         """One group of issues, earliest deadline first; each operand's pointer advances behind its pieces."""
@@ -169,7 +174,7 @@ class Gen:
         out = []
         if not self.wide:
             ins = {"i8": "v_mfma_i32_16x16x64_i8", "f16": "v_mfma_f32_16x16x32_f16", "bf16": "v_mfma_f32_16x16x32_bf16"}[self.op]
-            for s in range(16):
+            for s in range(2 * self.frags["a"]):
                 i, h = s >> 1, s & 1
                 for j in range(4):
                     t = 32 * h + 4 * i + j
@@ -302,6 +307,7 @@ HEAD = "// GENERATED by tools/gen_w4_asm.py -- do not edit; see that file for th
 def main():
     # loops beside the dense 8-bit ones: ragged K (products grouped by expert), 16-bit floats
     more = [HEAD] + [macro(f"GNK_W4_ASM_{op.upper()}_MM_RAGGED", Gen(op, False, False, ragged=True)) for op in ("i8", "f8")]
+    more += [macro(f"GNK_W4_ASM_I8_K{'K' if bk else 'M'}_192", Gen("i8", True, bk, rows=192)) for bk in (True, False)]
     more += [macro(f"GNK_W4_ASM_F16_{'K' if ak else 'M'}{'K' if bk else 'M'}", Gen("f16", ak, bk)) for ak, bk in ((True, True), (True, False), (False, False))]
     more.append("#define GNK_W4_CLOBBERS_RAGGED GNK_W4_CLOBBERS, " + ", ".join(f'"s{r}"' for r in range(92, 100)) + "\n")
     MORE.write_text("\n".join(more))
