@@ -117,6 +117,21 @@ __device__ __forceinline__ Tile rows_tile(const GroupedParams &p, int grid_n, in
     constexpr int SH = BM == 256 ? 8 : BM == 192 ? ROWS_192 : BM == 128 ? 7 : 6;
     static_assert(BM == 256 || BM == 192 || BM == 128 || BM == 64, "row tiles");
     Tile t;
+    if (p.E < 64) {                          // all groups in one wave: one load and one prefix sum give the count and the place
+        int l, h;
+        lane_group(p.ends, p.E, p.T, 0, lane, l, h);
+        const int n = pieces_of(h - l, SH), incl = wave_prefix(n), grid_m = __builtin_amdgcn_readlane(incl, 63);
+        t.work = (int64_t)blockIdx.x < (int64_t)grid_m * grid_n;
+        if (!t.work) return t;
+        int tm;
+        tile_of_block(grid_m, grid_n, tm, t.tn);
+        const int src = __builtin_ctzll(__ballot(incl > tm));
+        t.e = src;
+        t.tm = tm - __builtin_amdgcn_readlane(incl - n, src);
+        t.lo = __builtin_amdgcn_readlane(l, src);
+        t.hi = __builtin_amdgcn_readlane(h, src);
+        return t;
+    }
     const int grid_m = count_pieces(p.ends, p.E, p.T, lane, SH);
     t.work = (int64_t)blockIdx.x < (int64_t)grid_m * grid_n;
     if (!t.work) return t;
@@ -471,30 +486,36 @@ template <class Cfg, bool DEPTH, int BM = 256> int launch_w4(const GroupedParams
     return launch_tiles(w4_kernel<Cfg, DEPTH, BM>, done, Cfg::LDS_BYTES + 2048, 256, DEPTH, BM, 256, p, st);
 }
 
-// Tile choice, by the cost model of the dense products (gnk_api.hip: us per round of workgroups; one 256 x 256 or two 128 x 128 per CU) on the
-// sizes that the host knows: groups of T / E rows, half a tile of edge each.
+// Tile choice by a cost model in us on the sizes that the host knows: groups of T / E rows, half a tile of edge each.  Constants fitted to forced runs of every
+// variant over 16 .. 32768 rows, 1 .. 64 groups, K, N = 512 .. 5632: a 256 x 256 or 192 x 256 workgroup (one per CU) costs 11-12 + 1.08 / 0.86 per 128 k, a
+// 128 x 128 one (two per CU) 6 + 1.0 with both operands K-major, 1.5 with B N-major, 1.3 in the depth form, a 64 x 64 one 5 + 0.55.
 constexpr int VARIANT_192 = 100;             // beside gnk_set_gemm_variant's numbers: 192 x 256 (int8, rows form)
 
-static inline int choose_variant(const GroupedParams &p, bool depth, bool can_w4, bool can_192) {
-    const double cus = (double)gnk_num_cus();
-    const double groups = (double)(p.E < p.T ? p.E : p.T), rows = (double)p.T;
+static inline int choose_variant(const GroupedParams &p, bool depth, bool b_kmajor, bool can_w4, bool can_192) {
+    const double cus = (double)gnk_num_cus(), rows = (double)p.T, E = (double)(p.E > 0 ? p.E : 1);
+    const double groups = E * (1.0 - pow(1.0 - 1.0 / E, rows));      // groups that a uniform router leaves with a row
     auto tiles = [&](double bm, double bn) {
         const double gn = ceil((double)p.g.N / bn);
-        if (depth) return (double)p.E * ceil((double)p.g.M / bm) * gn;
-        const double m = rows / bm + 0.5 * groups, least = 1.15 * groups;      // sizes spread: some groups of less than a tile on average need two
+        if (depth) return E * ceil((double)p.g.M / bm) * gn;
+        // sizes spread: where a group has half a tile or more on average, some have more than one
+        const double m = rows / bm + 0.5 * groups, fill = groups > 0 ? rows / groups / bm : 0.0, least = groups * (1.0 + 0.3 * (fill < 0.5 ? fill : 0.5));
         return (m > least ? m : least) * gn;
     };
-    const double ks = depth ? rows / (double)p.E / 128.0 : (double)p.g.K / 128.0;
+    // whole rounds, but the number of row tiles is an estimate: the mean over 5 % less, 5 % and 15 % more of them (depth: it is known)
+    auto rounds = [&](double n, double slots) {
+        return depth ? ceil(n / slots) : (ceil(0.95 * n / slots) + ceil(1.05 * n / slots) + ceil(1.15 * n / slots)) / 3.0;
+    };
+    // two workgroups per CU run at different times: the rounds of the 128 x 128 kernel smear
+    auto smeared = [&](double n, double slots) { return n <= slots ? 1.0 : n / slots + 0.25; };
+    const double ks = depth ? rows / E / 128.0 : (double)p.g.K / 128.0;
     const double edge = depth ? 1.0 : 0.0;       // a 256-k step of the ragged loop is half empty on average
-    // the number of row tiles is an estimate: a last round that it fills to a few percent may as well not be there or be full, so rounds count from
-    // 8 % of one on, and what a tile costs decides
-    auto rounds = [&](double n, double slots) { return n <= slots ? 1.0 : ceil(n / slots - 0.08); };
-    const double t256 = rounds(tiles(256, 256), cus) * (12.0 + 1.08 * (ks + edge)), t128 = ceil(tiles(128, 128) / (2.0 * cus)) * (6.0 + 1.0 * ks);
-    const double t192 = rounds(tiles(192, 256), cus) * (11.0 + 0.86 * ks);
-    const double t64 = ceil(tiles(64, 64) / (2.0 * cus)) * (5.0 + 0.45 * ks);
-    if (t64 <= t128 && (t64 <= t256 || !can_w4)) return GNK_VARIANT_64X128;
-    if (can_192 && t192 < 0.98 * t256 && t192 < t128) return VARIANT_192;
-    return can_w4 && t256 <= t128 ? GNK_VARIANT_256_W4 : GNK_VARIANT_128;
+    const double t256 = can_w4 ? rounds(tiles(256, 256), cus) * (12.0 + 1.08 * (ks + edge)) : 1e30;
+    const double t192 = can_192 ? rounds(tiles(192, 256), cus) * (11.0 + 0.86 * ks) : 1e30;
+    const double t128 = smeared(tiles(128, 128), 2.0 * cus) * (6.0 + (depth ? 1.3 : b_kmajor ? 1.0 : 1.5) * ks);
+    const double t64 = rounds(tiles(64, 64), 2.0 * cus) * (5.0 + 0.55 * ks);
+    if (t64 <= t128 && t64 <= t256 && t64 <= t192) return GNK_VARIANT_64X128;
+    if (t192 < 0.98 * t256 && t192 < t128) return VARIANT_192;
+    return t256 <= t128 ? GNK_VARIANT_256_W4 : GNK_VARIANT_128;
 }
 
 template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st) {
@@ -504,7 +525,7 @@ template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const Gr
     int variant = gnk_forced_variant_get();
     if (variant == GNK_VARIANT_256 && can_192) variant = VARIANT_192;
     else if ((variant != GNK_VARIANT_128 && variant != GNK_VARIANT_64X128 && variant != GNK_VARIANT_256_W4) || (variant == GNK_VARIANT_256_W4 && !can_w4))
-        variant = choose_variant(p, depth, can_w4, can_192);
+        variant = choose_variant(p, depth, b_kmajor, can_w4, can_192);
     if constexpr (OP == OP_I8) {
         if (variant == VARIANT_192)
             return b_kmajor ? launch_w4<PP2Cfg<true, true, OP, FA, FB, EPI_ROWCOL>, false, 192>(p, st)

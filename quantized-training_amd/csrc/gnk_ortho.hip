@@ -592,7 +592,8 @@ Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t ba
     };
     auto priced = [&](int bm, int kg, double slots, double per) { return Choice{bm, kg, ceil(tiles(bm) / slots) * per, tiles(bm) / slots * per}; };
     const Choice c256 = priced(256, 1, cus, 12.0 + 1.3 * ks), c128 = priced(128, 1, 2.0 * cus, 6.0 + 1.0 * ks);
-    const Choice c64 = priced(64, tiles(64) <= cus && ks >= 4.0 ? 2 : 1, 2.0 * cus, 4.0 + 0.4 * ks);
+    const bool kg2 = tiles(64) <= cus && ks >= 4.0;
+    const Choice c64 = priced(64, kg2 ? 2 : 1, 2.0 * cus, 4.0 + (kg2 ? 0.3 : 0.5) * ks);
     const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1, 5 and 6 force the 128, 256 and 64 tiles here as well
     if (forced == 6 || (forced != 1 && forced != 5 && c64.rounds_us <= c128.rounds_us && c64.rounds_us <= c256.rounds_us)) return c64;
     if (forced == 5 || (forced != 1 && c256.rounds_us <= c128.rounds_us)) return c256;
