@@ -212,7 +212,7 @@ template <bool KMAJOR, int BM> __device__ __forceinline__ v8h frag16(const char 
 
 // BM = 128: 2 x 2 waves of 64 x 64, two stages (64 KiB: two workgroups per CU).  BM = 64: 2 x 2 waves of 32 x 32 would halve the fragment reads, but the
 // stores want 64 columns per wave: 4 x 1 waves of 16 x 64; four stages (64 KiB) because few tiles are bound by the latency of a step, not by its work.
-// KG = 2 (BM = 64, at most one workgroup per CU): a second set of four waves with a ring of its own takes every other step of the contraction; the two
+// KG = 2 (at most one workgroup per CU): a second set of four waves with a ring of its own takes every other step of the contraction; the two
 // halves meet in LDS, in the same order on both sides, and then one set stores the tile and the other its mirror image.
 template <int BM> struct RingShape {
     static constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1, MT = BM / WM / 16, NST = BM == 128 ? 2 : 4, OPER = BM * 128, STAGE = 2 * OPER;
@@ -223,7 +223,7 @@ template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM>
 __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2))) product_ring_kernel(const Product p) {
     extern __shared__ __attribute__((aligned(16))) char smem_all[];
     typedef RingShape<BM> R;
-    static_assert(KG == 1 || (KG == 2 && BM == 64), "two sets of waves: 64 x 64 tiles");
+    static_assert(KG == 1 || KG == 2, "one or two sets of waves");
     typedef GemmCfg<BM, BM, R::WM, R::WN, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;     // fp32 accumulators and the epilogue's maps
     constexpr int MT = R::MT, NST = R::NST, PIECES = 2 * BM / 32;
     const int lane = threadIdx.x & 63;
@@ -281,12 +281,17 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
     }
     if constexpr (KG > 1) {
         __syncthreads();                                               // both rings are free
-        char *const mine = smem_all + kg * 16384, *const other = smem_all + (1 - kg) * 16384;
+        char *const mine = smem_all + kg * BM * BM * 4, *const other = smem_all + (1 - kg) * BM * BM * 4;      // at most both rings together
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *(GNK_LDS v4f *)(GNK_LDS char *)(mine + 16 * ((wave * 4 + j) * 64 + lane)) = acc[0][j];
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *(GNK_LDS v4f *)(GNK_LDS char *)(mine + 16 * (((wave * MT + i) * 4 + j) * 64 + lane)) = acc[i][j];
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[0][j] += *(const GNK_LDS v4f *)(const GNK_LDS char *)(other + 16 * ((wave * 4 + j) * 64 + lane));     // a + b = b + a
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                acc[i][j] += *(const GNK_LDS v4f *)(const GNK_LDS char *)(other + 16 * (((wave * MT + i) * 4 + j) * 64 + lane));     // a + b = b + a
     }
     float diag_sum = 0.0f;
     if constexpr (EPI == POLY) {
@@ -305,7 +310,7 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
     if constexpr (SYM) {
         if (tm != tn) {
             if constexpr (MT >= 4) {
-                store_mirror<MT>(p, b, acc, smem + R::LDS / 2 + wave * (64 * 32 * MT), lane, mw, nw);
+                if (kg == KG - 1) store_mirror<MT>(p, b, acc, smem + R::LDS / 2 + wave * (64 * 32 * MT), lane, mw, nw);
             } else {
                 // 16 rows per wave: transposed rows of 32 bytes would waste the stores; the four waves put theirs side by side first
                 // (KG = 2: the second set does, in its own ring's LDS; both pass the barrier)
@@ -591,7 +596,8 @@ Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t ba
         return (sym ? gm * (gm + 1) / 2 : gm * gn) * (double)batch;
     };
     auto priced = [&](int bm, int kg, double slots, double per) { return Choice{bm, kg, ceil(tiles(bm) / slots) * per, tiles(bm) / slots * per}; };
-    const Choice c256 = priced(256, 1, cus, 12.0 + 1.3 * ks), c128 = priced(128, 1, 2.0 * cus, 6.0 + 1.0 * ks);
+    const Choice c256 = priced(256, 1, cus, 12.0 + 1.3 * ks);
+    const Choice c128 = tiles(128) <= cus && ks >= 4.0 ? priced(128, 2, cus, 7.0 + 0.55 * ks) : priced(128, 1, 2.0 * cus, 6.0 + 1.0 * ks);
     const bool kg2 = tiles(64) <= cus && ks >= 4.0;
     const Choice c64 = priced(64, kg2 ? 2 : 1, 2.0 * cus, 4.0 + (kg2 ? 0.3 : 0.5) * ks);
     const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1, 5 and 6 force the 128, 256 and 64 tiles here as well
@@ -602,7 +608,7 @@ Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t ba
 
 template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p, const Choice &c, hipStream_t st) {
     if (c.bm == 256) return launch<256, 1, AK, BK, EPI, SYM>(p, st);
-    if (c.bm == 128) return launch<128, 1, AK, BK, EPI, SYM>(p, st);
+    if (c.bm == 128) return c.kg == 2 ? launch<128, 2, AK, BK, EPI, SYM>(p, st) : launch<128, 1, AK, BK, EPI, SYM>(p, st);
     if (c.kg == 2) return launch<64, 2, AK, BK, EPI, SYM>(p, st);
     return launch<64, 1, AK, BK, EPI, SYM>(p, st);
 }
