@@ -297,7 +297,7 @@ int gnk_grouped_scaled_mm_depth(const void *A, int a_dtype, const void *B, int b
  * rows; eager torch's `amax / 127` on a device, within 1.5 fp32 steps of gnk_quantize_int8's quotient),
  * q[t,c] = clip(round_half_even(x[t,c] / max(scale[e,c], eps)), -128, 127) with the unrounded scale, 0 for rows of no group.
  * x (T, C) with strides (sxt, sxc); q (T, C) and scale (E, C) contiguous; `ends` as above, or NULL for groups of T / E rows each (a stack of
- * matrices of that many rows).  sr, seed, offset as in gnk_quantize_int8 with
+ * matrices of that many rows).  T / 128 + E <= 65534.  sr, seed, offset as in gnk_quantize_int8 with
  * e = t * C + c + offset.  workspace: gnk_quantize_int8_grouped_workspace_bytes() bytes, 4-byte aligned, need not be cleared.
  */
 int64_t gnk_quantize_int8_grouped_workspace_bytes(int64_t T, int64_t E, int64_t C);

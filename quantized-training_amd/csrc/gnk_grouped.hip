@@ -131,6 +131,7 @@ extern "C" int gnk_grouped_scaled_mm_rows(const void *A, int a_dtype, const void
     if (!C || !row_scale || (E > 0 && (!ends || !col_scale || (K > 0 && (!A || !B))))) return gnk_fail(GNK_ERR_BAD_ARG, "%s: null pointer", name);
     rc = gnk_init();
     if (rc) return rc;
+    if (E == 0) K = 0;                       // no group: zeros, nothing is read
     const RowsPlan plan = plan_rows(A, B, T, E, N, K, sat, sak, sbe, sbk, sbn);
     rc = take_workspace(name, plan.a, plan.b, workspace, workspace_bytes);
     if (rc) return rc;

@@ -649,6 +649,11 @@ int launch_rowwise(const void *x, int8_t *q, void *scale, int64_t R, int64_t C, 
     return gnk_check_launch("quantize_int8 rowwise");
 }
 
+__global__ void __launch_bounds__(256) clear_words_kernel(unsigned *__restrict__ w, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) w[i] = 0u;
+}
+
 template <int DT, bool SR>
 int launch_colwise(const void *x, int8_t *q, void *scale, int64_t P, int64_t Q, int64_t ld, int64_t ldq, float eps,
                    uint64_t seed, uint64_t offset, unsigned *ws, int64_t ws_bytes, hipStream_t st) {
@@ -675,8 +680,8 @@ int launch_colwise(const void *x, int8_t *q, void *scale, int64_t P, int64_t Q, 
         return gnk_check_launch("quantize_int8 colwise");
     }
     // a workspace of one word per logical row (the minimum; gnk_quantize_int8_noalloc beyond what its scratch holds as partial rows):
-    // atomicMax into words cleared on the stream first
-    if (hipMemsetAsync(ws, 0, (size_t)Q * 4, st) != hipSuccess) return gnk_fail(GNK_ERR_LAUNCH, "quantize_int8: memset of workspace failed");
+    // atomicMax into words cleared on the stream first -- by a kernel: memset nodes of a captured graph have not always run on its replays
+    hipLaunchKernelGGL(clear_words_kernel, dim3((unsigned)((Q + 255) / 256)), dim3(256), 0, st, ws, Q);
     if (big) {
         hipLaunchKernelGGL((col_absmax_kernel<DT, 128>), grid, block, 0, st, (const char *)x, ws, P, Q, ld_bytes);
         if (nt) hipLaunchKernelGGL((col_quant_kernel<DT, SR, 128, true>), grid, block, 0, st, (const char *)x, q, scale, ws, P, Q, ld_bytes, ldq, eps, seed, offset, 0);
@@ -810,8 +815,7 @@ extern "C" int gnk_quantize_int8(const void *x, int x_dtype, int64_t R, int64_t 
 // The strided reduction needs one fp32 absmax word per logical row between its two kernels.  gnk_quantize_int8 takes
 // that buffer from the caller; here it lives in the code object: every GPU that loads the library holds its own copy
 // of `scratch` (GNK_NOALLOC_SCRATCH_BYTES, until the process ends) at its own address.  In host code the array's name
-// is only a handle: the device address comes from hipGetSymbolAddress, once per device, and is what the kernels and
-// hipMemsetAsync receive.
+// is only a handle: the device address comes from hipGetSymbolAddress, once per device, and is what the kernels receive.
 static __device__ __align__(256) unsigned char scratch[GNK_NOALLOC_SCRATCH_BYTES];
 static void *g_scratch_ptr[64];
 static std::mutex g_scratch_mu;
@@ -848,7 +852,7 @@ extern "C" int gnk_quantize_int8_noalloc(const void *x, int x_dtype, int64_t R, 
     if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64 || !g_scratch_ptr[dev])
         return gnk_fail(GNK_ERR_LAUNCH, "quantize_int8_noalloc: no scratch address for the current device");
     void *ptr = g_scratch_ptr[dev];   // the DEVICE address; never the array's name
-    // launch_colwise either writes every partial word it later reads (small reductions) or clears the words it uses (hipMemsetAsync on
+    // launch_colwise either writes every partial word it later reads (small reductions) or clears the words it uses (on
     // `stream`) before pass 1, so the previous call's maxima do not leak
     return gnk_quantize_int8(x, x_dtype, R, C, sxr, sxc, q, sqr, sqc, scale, eps, sr, seed, offset, ptr, GNK_NOALLOC_SCRATCH_BYTES, stream);
 }

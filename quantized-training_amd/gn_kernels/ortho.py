@@ -23,6 +23,7 @@ def orthogonalize(G: Tensor, *, steps: int = 5, coefficients: tuple[float, float
     Pushes all singular values of G towards 1; bf16, fp16 or fp32, the result has G's dtype and shape and is contiguous.  About 1.5e-3 of the
     result's norm off for the default five steps on singular values within a factor of 1000 of each other (fp32 inputs get no more: the
     intermediates are fp16).  The coefficients must keep the singular values below sqrt(2).  A matrix with a NaN or Inf comes out as NaN.
+    Not differentiable.
     """
     assert G.ndim >= 2 and G.dtype in _FLOAT
     assert 1 <= steps <= 100 and len(coefficients) == 3 and eps >= 0

@@ -355,6 +355,37 @@ def test_other_stream():
     assert all(torch.equal(o, want) for out in outs for o in out)
 
 
+@pytest.mark.parametrize("dt", ["int8", "e4m3"])
+def test_nothing_to_multiply(dt):
+    """No groups, no rows, no features to sum over: zeros of the right shape (scaled sums of nothing)."""
+    g = torch.Generator().manual_seed(7)
+    none, two = torch.zeros(0, dtype=torch.int32, device=DEV), offs_of([3, 2])
+    sc = lambda *s: scales(s, "bf16", g).to(DEV)  # noqa: E731
+    e8 = lambda *s: make8(s, dt, g).to(DEV)  # noqa: E731
+    for y in (gn_kernels.grouped_scaled_mm(e8(5, 17), e8(0, 17, 24), sc(5, 1), sc(0, 1, 24), none),
+              gn_kernels.grouped_scaled_mm(e8(5, 0), e8(2, 0, 24), sc(5, 1), sc(2, 1, 24), two)):
+        assert y.shape == (5, 24) and (y == 0).all()
+    assert gn_kernels.grouped_scaled_mm(e8(0, 16), e8(2, 16, 24), sc(0, 1), sc(2, 1, 24), offs_of([0, 0])).shape == (0, 24)
+    assert gn_kernels.grouped_scaled_mm(e8(5, 16), e8(2, 16, 0), sc(5, 1), sc(2, 1, 0), two).shape == (5, 0)
+    y = gn_kernels.grouped_scaled_mm(e8(32, 0), e8(0, 24), sc(2, 32, 1), sc(2, 1, 24), offs_of([0, 0]))
+    assert y.shape == (2, 32, 24) and (y == 0).all()
+    assert gn_kernels.grouped_scaled_mm(e8(32, 5), e8(5, 24), sc(0, 32, 1), sc(0, 1, 24), none).shape == (0, 32, 24)
+    q, s = gn_kernels.quantize_int8_grouped(torch.ones(5, 24, device=DEV), none)
+    assert s.shape == (0, 1, 24) and (q == 0).all()
+    q, s = gn_kernels.quantize_int8_grouped(torch.ones(0, 24, device=DEV), offs_of([0, 0]))
+    assert q.shape == (0, 24) and (s == 0).all()
+
+
+def test_one_weight_for_all_groups():
+    """B expanded over the groups: read in place."""
+    g = torch.Generator().manual_seed(8)
+    A, B = make8((50, 64), "int8", g), make8((1, 64, 32), "int8", g)
+    sA, sB = scales((50, 1), "bf16", g), scales((3, 1, 32), "bf16", g)
+    got = gn_kernels.grouped_scaled_mm(A.to(DEV), B.to(DEV).expand(3, 64, 32), sA.to(DEV), sB.to(DEV), offs_of([20, 0, 30]))
+    want, absum = rows_ref(A, B.expand(3, 64, 32), sA, sB, [20, 0, 30])
+    check(got, want, absum, "int8", "bf16", 64)
+
+
 def test_refusals_on_device():
     i8 = lambda *s: torch.zeros(*s, dtype=torch.int8, device=DEV)  # noqa: E731
     sc = lambda *s: torch.ones(*s, dtype=torch.bfloat16, device=DEV)  # noqa: E731

@@ -51,7 +51,7 @@ def formula(x, w, gy, sizes):
     return y, gx, gw
 
 
-@pytest.mark.parametrize("sizes,pad,K,N", [([5, 0, 130, 1], 3, 64, 48), ([300, 290], 0, 256, 512), ([0, 0], 4, 32, 16), ([7, 9], 0, 33, 21), ([1], 0, 16, 16)])
+@pytest.mark.parametrize("sizes,pad,K,N", [([5, 0, 130, 1], 3, 64, 48), ([300, 290], 0, 256, 512), ([0, 0], 4, 32, 16), ([7, 9], 0, 33, 21), ([1], 0, 16, 16), ([0, 0], 0, 32, 16), ([3], 2, 48, 1)])
 @pytest.mark.parametrize("op", [F.grouped_mm, torch._grouped_mm])
 def test_against_the_formula(sizes, pad, K, N, op):
     x, w, gy = make(sizes, pad, K, N)

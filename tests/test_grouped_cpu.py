@@ -196,6 +196,12 @@ def test_module_of_experts(cpu_ops, compiled, frozen):
         torch.testing.assert_close(grad, r.grad, rtol=1e-10, atol=1e-12)
 
 
+def test_every_way_to_transpose_a_stack_stays_wrapped():
+    w = MixedPrecisionLinearWeight(torch.randn(3, 4, 6), MixedPrecisionConfig())
+    for v in (w.transpose(-2, -1), w.transpose(1, 2), w.mT):
+        assert isinstance(v, MixedPrecisionLinearWeight) and v.shape == (3, 6, 4) and torch.equal(v._data, w._data.transpose(1, 2))
+
+
 def test_two_dimensional_weights_are_viewed_as_before():
     w = MixedPrecisionLinearWeight(torch.randn(4, 6), MixedPrecisionConfig())
     assert isinstance(w.t(), MixedPrecisionLinearWeight) and not isinstance(w.transpose(0, 1), MixedPrecisionLinearWeight)
