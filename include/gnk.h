@@ -266,8 +266,8 @@ int gnk_quantize_int8_noalloc(const void *x, int x_dtype, int64_t R, int64_t C, 
 /*
  * Products grouped by expert (no reference counterpart: its Linears are dense).  Rows are sorted by group; group e holds rows
  * ends[e - 1] .. ends[e] - 1 (ends[-1] = 0), `ends` being E int32 values ON THE DEVICE that do not decrease and do not exceed T -- nothing is
- * read back, so the calls can be captured into a graph and replayed with other sizes.  (Ends that break this give unspecified results, but no
- * access outside the operands: every end is clamped into [0, T].)  A group may be empty; rows behind the last end belong to no group.
+ * read back, so the calls can be captured into a graph and replayed with other sizes.  (Nothing checks that: a value below an earlier one counts
+ * as that one, a negative one as 0, one beyond T as T.)  A group may be empty; rows behind the last end belong to no group.
  *
  * gnk_grouped_scaled_mm_rows:   C[t,n] = cast_out( (f32(sum_k A[t,k] * B[e,k,n]) * row_scale[t]) * col_scale[e,n] ),  e the group of row t; rows
  *   of no group come out as zeros.  A (T, K) with strides (sat, sak); B (E, K, N) with strides (sbe, sbk, sbn); col_scale (E, N), or (E,) with

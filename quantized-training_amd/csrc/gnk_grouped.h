@@ -6,8 +6,8 @@
 // Group e holds rows ends[e - 1] .. ends[e] - 1 (ends[-1] = 0); rows behind the last end belong to no group and come out as zeros.
 // The host knows neither the sizes nor the number of tiles: it launches the most workgroups the sizes could need (sum of ceil(T_e / BM)
 // <= T / BM + E, one more for the rows behind), every workgroup scans the ends with one wave-wide prefix sum (64 groups per step) to find
-// its tile, and the surplus leaves at once.  Every end is clamped into [previous end, T], so that no value of `ends` reaches outside
-// the operands.  A group's tile is then an ordinary tile of gnk_gemm_kernel.h / gnk_gemm_w4.h: same LDS images, fragments and epilogue.
+// its tile, and the surplus leaves at once.  An end below an earlier one counts as that one, an end beyond T as T: the groups are disjoint and
+// in order whatever `ends` holds, so that no value of it reaches outside the operands, the tile counts above or the workspaces.  A group's tile is then an ordinary tile of gnk_gemm_kernel.h / gnk_gemm_w4.h: same LDS images, fragments and epilogue.
 #pragma once
 #include <math.h>
 
@@ -58,8 +58,20 @@ __device__ __forceinline__ int wave_prefix(int v) {
     return v;
 }
 
+// inclusive running maximum over the wave, of values >= 0
+__device__ __forceinline__ int wave_running_max(int v) {
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+    v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+    return v;
+}
+
 // Rows [lo, hi) of group g0 + lane; group E takes the rows behind the last end, groups beyond it none.  (T < 2^31.)  ends == NULL: equal groups.
-__device__ __forceinline__ void lane_group(const int *ends, int64_t E, int64_t T, int64_t g0, int lane, int &lo, int &hi) {
+// `before`: the largest end in front of group g0, 0 for g0 = 0; this call takes it on to g0 + 64.
+__device__ __forceinline__ void lane_group(const int *ends, int64_t E, int64_t T, int64_t g0, int lane, int &before, int &lo, int &hi) {
     const int64_t e = g0 + lane;
     if (!ends) {
         const int each = E > 0 ? (int)((unsigned)T / (unsigned)E) : 0;
@@ -67,9 +79,24 @@ __device__ __forceinline__ void lane_group(const int *ends, int64_t E, int64_t T
         hi = e < E ? lo + each : (e == E ? (int)T : lo);
         return;
     }
-    lo = e > 0 && e <= E ? (int)clamp_end(ends[e - 1], T) : 0;
-    hi = e < E ? (int)clamp_end(ends[e], T) : (e == E ? (int)T : lo);
-    if (hi < lo) hi = lo;
+    lo = wave_running_max(max(before, e > 0 && e <= E ? (int)clamp_end(ends[e - 1], T) : 0));
+    hi = max(lo, e < E ? (int)clamp_end(ends[e], T) : (e == E ? (int)T : 0));
+    before = __builtin_amdgcn_readlane(lo, 63);
+}
+
+// Rows [lo, hi) of group e <= E alone, the same for the whole wave
+__device__ __forceinline__ void one_group(const int *ends, int64_t E, int64_t T, int64_t e, int lane, int &lo, int &hi) {
+    if (!ends) {
+        const int each = E > 0 ? (int)((unsigned)T / (unsigned)E) : 0;
+        lo = (int)e * each;
+        hi = e < E ? lo + each : (int)T;
+        return;
+    }
+    const int own = e < E ? (int)clamp_end(ends[e], T) : (int)T;
+    int most = 0;
+    for (int64_t i = lane; i < e; i += 64) most = max(most, (int)clamp_end(ends[i], T));
+    lo = __builtin_amdgcn_readlane(wave_running_max(most), 63);
+    hi = max(lo, uniform(own));
 }
 
 // Every group (and the rows behind the last one) is cut into pieces of 1 << sh rows (sh = -192: of 192 rows), numbered in group order.
@@ -80,10 +107,10 @@ __device__ __forceinline__ int pieces_of(int rows, int sh) {
 }
 
 __device__ __forceinline__ int count_pieces(const int *ends, int64_t E, int64_t T, int lane, int sh) {
-    int total = 0;
+    int total = 0, end = 0;
     for (int64_t g0 = 0; g0 <= E; g0 += 64) {
         int lo, hi;
-        lane_group(ends, E, T, g0, lane, lo, hi);
+        lane_group(ends, E, T, g0, lane, end, lo, hi);
         total += __builtin_amdgcn_readlane(wave_prefix(pieces_of(hi - lo, sh)), 63);
     }
     return total;
@@ -93,10 +120,10 @@ __device__ __forceinline__ int count_pieces(const int *ends, int64_t E, int64_t 
 // number of pieces of 1 << sh2 rows in the groups in front of it.
 struct Piece { int e, idx, lo, hi, first2; };
 __device__ __forceinline__ Piece find_piece(const int *ends, int64_t E, int64_t T, int lane, int sh, int want, int sh2) {
-    int before = 0, before2 = 0;
+    int before = 0, before2 = 0, end = 0;
     for (int64_t g0 = 0; g0 <= E; g0 += 64) {
         int l, h;
-        lane_group(ends, E, T, g0, lane, l, h);
+        lane_group(ends, E, T, g0, lane, end, l, h);
         const int n = pieces_of(h - l, sh), n2 = pieces_of(h - l, sh2);
         const int incl = wave_prefix(n) + before, incl2 = wave_prefix(n2) + before2;
         const unsigned long long hit = __ballot(incl > want);
@@ -118,8 +145,8 @@ __device__ __forceinline__ Tile rows_tile(const GroupedParams &p, int grid_n, in
     static_assert(BM == 256 || BM == 192 || BM == 128 || BM == 64, "row tiles");
     Tile t;
     if (p.E < 64) {                          // all groups in one wave: one load and one prefix sum give the count and the place
-        int l, h;
-        lane_group(p.ends, p.E, p.T, 0, lane, l, h);
+        int l, h, end = 0;
+        lane_group(p.ends, p.E, p.T, 0, lane, end, l, h);
         const int n = pieces_of(h - l, SH), incl = wave_prefix(n), grid_m = __builtin_amdgcn_readlane(incl, 63);
         t.work = (int64_t)blockIdx.x < (int64_t)grid_m * grid_n;
         if (!t.work) return t;
@@ -143,7 +170,7 @@ __device__ __forceinline__ Tile rows_tile(const GroupedParams &p, int grid_n, in
     return t;
 }
 
-__device__ __forceinline__ Tile depth_tile(const GroupedParams &p, int grid_m, int grid_n) {
+__device__ __forceinline__ Tile depth_tile(const GroupedParams &p, int grid_m, int grid_n, int lane) {
     Tile t;
     const int per = grid_m * grid_n;
     int tm, tn;
@@ -156,9 +183,9 @@ __device__ __forceinline__ Tile depth_tile(const GroupedParams &p, int grid_m, i
     tm = first + r % gsz;
     tn = r / gsz;
     t.tm = tm; t.tn = tn;
-    t.lo = t.e > 0 ? clamp_end(p.ends[t.e - 1], p.T) : 0;
-    t.hi = clamp_end(p.ends[t.e], p.T);
-    if (t.hi < t.lo) t.hi = t.lo;
+    int lo, hi;
+    one_group(p.ends, p.E, p.T, t.e, lane, lo, hi);
+    t.lo = lo; t.hi = hi;
     t.work = true;
     return t;
 }
@@ -210,7 +237,7 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cf
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
-    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
+    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
     if (!tile.work) return;
     const int64_t m0 = (int64_t)tile.tm * Cfg::BM, n0 = (int64_t)tile.tn * Cfg::BN;
     if (!DEPTH && tile.e == gp.E) {      // rows of no group
@@ -284,7 +311,7 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(2)
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
-    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
+    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
     if (!tile.work) return;
     const int64_t m0 = (int64_t)tile.tm * Cfg::BM, n0 = (int64_t)tile.tn * Cfg::BN;
     if (!DEPTH && tile.e == gp.E) {
@@ -364,7 +391,7 @@ __global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
-    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n) : rows_tile<BM>(gp, gp.g.grid_n, lane);
+    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<BM>(gp, gp.g.grid_n, lane);
     if (!tile.work) return;
     constexpr int WTM = BM / 2;
     const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * 256;

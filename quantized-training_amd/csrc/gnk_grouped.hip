@@ -90,6 +90,8 @@ int check_call(const char *name, int a_dtype, int b_dtype, int out_dtype, int sc
     if (T >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "%s: group ends are 32-bit, %lld rows are too many", name, (long long)T);
     if (E >= (1LL << 20)) return gnk_fail(GNK_ERR_UNSUPPORTED, "%s: %lld groups are too many", name, (long long)E);
     if (d0 > MAX_PITCH || d1 > MAX_PITCH) return gnk_fail(GNK_ERR_UNSUPPORTED, "%s: feature sizes beyond %lld are not supported", name, (long long)MAX_PITCH);
+    if ((double)(E > 0 ? E : 1) * (double)up16(d0) * (double)up16(d1) > 4.0e18)      // what a copy of the operands would take, in 64 bits
+        return gnk_fail(GNK_ERR_UNSUPPORTED, "%s: %lld groups of %lld x %lld are too many", name, (long long)E, (long long)d0, (long long)d1);
     const bool i8 = a_dtype == GNK_I8 && b_dtype == GNK_I8, f8 = gnk_is_f8(a_dtype) && gnk_is_f8(b_dtype);
     if (!i8 && !f8) return gnk_fail(GNK_ERR_BAD_ARG, "%s: operands must be both int8 or both fp8 (got dtype codes %d, %d)", name, a_dtype, b_dtype);
     if (!gnk_is_float_dtype(scale_dtype)) return gnk_fail(GNK_ERR_BAD_ARG, "%s: scale dtype code %d is not bf16/f16/f32", name, scale_dtype);
@@ -304,7 +306,7 @@ group_quant_once_kernel(const char *__restrict__ x, int8_t *__restrict__ q, void
     const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
     const int64_t col0 = ((int64_t)blockIdx.x * CL + cl) * VEC, e = blockIdx.y;
     int lo, hi;
-    lane_group(ends, E, T, e, 0, lo, hi);
+    one_group(ends, E, T, e, threadIdx.x & 63, lo, hi);
     if (e == E) {                                // rows of no group
         if (col0 < C)
             for (int64_t r = lo + rl; r < hi; r += RL)
@@ -414,9 +416,10 @@ group_quant_kernel(const char *__restrict__ x, int8_t *__restrict__ q, void *__r
     const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
     const int64_t col0 = ((int64_t)blockIdx.x * CL + cl) * VEC;
     if (blockIdx.y == 0) {                       // groups without rows have no piece: their scale (0) is written here
+        int end = 0;
         for (int64_t g0 = 0; g0 < E; g0 += 64) {
             int l, h;
-            lane_group(ends, E, T, g0, lane, l, h);
+            lane_group(ends, E, T, g0, lane, end, l, h);
             unsigned long long none = __ballot(g0 + lane < E && h == l);
             while (none) {
                 const int64_t g = g0 + __builtin_ctzll(none);

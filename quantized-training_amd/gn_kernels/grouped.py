@@ -36,7 +36,7 @@ def grouped_scaled_mm(A: Tensor, B: Tensor, scale_A: Tensor, scale_B: Tensor, of
     A and B are both int8, or any mix of float8_e4m3fn / float8_e5m2; any strides, but operands whose contiguous extent is a multiple of
     16 and whose rows are 16-byte aligned are read where they lie: A along K and B along K or N (rows form), A along M and B along N (second
     form).  Others are copied first.  scales are contiguous, the result has their dtype.  offs: int32 on the same device, not decreasing,
-    at most T (not checked: that would wait for the device).
+    at most T (not checked, as that would wait for the device: a value below an earlier one counts as that one, one beyond T as T).
     """
     dt, E = A.dtype, offs.shape[0]
     assert (dt is torch.int8 and B.dtype is torch.int8) or (dt in _FP8 and B.dtype in _FP8)

@@ -214,6 +214,61 @@ def test_ends_that_do_not_fit_stay_inside(shift):
     assert torch.equal(q[:32].cpu(), wq) and torch.equal(s[0].cpu(), ws[0])
 
 
+# ends that decrease, with the sizes that they stand for: a value below an earlier one counts as that one, negative ones as 0, ones beyond T as T
+DECREASING = {
+    "one_step_back": ([300, 120, 700], 1100),
+    "back_and_forth": ([2500, 0] * 50, 2500),                       # read as pairs of ends, every second group would hold all rows
+    "back_over_a_wave": ([1] * 62 + [2300, 40] + [30] * 70 + [2400], 2500),
+    "below_and_beyond": ([-7, 50, -2 ** 31, 2 ** 31 - 1, 3], 2200),
+}
+
+
+def sizes_of(ends, T):
+    lo, sizes = 0, []
+    for e in ends:
+        hi = max(lo, min(max(e, 0), T))
+        sizes.append(hi - lo)
+        lo = hi
+    return sizes
+
+
+@pytest.mark.parametrize("name", list(DECREASING))
+@pytest.mark.parametrize("variant", [0, 1, 5, 6])
+def test_ends_that_decrease(name, variant):
+    ends, T = DECREASING[name]
+    sizes, E, g = sizes_of(ends, T), len(ends), torch.Generator().manual_seed(4)
+    assert sum(sizes) <= T and min(sizes) >= 0
+    offs = torch.tensor(ends, dtype=torch.int32, device=DEV)
+    A, B, D = make8((T, 256), "int8", g), make8((1, 256, 48), "int8", g), make8((T, 32), "int8", g)
+    sA, sB, sR = scales((T, 1), "f32", g), scales((E, 1, 48), "f32", g), scales((E, 256, 1), "f32", g)
+    sD = scales((E, 1, 32), "f32", g)
+    L = _cabi.load()
+    L.gnk_set_gemm_variant(variant)
+    try:
+        rows = gn_kernels.grouped_scaled_mm(A.to(DEV), B.to(DEV).expand(E, 256, 48), sA.to(DEV), sB.to(DEV), offs)
+        depth = gn_kernels.grouped_scaled_mm(A.to(DEV).t(), D.to(DEV), sR.to(DEV), sD.to(DEV), offs)
+        torch.cuda.synchronize()
+    finally:
+        L.gnk_set_gemm_variant(-1)
+    check(rows, *rows_ref(A, B.expand(E, 256, 48), sA, sB, sizes), "int8", "f32", 256)
+    assert (rows[sum(sizes):] == 0).all()
+    check(depth, *depth_ref(A.t(), D, sR, sD, sizes), "int8", "f32", T)
+
+
+@pytest.mark.parametrize("name", list(DECREASING))
+@pytest.mark.parametrize("T_extra", [-1000, 0, 3000])               # one launch, two, and pieces of 256 rows for the maxima
+def test_quantize_ends_that_decrease(name, T_extra):
+    ends, T = DECREASING[name]
+    T += T_extra
+    if T <= 0:
+        T = 500
+    sizes = sizes_of(ends, T)
+    x = torch.randn(T, 40, generator=torch.Generator().manual_seed(5))
+    q, s = gn_kernels.quantize_int8_grouped(x.to(DEV), torch.tensor(ends, dtype=torch.int32, device=DEV))
+    wq, ws = quant_ref(x, sizes)
+    assert torch.equal(q.cpu(), wq) and torch.equal(s.cpu(), ws)
+
+
 # ------------------------------------------------------------------------------------------------ quantizer
 def quant_ref(x, sizes):
     """Group by group on the host, bit for bit: scale = amax * fl(1 / 127) in fp32, q = clip(rne(x / max(scale, eps))); a NaN quotient gives
