@@ -19,6 +19,7 @@ def _plain(t: Tensor) -> Tensor:
 class Muon(torch.optim.Optimizer):
     """m <- momentum m + g;  u = orthogonalize(g + momentum m) (nesterov) or orthogonalize(m);  p <- (1 - lr weight_decay) p - lr max(1, rows / cols)^0.5 u.
 
+    The momentum m is held in fp32 whatever the weights' type (a bf16 sum would lose gradients below 2^-8 of it); u is rounded once, to the gradient's type.
     Weights of one shape and type share a call of `orthogonalize`: equal layers fill the chip where one matrix does not."""
 
     def __init__(self, params, lr: float = 0.02, *, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
@@ -26,10 +27,21 @@ class Muon(torch.optim.Optimizer):
         if lr < 0 or not 0 <= momentum < 1 or weight_decay < 0:
             raise ValueError(f"Muon: lr {lr}, momentum {momentum}, weight_decay {weight_decay}")
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=tuple(coefficients), eps=eps))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.ndim not in (2, 3) or not p.is_floating_point():
-                    raise ValueError(f"Muon takes matrices and stacks of matrices, not a {p.dtype} parameter of shape {tuple(p.shape)}")
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.ndim not in (2, 3) or not p.is_floating_point() or 0 in p.shape[-2:]:
+                self.param_groups.pop()
+                raise ValueError(f"Muon takes matrices and stacks of matrices, not a {p.dtype} parameter of shape {tuple(p.shape)}")
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(saved, params):          # the base class rounds floating-point state to the weight's type
+            if "momentum" in state_dict["state"].get(i, {}):
+                self.state[p]["momentum"] = state_dict["state"][i]["momentum"].detach().to(p.device, torch.float32, copy=True)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -45,9 +57,9 @@ class Muon(torch.optim.Optimizer):
                 g = _plain(p.grad)
                 state = self.state[p]
                 if "momentum" not in state:
-                    state["momentum"] = torch.zeros_like(g, memory_format=torch.contiguous_format)
+                    state["momentum"] = torch.zeros_like(g, dtype=torch.float32, memory_format=torch.contiguous_format)
                 m = state["momentum"].mul_(group["momentum"]).add_(g)
-                u = g.add(m, alpha=group["momentum"]) if group["nesterov"] else m
+                u = (torch.add(g, m, alpha=group["momentum"]) if group["nesterov"] else m).to(g.dtype)
                 alike.setdefault((tuple(p.shape[-2:]), u.dtype, u.device), []).append((p, u))
             for (shape, _, _), pairs in alike.items():
                 # one stack of all matrices of this shape; a single one goes as it is

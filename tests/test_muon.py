@@ -97,6 +97,34 @@ def test_refuses_what_it_cannot_update():
         Muon([nn.Parameter(torch.zeros(4, 4))], lr=-1.0)
 
 
+def test_momentum_is_fp32_and_survives_a_checkpoint(cpu_op):
+    """Gradients of 1 and then of 2^-10, which a bf16 momentum near 1 would lose: the state is the fp32 sum, before and after a reload."""
+    make = lambda: Muon([nn.Parameter(torch.zeros(2, 4, 4, dtype=torch.bfloat16)), nn.Parameter(torch.zeros(4, 6, dtype=torch.bfloat16))], momentum=1.0 - 2.0 ** -8)  # noqa: E731
+    opt = make()
+    for value in (1.0, 2.0 ** -10):
+        for p in opt.param_groups[0]["params"]:
+            p.grad = torch.full_like(p, value)
+        opt.step()
+    want = 1.0 - 2.0 ** -8 + 2.0 ** -10                       # exact in fp32
+    other = make()
+    other.load_state_dict(opt.state_dict())
+    for o in (opt, other):
+        for p in o.param_groups[0]["params"]:
+            m = o.state[p]["momentum"]
+            assert m.dtype is torch.float32 and (m == want).all()
+    assert all(other.state[a]["momentum"] is not opt.state[b]["momentum"]
+               for a, b in zip(other.param_groups[0]["params"], opt.param_groups[0]["params"]))
+
+
+def test_refuses_empty_matrices_and_bad_groups():
+    with pytest.raises(ValueError):
+        Muon([nn.Parameter(torch.zeros(0, 4))])
+    opt = Muon([nn.Parameter(torch.zeros(4, 4))])
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [nn.Parameter(torch.zeros(4))]})
+    assert len(opt.param_groups) == 1
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("quantize", ["none", "mixed_precision"])
 def test_training_harness_runs_on_the_device(quantize):
