@@ -42,7 +42,7 @@ typedef enum gnk_status {
 /* Library identification.  Rule: GNK_ABI_VERSION goes up by one whenever an entry point is added, removed, or changes its arguments or
  * the meaning of an argument or return code (kernel changes behind an unchanged signature do not count); a binding compares
  * gnk_abi_version() of the loaded library with the GNK_ABI_VERSION it was written against and refuses a mismatch.
- *   1: round 1.   2: rounds 2-3 -- gnk_scaled_mm_ws / gnk_scaled_mm_t, the fused quantize pair, gnk_quantize_int8_noalloc, the MX and BitNet
+ *   1: the first one.   2: gnk_scaled_mm_ws / gnk_scaled_mm_t, the fused quantize pair, gnk_quantize_int8_noalloc, the MX and BitNet
  *      entry points added; gnk_set_debug_flags removed from the shipped library; gnk_set_gemm_variant accepts 5, 6, -2 and -3; gnk_set_tile_rescale added.
  *   3: the products grouped by expert and their quantizer (gnk_grouped_scaled_mm_rows / _depth, gnk_quantize_int8_grouped).
  *   4: gnk_orthogonalize. */
@@ -228,7 +228,8 @@ int gnk_bitnet_unpack_i2(const void *x, int64_t nbytes, void *out, void *stream)
 /*
  * Test / tuning hook (no reference counterpart): force a GEMM kernel variant for subsequent
  * calls on this thread.  variant < 0 restores the built-in heuristic.  Returns the previous
- * value.  Variants are listed in csrc/gnk_gemm_dispatch.h.
+ * value.  Variants are listed in csrc/gnk_gemm_dispatch.h.  The grouped products and gnk_orthogonalize read it too, where the forced tile can run: 1, 5
+ * and 6 are their 128 x 128, 256 x 256 and 64 x 64 tiles, 0 the grouped int8 products' 192 x 256.
  */
 int gnk_set_gemm_variant(int variant);
 

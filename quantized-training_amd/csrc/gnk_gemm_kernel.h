@@ -407,8 +407,8 @@ template <class Cfg> struct EpiScales {
         static_assert(ORDER == 0 || ORDER == 1, "multiply order is a compile-time choice");
         return __fmul_rn(__fmul_rn(a, cs[j][r]), rs[i]);
     }
-    // Elements r, r + 1 of one lane's tile row at once: the two scale multiplies as v_pk_mul_f32 (each half rounded like v_mul_f32, so
-    // the bits do not change; the staged epilogues are VALU-issue bound with one or two waves per SIMD: 5.1 us of a 49 us 4096^3 launch).
+    // Elements r, r + 1 of one lane's tile row at once: the two scale multiplies side by side (packed fp32 instructions are switched
+    // off in the Makefile; the staged epilogues are VALU-issue bound with one or two waves per SIMD: 5.1 us of a 49 us 4096^3 launch).
     template <int ORDER, class AccT_>
     __device__ __forceinline__ v2f value2(const GemmParams &p, const AccT_ &acc, const v4f *accf, int i, int j, int r) const {
         if constexpr (Cfg::EPI == EPI_TILE) return (v2f){(*accf)[r], (*accf)[r + 1]};

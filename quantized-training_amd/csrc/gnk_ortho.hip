@@ -8,13 +8,15 @@
 //   X_0 as G 2^p with |G|_F 2^p in [2^14, 2^15): no rounding at all for bf16 and fp16 inputs (1 / |G|_F goes into the products' factors);
 //   later X as X 2^10, S as S 2^10, Q - mu I as (Q - mu I) 2^s with |a| + 2 |b| + 4 |c| < 2^(14 - s): nothing overflows, and what underflows is
 //   below 2^-24.  mu = p(mean of S's diagonal), p(s) = a + b s + c s^2, is about the mean of Q's diagonal, which otherwise carries most of Q's rounding error:
-//   three quarters of the whole result's for flat matrices (36 x 2230: 2.6e-3 -> 1.1e-3).  mu X is added in fp32 where Q X is stored.  From 512 rows on the
+//   three quarters of the whole result's for flat matrices (36 x 2230: 2.6e-3 -> 2.0e-3 of the result's norm, 1.7e-3 of which is the output's bf16).  mu X is added in fp32 where Q X is stored.  From 512 rows on the
 //   rounding of X is most of the error (512 x 512: 1.4e-3 of 1.6e-3) and the second read of X costs 15 % of that product: mu = 0 there.
 // Shapes are padded with zeros to multiples of 128 in the workspace: zero rows and columns stay zero through every product.
 //
 // The products: `wide` S = X X^T reads both operands along K, Q X reads X as it lies (N-contiguous, transposed on the way out of LDS); `tall` S = X^T X
 // reads X as it lies on both sides, X Q reads along K (Q is symmetric); S^2 = S S^T.  So nothing is ever transposed in memory.
 // Bound: the matrix cores, m^2 n + m^3 + 2 m^2 n operations per step (m <= n; S and S^2 are symmetric).
+// Measured, bf16, five steps: 8 x 2048 x 5632 2.88 ms, 1.1 PFLOP/s (a large fp16 product reaches 1.42); 2048 x 5632 650 us; 2048 x 2048 428 us; 999 x 333 120 us,
+// 64 x 64 67 us: 17 dependent launches of 3-10 us, 0.8 us apart.  (Requesting the epilogue's reads and the diagonal ahead of the loop changed nothing there.)
 #include <math.h>
 #include <string.h>
 
@@ -214,6 +216,8 @@ template <bool KMAJOR, int BM> __device__ __forceinline__ v8h frag16(const char 
 // stores want 64 columns per wave: 4 x 1 waves of 16 x 64; four stages (64 KiB) because few tiles are bound by the latency of a step, not by its work.
 // KG = 2 (at most one workgroup per CU): a second set of four waves with a ring of its own takes every other step of the contraction; the two
 // halves meet in LDS, in the same order on both sides, and then one set stores the tile and the other its mirror image.
+// Bound by latency: a launch with one step takes 3 us, each further 64-k step of a set 0.7 (fragment reads, barrier), so 333 x 333 over K = 1024 takes 8.2 us.
+// Two sets instead of one, tiles of 128: 2048 x 2048 530 -> 428 us, 2048 x 5632 749 -> 652 us (whole calls).
 template <int BM> struct RingShape {
     static constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1, MT = BM / WM / 16, NST = BM == 128 ? 2 : 4, OPER = BM * 128, STAGE = 2 * OPER;
     static constexpr int LDS = NST * STAGE;
@@ -340,6 +344,7 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
 
 // ------------------------------------------------------------------------------ 256 x 256 tiles, one wave per SIMD (gnk_gemm_w4.h)
 // The 8-bit loop with 16-bit fragments: a 64-byte stage holds 32 k, so K must be a multiple of 128 (four stages per iteration).
+// 8 x 2048 x 5632: the matrix pipes are busy 65 % (S), 50 % (Q, the shortest contraction) and 71 % (X) of the time.
 template <bool KMAJOR> struct StagerW4H {
     const char *base;
     unsigned off[8];
@@ -453,7 +458,7 @@ template <int DT, int V> __device__ __forceinline__ void load_floats(const void 
 }
 template <int DT> constexpr int VEC = DT == GNK_F32 ? 4 : 8;
 
-// Partial sums of squares: HBM-bound.  fp64: the squares of any fp32 fit, and nothing is lost on the way.
+// Partial sums of squares: HBM-bound (8 x 2048 x 5632 bf16: 38 us, 4.8 TB/s).  fp64: the squares of any fp32 fit, and nothing is lost on the way.
 template <int DT, int V>
 __global__ void __launch_bounds__(256) square_sum_kernel(const void *__restrict__ G, double *__restrict__ parts, int64_t numel, int nparts) {
     const int64_t b = blockIdx.y, words = numel / V, per = (words + nparts - 1) / nparts, i0 = (int64_t)blockIdx.x * per, i1 = i0 + per < words ? i0 + per : words;
@@ -480,7 +485,8 @@ __global__ void __launch_bounds__(256) square_sum_kernel(const void *__restrict_
     if (threadIdx.x == 0) parts[b * nparts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// G 2^p as fp16, padded; fac[b] = {factor of step 0's S, factor of step 0's update}: what takes G 2^p back to X_0.  HBM-bound.
+// G 2^p as fp16, padded; fac[b] = {factor of step 0's S, factor of step 0's update}: what takes G 2^p back to X_0.  HBM-bound (8 x 2048 x 5632
+// bf16: 59 us, 6.3 TB/s; most of G is still in the last-level cache).
 template <int DT, int V>
 __global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G, unsigned short *__restrict__ X, const double *__restrict__ parts, float *__restrict__ fac,
                                                       int64_t rows, int64_t cols, int64_t rows_p, int64_t cols_p, int nparts, float eps) {
