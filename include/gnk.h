@@ -45,8 +45,8 @@ typedef enum gnk_status {
  *   1: the first one.   2: gnk_scaled_mm_ws / gnk_scaled_mm_t, the fused quantize pair, gnk_quantize_int8_noalloc, the MX and BitNet
  *      entry points added; gnk_set_debug_flags removed from the shipped library; gnk_set_gemm_variant accepts 5, 6, -2 and -3; gnk_set_tile_rescale added.
  *   3: the products grouped by expert and their quantizer (gnk_grouped_scaled_mm_rows / _depth, gnk_quantize_int8_grouped).
- *   4: gnk_orthogonalize. */
-#define GNK_ABI_VERSION 4
+ *   4: gnk_orthogonalize.   5: gnk_grouped_scaled_mm_depth_split_bytes. */
+#define GNK_ABI_VERSION 5
 int gnk_abi_version(void);
 
 /* Message for the last non-zero status returned on this thread ("" if none). */
@@ -280,6 +280,8 @@ int gnk_quantize_int8_noalloc(const void *x, int x_dtype, int64_t R, int64_t C, 
  * workspace: gnk_grouped_scaled_mm_*_workspace_bytes() bytes, 16-byte aligned.  0 when the kernels can read both operands where they lie (16-byte
  * aligned bases and pitches, the contiguous extent a multiple of 16: rows form A K-contiguous and B K- or N-contiguous, depth form A M-contiguous and
  * B N-contiguous); otherwise room for a padded copy of those that they cannot.  Overlapping calls need a workspace each.
+ * The depth form takes gnk_grouped_scaled_mm_depth_split_bytes() bytes more (beyond the former rounded up to 16) if the caller has them: where few tiles share
+ * long contractions it cuts those into parts and adds their sums up from there, in a fixed order; without that room it does not.
  */
 int64_t gnk_grouped_scaled_mm_rows_workspace_bytes(const void *A, const void *B, int64_t T, int64_t E, int64_t N, int64_t K, int64_t sat, int64_t sak,
                                                    int64_t sbe, int64_t sbk, int64_t sbn);
@@ -289,6 +291,7 @@ int gnk_grouped_scaled_mm_rows(const void *A, int a_dtype, const void *B, int b_
                                void *stream);
 int64_t gnk_grouped_scaled_mm_depth_workspace_bytes(const void *A, const void *B, int64_t T, int64_t M, int64_t N, int64_t sam, int64_t sat, int64_t sbt,
                                                     int64_t sbn);
+int64_t gnk_grouped_scaled_mm_depth_split_bytes(int64_t T, int64_t E, int64_t M, int64_t N);
 int gnk_grouped_scaled_mm_depth(const void *A, int a_dtype, const void *B, int b_dtype, void *C, int out_dtype, const void *row_scale,
                                 const void *col_scale, int scale_dtype, int col_scale_is_scalar, const int32_t *ends, int64_t T, int64_t E, int64_t M,
                                 int64_t N, int64_t sam, int64_t sat, int64_t sbt, int64_t sbn, void *workspace, int64_t workspace_bytes, void *stream);

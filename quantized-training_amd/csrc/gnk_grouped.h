@@ -22,6 +22,9 @@ struct GroupedParams {
     int64_t b_group;         // rows: bytes from one group's B to the next
     int64_t ext_a, ext_b;    // depth: staged extents of A (>= M) and B (>= N); rows: ext_b (>= N) -- multiples of 16 for M/N-major operands
     int out_bytes, scale_bytes;
+    int splits;              // depth: parts that a group's contraction is cut into (1: none); their sums go to `slab`, part by part
+    void *slab;
+    int64_t slab_bytes;
 };
 
 typedef int (*gnk_grouped_launcher)(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st);
@@ -39,6 +42,7 @@ using namespace gnk_gemm;
 // One tile: rows [lo, hi) of group e (e == E: the rows behind the last group), row tile tm of that group, column tile tn.
 struct Tile {
     int e, tm, tn;
+    int part;                // depth: which part of the group's rows [lo, hi) are
     int64_t lo, hi;
     bool work;               // false: a surplus workgroup
 };
@@ -170,14 +174,18 @@ __device__ __forceinline__ Tile rows_tile(const GroupedParams &p, int grid_n, in
     return t;
 }
 
-__device__ __forceinline__ Tile depth_tile(const GroupedParams &p, int grid_m, int grid_n, int lane) {
+// STEP: rows per step of the kernel's loop; a part is a whole number of them
+template <int STEP> __device__ __forceinline__ Tile depth_tile(const GroupedParams &p, int grid_m, int grid_n, int lane) {
     Tile t;
-    const int per = grid_m * grid_n;
+    const int per = grid_m * grid_n * p.splits;
     int tm, tn;
-    // groups in order; within one, the strips of tile_of_block without its XCD split (a group's operands fit every L2 badly anyway)
+    // groups in order; within one, the strips of tile_of_block without its XCD split (a group's operands fit every L2 badly anyway).  The parts (a power of
+    // two of them) change fastest, so that the tiles that read the same rows run on the same XCDs.
     const int wg = (int)blockIdx.x;
     t.e = wg / per;
-    const int in = wg - t.e * per;
+    int in = wg - t.e * per;
+    t.part = in % p.splits;
+    in /= p.splits;
     constexpr int GROUP_M = 4;
     const int width = GROUP_M * grid_n, strip = in / width, first = strip * GROUP_M, gsz = min(grid_m - first, GROUP_M), r = in - strip * width;
     tm = first + r % gsz;
@@ -186,6 +194,11 @@ __device__ __forceinline__ Tile depth_tile(const GroupedParams &p, int grid_m, i
     int lo, hi;
     one_group(p.ends, p.E, p.T, t.e, lane, lo, hi);
     t.lo = lo; t.hi = hi;
+    if (p.splits > 1) {
+        const int64_t steps = (t.hi - t.lo + STEP - 1) / STEP, each = (steps + p.splits - 1) / p.splits * STEP;
+        t.lo = t.lo + t.part * each < t.hi ? t.lo + t.part * each : t.hi;
+        t.hi = t.lo + each < t.hi ? t.lo + each : t.hi;
+    }
     t.work = true;
     return t;
 }
@@ -199,7 +212,7 @@ __device__ __forceinline__ GemmParams tile_params(const GroupedParams &p, const 
         g.K = rows;
         g.A += t.lo * g.lda;
         g.B += t.lo * g.ldb;
-        g.C = (char *)g.C + (int64_t)t.e * g.M * g.N * p.out_bytes;
+        g.C = (char *)g.C + ((int64_t)t.part * p.E + t.e) * g.M * g.N * p.out_bytes;
         g.s0 = (const char *)g.s0 + (int64_t)t.e * g.M * p.scale_bytes;
         ext_a = p.ext_a;
     } else {
@@ -238,7 +251,7 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cf
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
-    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
+    const Tile tile = DEPTH ? depth_tile<GNK_BK>(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
     if (!tile.work) return;
     const int64_t m0 = (int64_t)tile.tm * Cfg::BM, n0 = (int64_t)tile.tn * Cfg::BN;
     if (!DEPTH && tile.e == gp.E) {      // rows of no group
@@ -250,7 +263,7 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cf
 
     char *const As0 = smem;
     char *const Bs0 = smem + 2 * Cfg::A_BYTES;
-    ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, EPI_ROWCOL> spf;
+    ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, Cfg::EPI> spf;
     spf.issue(p, m0, n0);
     Stager<Cfg::A_KMAJOR, Cfg::BM, Cfg::NW> sa;
     Stager<Cfg::B_KMAJOR, Cfg::BN, Cfg::NW> sb;
@@ -314,7 +327,7 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(2)
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
-    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
+    const Tile tile = DEPTH ? depth_tile<GNK_BK>(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
     if (!tile.work) return;
     const int64_t m0 = (int64_t)tile.tm * Cfg::BM, n0 = (int64_t)tile.tn * Cfg::BN;
     if (!DEPTH && tile.e == gp.E) {
@@ -397,7 +410,7 @@ __global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1;
-    const Tile tile = DEPTH ? depth_tile(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<BM>(gp, gp.g.grid_n, lane);
+    const Tile tile = DEPTH ? depth_tile<256>(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<BM>(gp, gp.g.grid_n, lane);
     if (!tile.work) return;
     constexpr int WTM = BM / 2;
     const int64_t m0 = (int64_t)tile.tm * BM, n0 = (int64_t)tile.tn * 256;
@@ -411,7 +424,11 @@ __global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
     const int t = threadIdx.x;
     const int64_t mi = m0 + t < p.M - 1 ? m0 + t : p.M - 1;
     const int64_t ni = p.col_scalar ? 0 : (n0 + t < p.N - 1 ? n0 + t : p.N - 1);
-    const unsigned raw_r = gnk_load_raw_rt(p.s0, p.scale_dtype, mi), raw_c = gnk_load_raw_rt(p.s1, p.scale_dtype, ni);
+    unsigned raw_r = 0, raw_c = 0;
+    if constexpr (Cfg::EPI == EPI_ROWCOL) {
+        raw_r = gnk_load_raw_rt(p.s0, p.scale_dtype, mi);
+        raw_c = gnk_load_raw_rt(p.s1, p.scale_dtype, ni);
+    }
 
     StagerW4<Cfg::A_KMAJOR> sa;
     StagerW4<Cfg::B_KMAJOR> sb;
@@ -490,12 +507,66 @@ template <class Kernel> static int reserve_lds(Kernel k, int bytes, std::atomic<
     return GNK_OK;
 }
 
+// A group's contraction in parts (few tiles, many rows: 1024 x 1024 over 32768 rows are 64 tiles of 256 steps, two thirds of the chip idle): every part's sum
+// lands in a slab of its own and this kernel adds them in order (so that equal calls give equal bits), scales and rounds once.  HBM-bound; V = 4 adjacent
+// columns per thread where N allows.
+template <int OP, int V>
+__global__ void __launch_bounds__(256) join_kernel(const void *__restrict__ slab, char *__restrict__ C, const char *__restrict__ s0, const char *__restrict__ s1, int64_t E,
+                                                   int64_t M, int64_t N, int splits, int scale_dtype, int col_scalar, int out_dtype) {
+    typedef typename AccT<OP>::type acc_t;                   // v4i or v4f
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, total = E * M * N;
+    if (i >= total) return;
+    const int64_t row = i / N, n = i - row * N, e = row / M;
+    const float rs = gnk_load_scalar_rt(s0, scale_dtype, row);
+    float cs[V];
+#pragma unroll
+    for (int r = 0; r < V; ++r) cs[r] = gnk_load_scalar_rt(s1, scale_dtype, col_scalar ? e : e * N + n + r);
+    const char *src = (const char *)slab + 4 * i;
+    acc_t acc = {0, 0, 0, 0};
+    for (int k0 = 0; k0 < splits; k0 += 4) {                 // four loads in flight
+        acc_t part[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            part[k] = (acc_t){0, 0, 0, 0};
+            if (k0 + k < splits) {
+                if constexpr (V == 4) part[k] = *(const acc_t *)(src + (k0 + k) * total * 4);
+                else __builtin_memcpy(&part[k], src + (k0 + k) * total * 4, 4);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc += part[k];
+    }
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < V; ++r) v[r] = __fmul_rn(__fmul_rn((float)acc[r], rs), cs[r]);
+    if constexpr (V == 4) {
+        if (out_dtype == GNK_F32) *(v4f *)(C + 4 * i) = (v4f){v[0], v[1], v[2], v[3]};
+        else if (out_dtype == GNK_BF16) *(v2i *)(C + 2 * i) = (v2i){(int)gnk_pack2_bf16(v[0], v[1]), (int)gnk_pack2_bf16(v[2], v[3])};
+        else *(v2i *)(C + 2 * i) = (v2i){(int)gnk_pack2_f16(v[0], v[1]), (int)gnk_pack2_f16(v[2], v[3])};
+    } else {
+        gnk_store_scalar_rt(C, out_dtype, i, v[0]);
+    }
+}
+
+template <int OP> int join_parts(const GroupedParams &p, hipStream_t st) {
+    const int64_t total = p.E * p.g.M * p.g.N;
+    const bool quads = p.g.N % 4 == 0 && ((uintptr_t)p.g.C & 15) == 0;
+    const int64_t blocks = (total / (quads ? 4 : 1) + 255) / 256;
+    const auto args = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, p.slab, (char *)p.g.C, (const char *)p.g.s0, (const char *)p.g.s1, p.E, p.g.M, p.g.N, p.splits,
+                           p.g.scale_dtype, p.g.col_scalar, p.g.out_dtype);
+    };
+    if (quads) args(join_kernel<OP, 4>);
+    else args(join_kernel<OP, 1>);
+    return gnk_check_launch("grouped mm: joining the parts");
+}
+
 // Tile sizes of a launch over the whole grid; KERNEL with its LDS.
 template <class Kernel> int launch_tiles(Kernel kernel, std::atomic<bool> (&done)[64], int lds, int threads, bool depth, int bm, int bn, const GroupedParams &p0, hipStream_t st) {
     GroupedParams p = p0;
     p.g.grid_n = (int)((p.g.N + bn - 1) / bn);
     p.g.grid_m = depth ? (int)((p.g.M + bm - 1) / bm) : 0;
-    const int64_t blocks = (depth ? p.E * p.g.grid_m : max_row_tiles(p.T, p.E, bm)) * p.g.grid_n;
+    const int64_t blocks = (depth ? p.E * p.g.grid_m * p.splits : max_row_tiles(p.T, p.E, bm)) * p.g.grid_n;
     if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "grouped mm: too many tiles");
     const int rc = reserve_lds(kernel, lds, done);
     if (rc) return rc;
@@ -505,7 +576,7 @@ template <class Kernel> int launch_tiles(Kernel kernel, std::atomic<bool> (&done
 
 template <class Cfg, bool DEPTH> int launch_two_buffer(const GroupedParams &p, hipStream_t st) {
     static std::atomic<bool> done[64];
-    return launch_tiles(two_buffer_kernel<Cfg, DEPTH>, done, Cfg::LDS_BYTES + ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, EPI_ROWCOL>::BYTES, Cfg::NT, DEPTH, Cfg::BM,
+    return launch_tiles(two_buffer_kernel<Cfg, DEPTH>, done, Cfg::LDS_BYTES + ScalePrefetch<Cfg::BM, Cfg::BN, Cfg::NT, Cfg::EPI>::BYTES, Cfg::NT, DEPTH, Cfg::BM,
                         Cfg::BN, p, st);
 }
 
@@ -522,14 +593,17 @@ template <class Cfg, bool DEPTH, int BM = 256> int launch_w4(const GroupedParams
 // Tile choice by a cost model in us on the sizes that the host knows: groups of T / E rows, half a tile of edge each.  Constants fitted to forced runs of every
 // variant over 16 .. 32768 rows, 1 .. 64 groups, K, N = 512 .. 5632: a 256 x 256 or 192 x 256 workgroup (one per CU) costs 11-12 + 1.08 / 0.86 per 128 k, a
 // 128 x 128 one (two per CU) 6 + 1.0 with both operands K-major, 1.5 with B N-major, 1.3 in the depth form, a 64 x 64 one 5 + 0.55.
+// Parts of a contraction (depth, 128 and 256 tiles): a second launch and the slabs, written and read at about 4 TB/s.
 constexpr int VARIANT_192 = 100;             // beside gnk_set_gemm_variant's numbers: 192 x 256 (int8, rows form)
+constexpr int MAX_SPLITS = 32;
+struct Plan { int variant, splits; };
 
-static inline int choose_variant(const GroupedParams &p, bool depth, bool b_kmajor, bool can_w4, bool can_192) {
-    const double cus = (double)gnk_num_cus(), rows = (double)p.T, E = (double)(p.E > 0 ? p.E : 1);
+static inline Plan choose_variant(int64_t T, int64_t groups_n, int64_t M, int64_t N, int64_t K, bool depth, bool b_kmajor, bool can_w4, bool can_192, int forced) {
+    const double cus = (double)gnk_num_cus(), rows = (double)T, E = (double)(groups_n > 0 ? groups_n : 1);
     const double groups = E * (1.0 - pow(1.0 - 1.0 / E, rows));      // groups that a uniform router leaves with a row
     auto tiles = [&](double bm, double bn) {
-        const double gn = ceil((double)p.g.N / bn);
-        if (depth) return E * ceil((double)p.g.M / bm) * gn;
+        const double gn = ceil((double)N / bn);
+        if (depth) return E * ceil((double)M / bm) * gn;
         // sizes spread: where a group has half a tile or more on average, some have more than one
         const double m = rows / bm + 0.5 * groups, fill = groups > 0 ? rows / groups / bm : 0.0, least = groups * (1.0 + 0.3 * (fill < 0.5 ? fill : 0.5));
         return (m > least ? m : least) * gn;
@@ -540,25 +614,50 @@ static inline int choose_variant(const GroupedParams &p, bool depth, bool b_kmaj
     };
     // two workgroups per CU run at different times: the rounds of the 128 x 128 kernel smear
     auto smeared = [&](double n, double slots) { return n <= slots ? 1.0 : n / slots + 0.25; };
-    const double ks = depth ? rows / E / 128.0 : (double)p.g.K / 128.0;
+    const double ks = depth ? rows / E / 128.0 : (double)K / 128.0;
     const double edge = depth ? 1.0 : 0.0;       // a 256-k step of the ragged loop is half empty on average
-    const double t256 = can_w4 ? rounds(tiles(256, 256), cus) * (12.0 + 1.08 * (ks + edge)) : 1e30;
-    const double t192 = can_192 ? rounds(tiles(192, 256), cus) * (11.0 + 0.86 * ks) : 1e30;
-    const double t128 = smeared(tiles(128, 128), 2.0 * cus) * (6.0 + (depth ? 1.3 : b_kmajor ? 1.0 : 1.5) * ks);
-    const double t64 = rounds(tiles(64, 64), 2.0 * cus) * (5.0 + 0.55 * ks);
-    if (t64 <= t128 && t64 <= t256 && t64 <= t192) return GNK_VARIANT_64X128;
-    if (t192 < 0.98 * t256 && t192 < t128) return VARIANT_192;
-    return t256 <= t128 ? GNK_VARIANT_256_W4 : GNK_VARIANT_128;
+    Plan best = {GNK_VARIANT_128, 1};
+    double t_best = 1e30;
+    auto offer = [&](int variant, int splits, double t) {
+        if (t < t_best && (forced < 0 || forced == variant)) { t_best = t; best = {variant, splits}; }
+    };
+    offer(GNK_VARIANT_64X128, 1, rounds(tiles(64, 64), 2.0 * cus) * (5.0 + 0.55 * ks));
+    if (can_w4) offer(GNK_VARIANT_256_W4, 1, rounds(tiles(256, 256), cus) * (12.0 + 1.08 * (ks + edge)));
+    if (can_192) offer(VARIANT_192, 1, rounds(tiles(192, 256), cus) * (11.0 + 0.86 * ks) / 0.98);
+    offer(GNK_VARIANT_128, 1, smeared(tiles(128, 128), 2.0 * cus) * (6.0 + (depth ? 1.3 : b_kmajor ? 1.0 : 1.5) * ks));
+    if (depth)
+        for (int s = 2; s <= MAX_SPLITS && ks / s >= 4.0; s *= 2) {
+            const double join = 4.0 + 8.0 * s * E * (double)M * (double)N / 4.0e6;
+            offer(GNK_VARIANT_128, s, smeared(tiles(128, 128) * s, 2.0 * cus) * (6.0 + 1.3 * ks / s) + join);
+            if (can_w4) offer(GNK_VARIANT_256_W4, s, rounds(tiles(256, 256) * s, cus) * (12.0 + 1.08 * (ks / s + edge)) + join);
+        }
+    return best;
 }
 
-template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st) {
-    const bool can_w4 = depth ? p.T * (p.g.lda > p.g.ldb ? p.g.lda : p.g.ldb) < (1LL << 32) : p.g.K >= 256 && p.g.K % 256 == 0;
+static inline int64_t split_bytes(int splits, int64_t E, int64_t M, int64_t N) { return splits > 1 ? splits * E * M * N * 4 : 0; }
+
+template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const GroupedParams &p0, hipStream_t st) {
+    const bool can_w4 = depth ? p0.T * (p0.g.lda > p0.g.ldb ? p0.g.lda : p0.g.ldb) < (1LL << 32) : p0.g.K >= 256 && p0.g.K % 256 == 0;
     const bool can_192 = OP == OP_I8 && !depth && can_w4;
     // gnk_set_gemm_variant: 1, 5 and 6 force the 128 x 128, the 256 x 256 (where it can run) and the 64 x 64 kernel, 0 the 192 x 256 one
-    int variant = gnk_forced_variant_get();
-    if (variant == GNK_VARIANT_256 && can_192) variant = VARIANT_192;
-    else if ((variant != GNK_VARIANT_128 && variant != GNK_VARIANT_64X128 && variant != GNK_VARIANT_256_W4) || (variant == GNK_VARIANT_256_W4 && !can_w4))
-        variant = choose_variant(p, depth, b_kmajor, can_w4, can_192);
+    int forced = gnk_forced_variant_get();
+    if (forced == GNK_VARIANT_256 && can_192) forced = VARIANT_192;
+    else if ((forced != GNK_VARIANT_128 && forced != GNK_VARIANT_64X128 && forced != GNK_VARIANT_256_W4) || (forced == GNK_VARIANT_256_W4 && !can_w4)) forced = -1;
+    const Plan plan = choose_variant(p0.T, p0.E, p0.g.M, p0.g.N, p0.g.K, depth, b_kmajor, can_w4, can_192, forced);
+    const int variant = plan.variant;
+    GroupedParams p = p0;
+    p.splits = plan.splits;
+    while (p.splits > 1 && split_bytes(p.splits, p.E, p.g.M, p.g.N) > p.slab_bytes) p.splits /= 2;       // no room for the parts: fewer of them
+    if (p.splits > 1) {
+        p.g.C = p.slab;
+        p.g.out_dtype = OP == OP_I8 ? GNK_I32 : GNK_F32;
+        p.out_bytes = 4;
+        const int rc = variant == GNK_VARIANT_256_W4 ? launch_w4<PP2Cfg<false, false, OP, FA, FB, EPI_PLAIN>, true>(p, st)
+                                                     : launch_two_buffer<GemmCfg<128, 128, 2, 2, false, false, OP, FA, FB, EPI_PLAIN>, true>(p, st);
+        p.g.C = p0.g.C;
+        p.g.out_dtype = p0.g.out_dtype;
+        return rc ? rc : join_parts<OP>(p, st);
+    }
     if constexpr (OP == OP_I8) {
         if (variant == VARIANT_192)
             return b_kmajor ? launch_w4<PP2Cfg<true, true, OP, FA, FB, EPI_ROWCOL>, false, 192>(p, st)

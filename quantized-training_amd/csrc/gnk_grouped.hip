@@ -162,6 +162,13 @@ extern "C" int64_t gnk_grouped_scaled_mm_depth_workspace_bytes(const void *A, co
     return p.a.bytes() + p.b.bytes();
 }
 
+extern "C" int64_t gnk_grouped_scaled_mm_depth_split_bytes(int64_t T, int64_t E, int64_t M, int64_t N) {
+    if (T <= 0 || E <= 0 || M <= 0 || N <= 0 || E >= (1LL << 20) || M > MAX_PITCH || N > MAX_PITCH) return 0;
+    const int64_t pitch = up16(M > N ? M : N);
+    const int f = gnk_forced_variant_get(), forced = f == GNK_VARIANT_128 || f == GNK_VARIANT_64X128 || (f == GNK_VARIANT_256_W4 && T * pitch < (1LL << 32)) ? f : -1;
+    return split_bytes(choose_variant(T, E, M, N, 0, true, false, T * pitch < (1LL << 32), false, forced).splits, E, M, N);
+}
+
 extern "C" int gnk_grouped_scaled_mm_depth(const void *A, int a_dtype, const void *B, int b_dtype, void *C, int out_dtype, const void *row_scale,
                                            const void *col_scale, int scale_dtype, int col_scale_is_scalar, const int32_t *ends, int64_t T, int64_t E,
                                            int64_t M, int64_t N, int64_t sam, int64_t sat, int64_t sbt, int64_t sbn, void *workspace,
@@ -189,6 +196,12 @@ extern "C" int gnk_grouped_scaled_mm_depth(const void *A, int a_dtype, const voi
     p.g.out_dtype = out_dtype; p.g.scale_dtype = scale_dtype; p.g.col_scalar = col_scale_is_scalar != 0;
     p.ends = ends; p.T = T; p.E = E;
     p.ext_a = up16(M); p.ext_b = up16(N);
+    // what the caller gave beyond the copies may hold the sums of a split contraction
+    const int64_t copies = (plan.a.bytes() + plan.b.bytes() + 15) / 16 * 16;
+    if (workspace && workspace_bytes > copies && ((uintptr_t)workspace & 15) == 0) {
+        p.slab = (char *)workspace + copies;
+        p.slab_bytes = workspace_bytes - copies;
+    }
     p.out_bytes = gnk_dtype_size(out_dtype); p.scale_bytes = gnk_dtype_size(scale_dtype);
     return pick(a_dtype, b_dtype)(true, false, p, st);
 }

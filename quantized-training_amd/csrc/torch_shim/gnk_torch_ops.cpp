@@ -233,8 +233,8 @@ at::Tensor grouped_scaled_mm_depth(const at::Tensor &A, const at::Tensor &B, con
     at::Tensor C = at::empty({E, M, N}, sA.options());
     const int ad = dtype_code(A.scalar_type(), op), bd = dtype_code(B.scalar_type(), op), sd = dtype_code(sA.scalar_type(), op);
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(A.device());
-    const int64_t nws =
-        gnk_grouped_scaled_mm_depth_workspace_bytes(A.data_ptr(), B.data_ptr(), T, M, N, A.stride(0), A.stride(1), B.stride(0), B.stride(1));
+    const int64_t copies = gnk_grouped_scaled_mm_depth_workspace_bytes(A.data_ptr(), B.data_ptr(), T, M, N, A.stride(0), A.stride(1), B.stride(0), B.stride(1));
+    const int64_t nws = (copies + 15) / 16 * 16 + gnk_grouped_scaled_mm_depth_split_bytes(T, E, M, N);
     const at::Tensor ws = workspace_for(A, nws);
     check(gnk_grouped_scaled_mm_depth(A.data_ptr(), ad, B.data_ptr(), bd, C.data_ptr(), sd, sA.data_ptr(), sB.data_ptr(), sd, sB.size(2) == 1 && N != 1,
                                       (const int32_t *)ends.data_ptr(), T, E, M, N, A.stride(0), A.stride(1), B.stride(0), B.stride(1),
@@ -343,7 +343,8 @@ std::tuple<at::Tensor, at::Tensor> grouped_linear_int8_backward(const at::Tensor
     }
     if (need_w) {
         const int64_t qg = gnk_quantize_int8_grouped_workspace_bytes(T, E, N), qx = gnk_quantize_int8_grouped_workspace_bytes(T, E, K);
-        const int64_t nws = gnk_grouped_scaled_mm_depth_workspace_bytes(nullptr, nullptr, T, N, K, 1, N, K, 1);
+        const int64_t nws = (gnk_grouped_scaled_mm_depth_workspace_bytes(nullptr, nullptr, T, N, K, 1, N, K, 1) + 15) / 16 * 16 +
+                            gnk_grouped_scaled_mm_depth_split_bytes(T, E, N, K);
         Carver c{at::empty({Carver::up(T * N) + Carver::up(E * N * es) + Carver::up(T * K) + Carver::up(E * K * es) + Carver::up(std::max(qg, qx)) + nws + 256},
                            x.options().dtype(at::kByte))};
         char *const gq = c.take(T * N), *const gs = c.take(E * N * es), *const xq = c.take(T * K), *const xs = c.take(E * K * es), *const part = c.take(std::max(qg, qx));

@@ -11,7 +11,7 @@ import torch
 
 # GNK_LIBRARY: tuning only (an A/B build of the same sources, e.g. `make ABLATE=1 OUT=...`); the shipped library is the default
 _LIB_PATH = Path(os.environ.get("GNK_LIBRARY") or Path(__file__).resolve().parent / "libgnk_hip.so")
-ABI_VERSION = 4   # include/gnk.h GNK_ABI_VERSION
+ABI_VERSION = 5   # include/gnk.h GNK_ABI_VERSION
 
 BF16, F16, F32, I8, E4M3, E5M2, I32 = range(7)
 DTYPE_CODE = {
@@ -112,6 +112,8 @@ def load() -> ctypes.CDLL:
     L.gnk_grouped_scaled_mm_rows.argtypes = [vp, ci, vp, ci, vp, ci, vp, vp, ci, ci, vp] + [i64] * 9 + [vp, i64, vp]
     L.gnk_grouped_scaled_mm_depth_workspace_bytes.argtypes = [vp, vp] + [i64] * 7
     L.gnk_grouped_scaled_mm_depth_workspace_bytes.restype = i64
+    L.gnk_grouped_scaled_mm_depth_split_bytes.argtypes = [i64] * 4
+    L.gnk_grouped_scaled_mm_depth_split_bytes.restype = i64
     L.gnk_grouped_scaled_mm_depth.argtypes = [vp, ci, vp, ci, vp, ci, vp, vp, ci, ci, vp] + [i64] * 8 + [vp, i64, vp]
     L.gnk_quantize_int8_grouped_workspace_bytes.argtypes = [i64] * 3
     L.gnk_quantize_int8_grouped_workspace_bytes.restype = i64

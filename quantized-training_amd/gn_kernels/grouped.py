@@ -123,6 +123,7 @@ def _depth_hip(A: Tensor, B: Tensor, scale_A: Tensor, scale_B: Tensor, offs: Ten
     L, code = _cabi.load(), _cabi.DTYPE_CODE
     with _cabi.device_of(A):
         nws = L.gnk_grouped_scaled_mm_depth_workspace_bytes(A.data_ptr(), B.data_ptr(), T, M, N, *A.stride(), *B.stride())
+        nws = (nws + 15) // 16 * 16 + L.gnk_grouped_scaled_mm_depth_split_bytes(T, E, M, N)
         ws = torch.empty(nws, device=A.device, dtype=torch.uint8) if nws else None
         rc = L.gnk_grouped_scaled_mm_depth(A.data_ptr(), code[A.dtype], B.data_ptr(), code[B.dtype], C.data_ptr(), code[C.dtype], scale_A.data_ptr(),
                                            scale_B.data_ptr(), code[scale_A.dtype], int(scale_B.shape[2] == 1 and N != 1), offs.data_ptr(), T, E, M, N,

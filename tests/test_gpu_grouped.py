@@ -496,3 +496,91 @@ def test_variants_outputs(forced, out, N):
     run_rows([300, 0, 270], 3, 256, N, "int8", out)
     run_depth([300, 0, 270], 3, N, 264, "int8", out)
     run_depth([300, 0, 270], 3, 264, N, "int8", out, scalar=True)
+
+
+# ------------------------------------------------------------------------------------------------ contractions cut into parts
+LONG = {
+    "one": ([5000], 3),
+    "short_ones_beside_it": ([0, 4100, 0, 1, 900], 130),
+    "just_over_a_step": ([1025, 0, 1023], 0),
+    "longest": ([30000], 0),
+}
+
+
+@pytest.mark.parametrize("name", list(LONG))
+@pytest.mark.parametrize("M,N", [(144, 272), (17, 15), (64, 64), (300, 130)])
+@pytest.mark.parametrize("dt", ["int8", "e4m3", "e5m2"])
+@pytest.mark.parametrize("variant", [-1, 1, 5])
+def test_depth_in_parts(name, M, N, dt, variant):
+    sizes, pad = LONG[name]
+    L = _cabi.load()
+    L.gnk_set_gemm_variant(variant)
+    try:
+        if name in ("one", "longest"):                             # the others are split or not as the sizes say
+            assert L.gnk_grouped_scaled_mm_depth_split_bytes(sum(sizes) + pad, len(sizes), M, N) >= 2 * 4 * len(sizes) * M * N
+        run_depth(sizes, pad, M, N, dt, "bf16")
+    finally:
+        L.gnk_set_gemm_variant(-1)
+
+
+@pytest.mark.parametrize("out", list(OUT))
+@pytest.mark.parametrize("scalar", [False, True])
+@pytest.mark.parametrize("N", [48, 46])
+def test_depth_in_parts_output_types(out, scalar, N):
+    run_depth([3000, 0, 2500], 1, 40, N, "int8", out, scalar=scalar)
+    run_depth([3000, 0, 2500], 1, 40, N, "e5m2", out, scalar=scalar)
+
+
+def test_depth_in_parts_strides():
+    for a_order, b_order, pitch in (((0, 1), (0, 1), 0), ((1, 0), (1, 0), 0), ((1, 0), (0, 1), 3), ((0, 1), (1, 0), 16)):
+        run_depth([4000, 100], 5, 60, 33, "int8", "bf16", a_order=a_order, b_order=b_order, pitch=pitch)
+
+
+def test_depth_with_less_room_for_its_parts():
+    """The C entry with room for all parts, for half of them, for one and for none, and with the slab behind copied operands: the same int8 result."""
+    L, g = _cabi.load(), torch.Generator().manual_seed(3)
+    sizes, M, N = [6000, 500], 64, 96
+    T, E = sum(sizes), len(sizes)
+    A, B = make8((T, M), "int8", g).to(DEV), make8((T, N), "int8", g).to(DEV)
+    sA, sB, offs = scales((E, M, 1), "f32", g).to(DEV), scales((E, 1, N), "f32", g).to(DEV), offs_of(sizes)
+    room = L.gnk_grouped_scaled_mm_depth_split_bytes(T, E, M, N)
+    assert room > 0
+    want = None
+    for n in (0, E * M * N * 4, room // 2, room, room + 4096):
+        C, ws = torch.empty(E, M, N, device=DEV), torch.empty(max(n, 1), dtype=torch.uint8, device=DEV)
+        rc = L.gnk_grouped_scaled_mm_depth(A.data_ptr(), _cabi.I8, B.data_ptr(), _cabi.I8, C.data_ptr(), _cabi.DTYPE_CODE[torch.float32], sA.data_ptr(), sB.data_ptr(),
+                                           _cabi.DTYPE_CODE[torch.float32], 0, offs.data_ptr(), T, E, M, N, 1, M, N, 1, ws.data_ptr() if n else None, n,
+                                           torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        torch.cuda.synchronize()
+        want = C if want is None else want
+        assert torch.equal(C, want)
+    check(want, *depth_ref(A.cpu().t(), B.cpu(), sA.cpu(), sB.cpu(), sizes), "int8", "f32", T)
+
+
+def test_depth_in_parts_repeats_and_replays():
+    """fp8 sums depend on their order: equal calls give equal bits, on other streams and in a graph replayed with other sizes too."""
+    g = torch.Generator().manual_seed(6)
+    T, M, N = 8000, 96, 80
+    A, B = make8((T, M), "e4m3", g).to(DEV), make8((T, N), "e4m3", g).to(DEV)
+    sA, sB = scales((2, M, 1), "bf16", g).to(DEV), scales((2, 1, N), "bf16", g).to(DEV)
+    offs = offs_of([5000, 2000])
+    call = lambda: gn_kernels.grouped_scaled_mm(A.t(), B, sA, sB, offs)  # noqa: E731
+    want = call()
+    torch.cuda.synchronize()
+    for s in [torch.cuda.Stream() for _ in range(2)]:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs = [call() for _ in range(5)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for sizes in ([5000, 2000], [0, 8000], [10, 0], [5000, 2000]):
+        offs.copy_(offs_of(sizes))
+        graph.replay()
+        eager = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
+        check(eager, *depth_ref(A.cpu().t(), B.cpu(), sA.cpu(), sB.cpu(), sizes), "e4m3", "bf16", T)
