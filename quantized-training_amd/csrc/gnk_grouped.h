@@ -318,20 +318,24 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cf
 // wave has read by then, takes stage t + 3 behind it.  Towards the end nothing is left to issue and the wait is for everything.
 // 16 rows over 8 experts, 1024 -> 4096, int8: 8.4 us a call for 30 MB of weights, 3.5 TB/s (5.9 us at a copy's rate; the rest is the launch and the
 // first loads); depth form, 1021 rows over 8 experts to 512 x 256: 5 us.
-template <class Cfg, bool DEPTH>
-__global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(2))) ring_kernel(const GroupedParams gp) {
-    extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int MT = Cfg::MT, NTL = Cfg::NTL, NST = 4, STAGE = Cfg::A_BYTES + Cfg::B_BYTES;
+// KG = 2 (at most one workgroup per CU): a second set of four waves with a ring of its own takes every other step; the two halves are added in LDS.
+// 16 rows over 4 experts, 4096 -> 1024: 17.7 -> 11.6 us with B K-major, 23.2 -> 18.2 N-major (rows of 64 bytes are half lines); 5632 -> 2048, one row: 18.2 -> 15.0.
+template <class Cfg, bool DEPTH, int KG>
+__global__ void __launch_bounds__(Cfg::NT * KG) __attribute__((amdgpu_waves_per_eu(2))) ring_kernel(const GroupedParams gp) {
+    extern __shared__ __attribute__((aligned(16))) char smem_all[];
+    constexpr int MT = Cfg::MT, NTL = Cfg::NTL, NST = 4, STAGE = Cfg::A_BYTES + Cfg::B_BYTES, RING = NST * STAGE, NT = Cfg::NT * KG;
     constexpr int PIECES = (Cfg::BM + Cfg::BN) / 8 / Cfg::NW;      // LDS-DMA instructions per wave and stage
+    static_assert(KG == 1 || KG == 2, "one or two sets of waves");
     typedef typename AccT<Cfg::OP>::type acc_t;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kg = wave_all / Cfg::NW, wave = wave_all % Cfg::NW;
     const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+    char *const smem = smem_all + kg * RING;
     const Tile tile = DEPTH ? depth_tile<GNK_BK>(gp, gp.g.grid_m, gp.g.grid_n, lane) : rows_tile<Cfg::BM>(gp, gp.g.grid_n, lane);
     if (!tile.work) return;
     const int64_t m0 = (int64_t)tile.tm * Cfg::BM, n0 = (int64_t)tile.tn * Cfg::BN;
     if (!DEPTH && tile.e == gp.E) {
-        zero_tile<Cfg::BM, Cfg::BN, Cfg::NT>((char *)gp.g.C + tile.lo * gp.g.N * gp.out_bytes, tile.hi - tile.lo, gp.g.N, m0, n0, gp.out_bytes);
+        zero_tile<Cfg::BM, Cfg::BN, NT>((char *)gp.g.C + tile.lo * gp.g.N * gp.out_bytes, tile.hi - tile.lo, gp.g.N, m0, n0, gp.out_bytes);
         return;
     }
     int64_t ext_a, ext_b;
@@ -342,15 +346,22 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(2)
     Stager<Cfg::B_KMAJOR, Cfg::BN, Cfg::NW> sb;
     sa.init(p.A, p.lda, m0, ext_a, wave, lane);
     sb.init(p.B, p.ldb, n0, ext_b, wave, lane);
+    if constexpr (KG > 1) {
+        sa.base += kg * sa.step;
+        sb.base += kg * sb.step;
+        sa.step *= KG;
+        sb.step *= KG;
+    }
     acc_t acc[MT][NTL];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NTL; ++j) acc[i][j] = (acc_t){0, 0, 0, 0};
-    const int nk = (int)((p.K + GNK_BK - 1) / GNK_BK), ktail = (int)(p.K % GNK_BK);
+    const int nk_all = (int)((p.K + GNK_BK - 1) / GNK_BK), ktail = (int)(p.K % GNK_BK), last = nk_all - 1;
+    const int nk = (nk_all + KG - 1 - kg) / KG, nk_most = (nk_all + KG - 1) / KG;      // this set's steps kg, kg + KG, ...
     auto fetch = [&](int t) {
         char *const As = smem + (t % NST) * STAGE, *const Bs = As + Cfg::A_BYTES;
-        if (ktail && t + 1 == nk) {
+        if (ktail && t * KG + kg == last) {
             sa.issue_tail(As, p.lda, m0, ext_a, wave, lane, ktail);
             sb.issue_tail(Bs, p.ldb, n0, ext_b, wave, lane, ktail);
         } else {
@@ -359,23 +370,39 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(2)
         }
     };
     for (int t = 0; t < NST - 1 && t < nk; ++t) fetch(t);
-    for (int t = 0; t < nk; ++t) {
+    for (int t = 0; t < nk_most; ++t) {
         static_assert(2 * PIECES <= 63, "vmcnt holds 6 bits");
         if (t + NST - 2 < nk) asm volatile("s_waitcnt vmcnt(%0)" : : "i"((NST - 2) * PIECES) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        char *const As = smem + (t % NST) * STAGE, *const Bs = As + Cfg::A_BYTES;
-        if (ktail && t + 1 == nk) {
-            zero_tail<Cfg::A_KMAJOR, Cfg::BM, Cfg::NT>(As, ktail);
-            zero_tail<Cfg::B_KMAJOR, Cfg::BN, Cfg::NT>(Bs, ktail);
+        if (ktail && t == last / KG) {                                // every thread clears its share of the tail, whichever set owns it
+            char *const Az = smem_all + (last % KG) * RING + (t % NST) * STAGE, *const Bz = Az + Cfg::A_BYTES;
+            zero_tail<Cfg::A_KMAJOR, Cfg::BM, NT>(Az, ktail);
+            zero_tail<Cfg::B_KMAJOR, Cfg::BN, NT>(Bz, ktail);
             __syncthreads();
         }
         if (t + NST - 1 < nk) fetch(t + NST - 1);
-        compute_step<Cfg, false>(As, Bs, acc, wm, wn, lane);
+        char *const As = smem + (t % NST) * STAGE, *const Bs = As + Cfg::A_BYTES;
+        if (t < nk) compute_step<Cfg, false>(As, Bs, acc, wm, wn, lane);
     }
-    float *const lsc = (float *)(smem + NST * STAGE);
+    float *const lsc = (float *)(smem_all + KG * RING);
     spf.park(p, (char *)lsc);
     __syncthreads();
+    if constexpr (KG > 1) {
+        // the second set's sums through its own ring, free now
+        char *const sums = smem_all + RING;
+        if (kg == 1)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NTL; ++j) *(GNK_LDS acc_t *)(GNK_LDS char *)(sums + 16 * (((wave * MT + i) * NTL + j) * 64 + lane)) = acc[i][j];
+        __syncthreads();
+        if (kg == 1) return;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NTL; ++j) acc[i][j] += *(const GNK_LDS acc_t *)(const GNK_LDS char *)(sums + 16 * (((wave * MT + i) * NTL + j) * 64 + lane));
+    }
     run_epilogue<Cfg>(p, acc, nullptr, smem, wave, lane, m0 + wm * Cfg::WTM, n0 + wn * Cfg::WTN, lsc, wm * Cfg::WTM, wn * Cfg::WTN);
 }
 
@@ -509,7 +536,8 @@ template <class Kernel> static int reserve_lds(Kernel k, int bytes, std::atomic<
 
 // A group's contraction in parts (few tiles, many rows: 1024 x 1024 over 32768 rows are 64 tiles of 256 steps, two thirds of the chip idle): every part's sum
 // lands in a slab of its own and this kernel adds them in order (so that equal calls give equal bits), scales and rounds once.  HBM-bound; V = 4 adjacent
-// columns per thread where N allows.
+// columns per thread where N allows.  Whole calls, one part -> the parts chosen, int8: 1024 x 1024 over 32768 rows 182 -> 49 us (16 parts, 1.4 POP/s; the slabs,
+// 67 MB written and read, are half of it), 4096 x 1024 252 -> 115 (4), 64 x 64 127 -> 16 (32), four groups of 512 x 512 51 -> 28 (8).
 template <int OP, int V>
 __global__ void __launch_bounds__(256) join_kernel(const void *__restrict__ slab, char *__restrict__ C, const char *__restrict__ s0, const char *__restrict__ s1, int64_t E,
                                                    int64_t M, int64_t N, int splits, int scale_dtype, int col_scalar, int out_dtype) {
@@ -580,9 +608,12 @@ template <class Cfg, bool DEPTH> int launch_two_buffer(const GroupedParams &p, h
                         Cfg::BN, p, st);
 }
 
-template <class Cfg, bool DEPTH> int launch_ring(const GroupedParams &p, hipStream_t st) {
+template <class Cfg, bool DEPTH, int KG> int launch_ring_of(const GroupedParams &p, hipStream_t st) {
     static std::atomic<bool> done[64];
-    return launch_tiles(ring_kernel<Cfg, DEPTH>, done, 4 * (Cfg::A_BYTES + Cfg::B_BYTES) + (Cfg::BM + Cfg::BN) * 4, Cfg::NT, DEPTH, Cfg::BM, Cfg::BN, p, st);
+    return launch_tiles(ring_kernel<Cfg, DEPTH, KG>, done, KG * 4 * (Cfg::A_BYTES + Cfg::B_BYTES) + (Cfg::BM + Cfg::BN) * 4, KG * Cfg::NT, DEPTH, Cfg::BM, Cfg::BN, p, st);
+}
+template <class Cfg, bool DEPTH> int launch_ring(const GroupedParams &p, int kg, hipStream_t st) {
+    return kg == 2 ? launch_ring_of<Cfg, DEPTH, 2>(p, st) : launch_ring_of<Cfg, DEPTH, 1>(p, st);
 }
 
 template <class Cfg, bool DEPTH, int BM = 256> int launch_w4(const GroupedParams &p, hipStream_t st) {
@@ -592,11 +623,12 @@ template <class Cfg, bool DEPTH, int BM = 256> int launch_w4(const GroupedParams
 
 // Tile choice by a cost model in us on the sizes that the host knows: groups of T / E rows, half a tile of edge each.  Constants fitted to forced runs of every
 // variant over 16 .. 32768 rows, 1 .. 64 groups, K, N = 512 .. 5632: a 256 x 256 or 192 x 256 workgroup (one per CU) costs 11-12 + 1.08 / 0.86 per 128 k, a
-// 128 x 128 one (two per CU) 6 + 1.0 with both operands K-major, 1.5 with B N-major, 1.3 in the depth form, a 64 x 64 one 5 + 0.55.
+// 128 x 128 one (two per CU) 6 + 1.0 with both operands K-major, 1.5 with B N-major, 1.3 in the depth form, a 64 x 64 one 5 + 0.55, or 0.33 with
+// two sets of waves, one per CU.
 // Parts of a contraction (depth, 128 and 256 tiles): a second launch and the slabs, written and read at about 4 TB/s.
 constexpr int VARIANT_192 = 100;             // beside gnk_set_gemm_variant's numbers: 192 x 256 (int8, rows form)
 constexpr int MAX_SPLITS = 32;
-struct Plan { int variant, splits; };
+struct Plan { int variant, splits, kg; };      // kg: sets of waves of the 64 x 64 kernel
 
 static inline Plan choose_variant(int64_t T, int64_t groups_n, int64_t M, int64_t N, int64_t K, bool depth, bool b_kmajor, bool can_w4, bool can_192, int forced) {
     const double cus = (double)gnk_num_cus(), rows = (double)T, E = (double)(groups_n > 0 ? groups_n : 1);
@@ -616,12 +648,13 @@ static inline Plan choose_variant(int64_t T, int64_t groups_n, int64_t M, int64_
     auto smeared = [&](double n, double slots) { return n <= slots ? 1.0 : n / slots + 0.25; };
     const double ks = depth ? rows / E / 128.0 : (double)K / 128.0;
     const double edge = depth ? 1.0 : 0.0;       // a 256-k step of the ragged loop is half empty on average
-    Plan best = {GNK_VARIANT_128, 1};
+    Plan best = {GNK_VARIANT_128, 1, 1};
     double t_best = 1e30;
-    auto offer = [&](int variant, int splits, double t) {
-        if (t < t_best && (forced < 0 || forced == variant)) { t_best = t; best = {variant, splits}; }
+    auto offer = [&](int variant, int splits, double t, int kg = 1) {
+        if (t < t_best && (forced < 0 || forced == variant)) { t_best = t; best = {variant, splits, kg}; }
     };
     offer(GNK_VARIANT_64X128, 1, rounds(tiles(64, 64), 2.0 * cus) * (5.0 + 0.55 * ks));
+    if (ks >= 4.0) offer(GNK_VARIANT_64X128, 1, rounds(tiles(64, 64), cus) * (5.0 + 0.33 * ks), 2);
     if (can_w4) offer(GNK_VARIANT_256_W4, 1, rounds(tiles(256, 256), cus) * (12.0 + 1.08 * (ks + edge)));
     if (can_192) offer(VARIANT_192, 1, rounds(tiles(192, 256), cus) * (11.0 + 0.86 * ks) / 0.98);
     offer(GNK_VARIANT_128, 1, smeared(tiles(128, 128), 2.0 * cus) * (6.0 + (depth ? 1.3 : b_kmajor ? 1.0 : 1.5) * ks));
@@ -669,9 +702,9 @@ template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const Gr
         return launch_w4<PP2Cfg<true, false, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
     }
     if (variant == GNK_VARIANT_64X128) {
-        if (depth) return launch_ring<GemmCfg<64, 64, 4, 1, false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
-        if (b_kmajor) return launch_ring<GemmCfg<64, 64, 4, 1, true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
-        return launch_ring<GemmCfg<64, 64, 4, 1, true, false, OP, FA, FB, EPI_ROWCOL>, false>(p, st);
+        if (depth) return launch_ring<GemmCfg<64, 64, 4, 1, false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, plan.kg, st);
+        if (b_kmajor) return launch_ring<GemmCfg<64, 64, 4, 1, true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, plan.kg, st);
+        return launch_ring<GemmCfg<64, 64, 4, 1, true, false, OP, FA, FB, EPI_ROWCOL>, false>(p, plan.kg, st);
     }
     if (depth) return launch_two_buffer<GemmCfg<128, 128, 2, 2, false, false, OP, FA, FB, EPI_ROWCOL>, true>(p, st);
     if (b_kmajor) return launch_two_buffer<GemmCfg<128, 128, 2, 2, true, true, OP, FA, FB, EPI_ROWCOL>, false>(p, st);

@@ -523,20 +523,28 @@ def test_depth_in_parts(name, M, N, dt, variant):
         L.gnk_set_gemm_variant(-1)
 
 
+@pytest.fixture
+def tiles_of_128():
+    L = _cabi.load()
+    L.gnk_set_gemm_variant(1)
+    yield
+    L.gnk_set_gemm_variant(-1)
+
+
 @pytest.mark.parametrize("out", list(OUT))
 @pytest.mark.parametrize("scalar", [False, True])
 @pytest.mark.parametrize("N", [48, 46])
-def test_depth_in_parts_output_types(out, scalar, N):
+def test_depth_in_parts_output_types(tiles_of_128, out, scalar, N):
     run_depth([3000, 0, 2500], 1, 40, N, "int8", out, scalar=scalar)
     run_depth([3000, 0, 2500], 1, 40, N, "e5m2", out, scalar=scalar)
 
 
-def test_depth_in_parts_strides():
+def test_depth_in_parts_strides(tiles_of_128):
     for a_order, b_order, pitch in (((0, 1), (0, 1), 0), ((1, 0), (1, 0), 0), ((1, 0), (0, 1), 3), ((0, 1), (1, 0), 16)):
         run_depth([4000, 100], 5, 60, 33, "int8", "bf16", a_order=a_order, b_order=b_order, pitch=pitch)
 
 
-def test_depth_with_less_room_for_its_parts():
+def test_depth_with_less_room_for_its_parts(tiles_of_128):
     """The C entry with room for all parts, for half of them, for one and for none, and with the slab behind copied operands: the same int8 result."""
     L, g = _cabi.load(), torch.Generator().manual_seed(3)
     sizes, M, N = [6000, 500], 64, 96
@@ -558,7 +566,7 @@ def test_depth_with_less_room_for_its_parts():
     check(want, *depth_ref(A.cpu().t(), B.cpu(), sA.cpu(), sB.cpu(), sizes), "int8", "f32", T)
 
 
-def test_depth_in_parts_repeats_and_replays():
+def test_depth_in_parts_repeats_and_replays(tiles_of_128):
     """fp8 sums depend on their order: equal calls give equal bits, on other streams and in a graph replayed with other sizes too."""
     g = torch.Generator().manual_seed(6)
     T, M, N = 8000, 96, 80
