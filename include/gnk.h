@@ -45,8 +45,8 @@ typedef enum gnk_status {
  *   1: the first one.   2: gnk_scaled_mm_ws / gnk_scaled_mm_t, the fused quantize pair, gnk_quantize_int8_noalloc, the MX and BitNet
  *      entry points added; gnk_set_debug_flags removed from the shipped library; gnk_set_gemm_variant accepts 5, 6, -2 and -3; gnk_set_tile_rescale added.
  *   3: the products grouped by expert and their quantizer (gnk_grouped_scaled_mm_rows / _depth, gnk_quantize_int8_grouped).
- *   4: gnk_orthogonalize.   5: gnk_grouped_scaled_mm_depth_split_bytes. */
-#define GNK_ABI_VERSION 5
+ *   4: gnk_orthogonalize.   5: gnk_grouped_scaled_mm_depth_split_bytes.   6: gnk_orthogonalize_workspace_bytes_of. */
+#define GNK_ABI_VERSION 6
 int gnk_abi_version(void);
 
 /* Message for the last non-zero status returned on this thread ("" if none). */
@@ -315,9 +315,11 @@ int gnk_quantize_int8_grouped(const void *x, int x_dtype, const int32_t *ends, i
  * of two, sums fp32, the norm fp64: the result is off by about 1.5e-3 of its norm for five steps of the usual (3.4445, -4.7750, 2.0315) on matrices
  * with singular values within a factor of 1000, more for directions below that.  The coefficients must keep the singular values below sqrt 2 (larger
  * intermediates may overflow to Inf).  A matrix that holds a NaN or Inf comes out as NaN; one of zeros as zeros.  rows, cols <= 2^20, batch < 2^16.
- * workspace: gnk_orthogonalize_workspace_bytes() bytes, 16-byte aligned, need not be cleared.  Overlapping calls need one each.
+ * workspace: gnk_orthogonalize_workspace_bytes_of() bytes for results of that type (half as much for BF16 as for the others), or
+ * gnk_orthogonalize_workspace_bytes(), enough for any; 16-byte aligned, need not be cleared.  Overlapping calls need one each.
  */
 int64_t gnk_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+int64_t gnk_orthogonalize_workspace_bytes_of(int out_dtype, int64_t batch, int64_t rows, int64_t cols);
 int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
                       float eps, void *workspace, int64_t workspace_bytes, void *stream);
 

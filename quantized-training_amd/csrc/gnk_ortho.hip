@@ -10,6 +10,9 @@
 //   below 2^-24.  mu = p(mean of S's diagonal), p(s) = a + b s + c s^2, is about the mean of Q's diagonal, which otherwise carries most of Q's rounding error:
 //   three quarters of the whole result's for flat matrices (36 x 2230: 2.6e-3 -> 2.0e-3 of the result's norm, 1.7e-3 of which is the output's bf16).  mu X is added in fp32 where Q X is stored.  From 512 rows on the
 //   rounding of X is most of the error (512 x 512: 1.4e-3 of 1.6e-3) and the second read of X costs 15 % of that product: mu = 0 there.
+// That is an eighth of what a bf16 result is rounded by and five times a fp16 result's rounding, so results of 11 and 24 bits (fp16, fp32) are computed with every
+// matrix in two fp16 parts, hi + lo (PAIRS; 22 bits, no mu): a product is hi hi + lo hi + hi lo, one loop over three times the contraction.  Off by 2.1e-4 of the
+// norm for fp16, its rounding, and ORTHO_F32_ERR for fp32; ORTHO_F16_TIMES.
 // Shapes are padded with zeros to multiples of 128 in the workspace: zero rows and columns stay zero through every product.
 //
 // The products: `wide` S = X X^T reads both operands along K, Q X reads X as it lies (N-contiguous, transposed on the way out of LDS); `tall` S = X^T X
@@ -44,6 +47,7 @@ struct Product {
     void *C;
     const char *D;                           // POLY: the matrix S; UPDATE: X
     int64_t ba, bb, bc, bd;                  // bytes from one matrix of the stack to the next
+    int64_t a_lo, b_lo, c_lo, d_lo;          // PAIRS: bytes from the hi part to the lo part (c_lo = 0: the result has none)
     int64_t M, N, K;                         // output extents that are stored; K a multiple of 128
     int64_t lda, ldb, ldd;                   // bytes
     int64_t ext_a, ext_b;                    // staged extents (elements, >= M / N, multiples of 128)
@@ -85,17 +89,20 @@ struct Finish {
 };
 
 // acc (lane: row m, columns n .. n + 3) -> the stored value
-template <int EPI>
+template <int EPI, bool PAIRS = false>
 __device__ __forceinline__ void finish_value(const Product &p, const Finish &fin, v4f &acc, int64_t m, int64_t n) {
     if constexpr (EPI == GRAM) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) acc[r] *= fin.f;
     } else {
         const int64_t mm = m < p.ext_a ? m : p.ext_a - 1, nn = n < p.ext_b ? n : p.ext_b - 4;
-        const v4h d = *(const v4h *)(fin.D + mm * p.ldd + 2 * nn);
+        const char *at = fin.D + mm * p.ldd + 2 * nn;
+        const v4h d = *(const v4h *)at;
+        v4h lo = {0, 0, 0, 0};
+        if constexpr (PAIRS) lo = *(const v4h *)(at + p.d_lo);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            acc[r] = __builtin_fmaf(acc[r], fin.f, (float)d[r] * fin.d);
+            acc[r] = __builtin_fmaf(acc[r], fin.f, (PAIRS ? (float)d[r] + (float)lo[r] : (float)d[r]) * fin.d);
             if (EPI == POLY && m == n + r) acc[r] += fin.diag;
         }
     }
@@ -148,7 +155,7 @@ __device__ __forceinline__ GemmParams store_params(const Product &p, int b) {
 // The transpose of a wave's 16 MT x 64 results (fp16 output, rows m0 .., columns n0 ..; both inside the padded matrix), through its slice of LDS:
 // image [64 n][16 MT m], 16-byte chunk c of row n at c ^ 2 ((n >> 2) & 3), so that the four lane groups of a write land in different banks; rows of
 // 32 MT bytes go out whole.
-template <int MT> __device__ __forceinline__ void store_mirror(const Product &p, int b, const v4f (&acc)[MT][4], char *region, int lane, int64_t m0, int64_t n0) {
+template <int MT> __device__ __forceinline__ void store_mirror(const Product &p, char *C, const v4f (&acc)[MT][4], char *region, int lane, int64_t m0, int64_t n0) {
     constexpr int PITCH = 32 * MT, CHUNKS = 2 * MT;
     static_assert(MT >= 4, "the swizzle needs eight chunks per row");
     if (m0 + 16 * MT > p.ext_a || n0 + 64 > p.ext_b) return;                  // padding tiles beyond the matrix (extents are multiples of 128)
@@ -163,7 +170,6 @@ template <int MT> __device__ __forceinline__ void store_mirror(const Product &p,
                 const int n = 16 * j + 4 * g + r, c = (2 * i + (ml >> 3)) ^ (2 * g);
                 *(GNK_LDS _Float16 *)(GNK_LDS char *)(region + n * PITCH + 16 * c + 2 * (ml & 7)) = (_Float16)acc[i][j][r];
             }
-    char *const C = (char *)p.C + b * p.bc;
 #pragma unroll
     for (int u = 0; u < CHUNKS; ++u) {                                         // 64 rows x CHUNKS chunks over 64 lanes
         const int e = u * 64 + lane, n = e / CHUNKS, c = e % CHUNKS;
@@ -223,7 +229,8 @@ template <int BM> struct RingShape {
     static constexpr int LDS = NST * STAGE;
 };
 
-template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM>
+// PAIRS: the steps of hi hi, then lo hi, then hi lo; the result is stored as hi = fp16(v) and lo = fp16(v - hi), the last one in its own type.
+template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM, bool PAIRS>
 __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2))) product_ring_kernel(const Product p) {
     extern __shared__ __attribute__((aligned(16))) char smem_all[];
     typedef RingShape<BM> R;
@@ -247,28 +254,33 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-    const int nk = ((int)(p.K / 64) + KG - 1 - kg) / KG, nk_most = KG == 1 ? nk : ((int)(p.K / 64) + KG - 1) / KG;      // steps kg, kg + KG, ...
-    if constexpr (KG > 1) {
+    const int nk_one = (int)(p.K / 64), nk_all = PAIRS ? 3 * nk_one : nk_one;
+    const int nk = (nk_all + KG - 1 - kg) / KG, nk_most = KG == 1 ? nk : (nk_all + KG - 1) / KG;      // steps kg, kg + KG, ...
+    const char *const a0 = sa.base, *const b0 = sb.base;
+    if constexpr (KG > 1 && !PAIRS) {
         sa.base += kg * sa.step;
         sb.base += kg * sb.step;
         sa.step *= KG;
         sb.step *= KG;
     }
-    for (int t = 0; t < NST - 1 && t < nk; ++t) {
-        sa.issue(smem + t * R::STAGE, wave);
-        sb.issue(smem + t * R::STAGE + R::OPER, wave);
-    }
+    auto fetch = [&](int t) {
+        if constexpr (PAIRS) {
+            const int step = t * KG + kg, part = step >= 2 * nk_one ? 2 : (step >= nk_one ? 1 : 0), k = step - part * nk_one;
+            sa.base = a0 + (part == 1 ? p.a_lo : 0) + k * sa.step;
+            sb.base = b0 + (part == 2 ? p.b_lo : 0) + k * sb.step;
+        }
+        char *const into = smem + (t % NST) * R::STAGE;
+        sa.issue(into, wave);
+        sb.issue(into + R::OPER, wave);
+    };
+    for (int t = 0; t < NST - 1 && t < nk; ++t) fetch(t);
     for (int t = 0; t < nk_most; ++t) {
         // stage t has landed; t + 1 .. t + NST - 2 may stay in flight
         if (t + NST - 2 < nk) asm volatile("s_waitcnt vmcnt(%0)" : : "i"((NST - 2) * PIECES) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         char *const As = smem + (t % NST) * R::STAGE, *const Bs = As + R::OPER;
-        if (t + NST - 1 < nk) {                                        // into the buffer of stage t - 1, which every wave has read
-            char *const next = smem + ((t + NST - 1) % NST) * R::STAGE;
-            sa.issue(next, wave);
-            sb.issue(next + R::OPER, wave);
-        }
+        if (t + NST - 1 < nk) fetch(t + NST - 1);                      // into the buffer of stage t - 1, which every wave has read
         if (KG > 1 && t >= nk) break;                                  // the other set has one step more
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -307,35 +319,49 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, fin, acc[i][j], mw + 16 * i + (lane & 15), nw + 16 * j + 4 * (lane >> 4));
-    __syncthreads();
-    const GemmParams g = store_params(p, b);
-    if (kg == 0) run_epilogue<Cfg>(g, acc, nullptr, smem, wave, lane, mw, nw);
-    if constexpr (SYM) {
-        if (tm != tn) {
-            if constexpr (MT >= 4) {
-                if (kg == KG - 1) store_mirror<MT>(p, b, acc, smem + R::LDS / 2 + wave * (64 * 32 * MT), lane, mw, nw);
-            } else {
-                // 16 rows per wave: transposed rows of 32 bytes would waste the stores; the four waves put theirs side by side first
-                // (KG = 2: the second set does, in its own ring's LDS; both pass the barrier)
-                char *const T = smem + R::LDS / 2;                     // [64 n][64 m] fp16, rows of 128 bytes, 16-byte chunk c at c ^ (n & 7)
-                const int gq = lane >> 4, ml = lane & 15;
-                if (kg == KG - 1)
+        for (int j = 0; j < 4; ++j) finish_value<EPI, PAIRS>(p, fin, acc[i][j], mw + 16 * i + (lane & 15), nw + 16 * j + 4 * (lane >> 4));
+    GemmParams g = store_params(p, b);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+    for (int part = 0; part < (PAIRS ? 2 : 1); ++part) {
+        if constexpr (PAIRS) {
+            if (part == 1) {
+                if (!p.c_lo) break;
+                g.C = (char *)g.C + p.c_lo;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int n = 16 * j + 4 * gq + r, c = (2 * wave + (ml >> 3)) ^ (n & 7);
-                        *(GNK_LDS _Float16 *)(GNK_LDS char *)(T + n * 128 + 16 * c + 2 * (ml & 7)) = (_Float16)acc[0][j][r];
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[i][j][r] -= (float)(_Float16)acc[i][j][r];
+            }
+        }
+        __syncthreads();                                               // the staging below overwrites the rings, or the hi part's staging
+        if (kg == 0) run_epilogue<Cfg>(g, acc, nullptr, smem, wave, lane, mw, nw);
+        if constexpr (SYM) {
+            if (tm != tn) {
+                if constexpr (MT >= 4) {
+                    if (kg == KG - 1) store_mirror<MT>(p, (char *)g.C, acc, smem + R::LDS / 2 + wave * (64 * 32 * MT), lane, mw, nw);
+                } else {
+                    // 16 rows per wave: transposed rows of 32 bytes would waste the stores; the four waves put theirs side by side first
+                    // (KG = 2: the second set does, in its own ring's LDS; both pass the barrier)
+                    char *const T = smem + R::LDS / 2;                 // [64 n][64 m] fp16, rows of 128 bytes, 16-byte chunk c at c ^ (n & 7)
+                    const int gq = lane >> 4, ml = lane & 15;
+                    if (kg == KG - 1)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int n = 16 * j + 4 * gq + r, c = (2 * wave + (ml >> 3)) ^ (n & 7);
+                            *(GNK_LDS _Float16 *)(GNK_LDS char *)(T + n * 128 + 16 * c + 2 * (ml & 7)) = (_Float16)acc[0][j][r];
+                        }
+                    __syncthreads();
+                    if (kg == KG - 1)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int e = u * 256 + ((int)threadIdx.x & 255), n = e >> 3, c = e & 7;
+                        const v4i v = *(const GNK_LDS v4i *)(const GNK_LDS char *)(T + n * 128 + 16 * (c ^ (n & 7)));
+                        gnk_store16_out((char *)g.C + 2 * ((n0 + n) * p.N + m0) + 16 * c, v);
                     }
-                __syncthreads();
-                char *const C = (char *)p.C + b * p.bc;
-                if (kg == KG - 1)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int e = u * 256 + ((int)threadIdx.x & 255), n = e >> 3, c = e & 7;
-                    const v4i v = *(const GNK_LDS v4i *)(const GNK_LDS char *)(T + n * 128 + 16 * (c ^ (n & 7)));
-                    gnk_store16_out(C + 2 * ((n0 + n) * p.N + m0) + 16 * c, v);
                 }
             }
         }
@@ -389,7 +415,7 @@ __device__ __forceinline__ void finish_half(const Product &p, const GemmParams &
 #pragma unroll
         for (int j = 0; j < 4; ++j) finish_value<EPI>(p, fin, acc[i][j], mw + 16 * i + (lane & 15), nw + 64 * H + 16 * j + 4 * (lane >> 4));
     run_epilogue<Cfg>(g, acc, nullptr, smem, wave * 2 + H, lane, mw, nw + 64 * H);
-    if (mirror) store_mirror<8>(p, b, acc, smem + (wave * 2 + H) * 16384, lane, mw, nw + 64 * H);     // the same slice: a wave's LDS accesses stay in order
+    if (mirror) store_mirror<8>(p, (char *)p.C + b * p.bc, acc, smem + (wave * 2 + H) * 16384, lane, mw, nw + 64 * H);     // the same slice: a wave's LDS accesses stay in order
 }
 
 template <bool AK, bool BK, int EPI, bool SYM>
@@ -485,10 +511,10 @@ __global__ void __launch_bounds__(256) square_sum_kernel(const void *__restrict_
     if (threadIdx.x == 0) parts[b * nparts + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// G 2^p as fp16, padded; fac[b] = {factor of step 0's S, factor of step 0's update}: what takes G 2^p back to X_0.  HBM-bound (8 x 2048 x 5632
+// G 2^p as fp16 (PAIRS: and what that leaves, x_lo bytes behind), padded; fac[b] = {factor of step 0's S, factor of step 0's update}: what takes G 2^p back to X_0.  HBM-bound (8 x 2048 x 5632
 // bf16: 59 us, 6.3 TB/s; most of G is still in the last-level cache).
 template <int DT, int V>
-__global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G, unsigned short *__restrict__ X, const double *__restrict__ parts, float *__restrict__ fac,
+__global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G, unsigned short *__restrict__ X, int64_t x_lo, const double *__restrict__ parts, float *__restrict__ fac,
                                                       int64_t rows, int64_t cols, int64_t rows_p, int64_t cols_p, int nparts, float eps) {
     const int64_t b = blockIdx.y;
     __shared__ double total;
@@ -537,16 +563,25 @@ __global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G
         }
         v4i o;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = (int)gnk_pack2_f16(ldexpf(v[2 * k], p), ldexpf(v[2 * k + 1], p));
-        *(v4i *)(X + (b * rows_p + r) * cols_p + c) = o;
+        for (int k = 0; k < 8; ++k) v[k] = ldexpf(v[k], p);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = (int)gnk_pack2_f16(v[2 * k], v[2 * k + 1]);
+        char *const dst = (char *)(X + (b * rows_p + r) * cols_p + c);
+        *(v4i *)dst = o;
+        if (x_lo) {                                                    // PAIRS
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                o[k] = (int)gnk_pack2_f16(v[2 * k] - (float)(_Float16)v[2 * k], v[2 * k + 1] - (float)(_Float16)v[2 * k + 1]);
+            *(v4i *)(dst + x_lo) = o;
+        }
     }
 }
 
-template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM> int launch(const Product &p0, hipStream_t st) {
+template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM, bool PAIRS = false> int launch(const Product &p0, hipStream_t st) {
     constexpr int LDS_TOTAL = BM == 256 ? 131072 : KG * RingShape<BM == 256 ? 128 : BM>::LDS;
     void (*kernel)(const Product);
     if constexpr (BM == 256) kernel = product256_kernel<AK, BK, EPI, SYM>;
-    else kernel = product_ring_kernel<BM, KG, AK, BK, EPI, SYM>;
+    else kernel = product_ring_kernel<BM, KG, AK, BK, EPI, SYM, PAIRS>;
     Product p = p0;
     p.grid_m = (int)((p.ext_a + BM - 1) / BM);
     p.grid_n = (int)((p.ext_b + BM - 1) / BM);
@@ -571,9 +606,13 @@ struct Plan {
     int64_t x_bytes, s_bytes;                // one matrix
     int nparts;
     int64_t off_x0, off_x1, off_s, off_q, off_parts, off_fac, off_mu, total;
+    int64_t lo_part;                         // pairs: bytes from a matrix's hi part to its lo part, 0 without
 };
 
-Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
+// Results of more than bf16's 8 bits: matrices in two parts
+bool wants_pairs(int out_dtype) { return out_dtype != GNK_BF16; }
+
+Plan make_plan(int64_t batch, int64_t rows, int64_t cols, bool pairs) {
     Plan p;
     p.rp = up(rows); p.cp = up(cols);
     p.lo = rows <= cols ? p.rp : p.cp;
@@ -585,7 +624,8 @@ Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
     p.off_x1 = p.off_x0 + batch * p.x_bytes;
     p.off_s = p.off_x1 + batch * p.x_bytes;
     p.off_q = p.off_s + batch * p.s_bytes;
-    p.off_parts = p.off_q + batch * p.s_bytes;
+    p.lo_part = pairs ? p.off_q + batch * p.s_bytes : 0;
+    p.off_parts = p.off_q + batch * p.s_bytes + p.lo_part;
     p.off_fac = p.off_parts + (batch * p.nparts * 8 + 15) / 16 * 16;
     p.off_mu = p.off_fac + (batch * 8 + 15) / 16 * 16;
     p.total = p.off_mu + (batch * 4 + 15) / 16 * 16;
@@ -595,20 +635,21 @@ Plan make_plan(int64_t batch, int64_t rows, int64_t cols) {
 // Tile size of a product over `batch` matrices, and its time by the cost model of the dense products (gnk_api.hip: us per round of workgroups, one
 // 256 x 256 or two smaller ones per CU; a step is 64 k) with whole rounds and without (what is left where another launch fills the last one).
 struct Choice { int bm, kg; double rounds_us, work_us; };
-Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t batch) {
-    const double cus = (double)gnk_num_cus(), ks = (double)K / 64.0;
+Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t batch, bool pairs) {
+    const double cus = (double)gnk_num_cus(), ks = (double)K / 64.0 * (pairs ? 3.0 : 1.0);
     auto tiles = [&](int64_t bm) {
         const double gm = (double)((ext_a + bm - 1) / bm), gn = (double)((ext_b + bm - 1) / bm);
         return (sym ? gm * (gm + 1) / 2 : gm * gn) * (double)batch;
     };
     auto priced = [&](int bm, int kg, double slots, double per) { return Choice{bm, kg, ceil(tiles(bm) / slots) * per, tiles(bm) / slots * per}; };
-    const Choice c256 = priced(256, 1, cus, 12.0 + 1.3 * ks);
+    Choice c256 = priced(256, 1, cus, 12.0 + 1.3 * ks);
+    if (pairs) c256.rounds_us = 1e30;                 // its loop walks one contraction
     const Choice c128 = tiles(128) <= cus && ks >= 4.0 ? priced(128, 2, cus, 7.0 + 0.55 * ks) : priced(128, 1, 2.0 * cus, 6.0 + 1.0 * ks);
     const bool kg2 = tiles(64) <= cus && ks >= 4.0;
     const Choice c64 = priced(64, kg2 ? 2 : 1, 2.0 * cus, 4.0 + (kg2 ? 0.3 : 0.5) * ks);
     const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1, 5 and 6 force the 128, 256 and 64 tiles here as well
     if (forced == 6 || (forced != 1 && forced != 5 && c64.rounds_us <= c128.rounds_us && c64.rounds_us <= c256.rounds_us)) return c64;
-    if (forced == 5 || (forced != 1 && c256.rounds_us <= c128.rounds_us)) return c256;
+    if (!pairs && (forced == 5 || (forced != 1 && c256.rounds_us <= c128.rounds_us))) return c256;
     return c128;
 }
 
@@ -619,16 +660,21 @@ template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p,
     return launch<64, 1, AK, BK, EPI, SYM>(p, st);
 }
 
+template <bool AK, bool BK, int EPI, bool SYM> int run_pairs(const Product &p, const Choice &c, hipStream_t st) {
+    if (c.bm == 128) return c.kg == 2 ? launch<128, 2, AK, BK, EPI, SYM, true>(p, st) : launch<128, 1, AK, BK, EPI, SYM, true>(p, st);
+    return c.kg == 2 ? launch<64, 2, AK, BK, EPI, SYM, true>(p, st) : launch<64, 1, AK, BK, EPI, SYM, true>(p, st);
+}
+
 template <int DT> int read_input(const void *G, char *X, double *parts, float *fac, int64_t batch, int64_t rows, int64_t cols, const Plan &pl, float eps, hipStream_t st) {
     const dim3 g1((unsigned)pl.nparts, (unsigned)batch);
     const int64_t octets = pl.rp * pl.cp / 8, want = (octets + 255) / 256;
     const dim3 g2((unsigned)(want < 1024 ? want : 1024), (unsigned)batch);
     if (cols % VEC<DT> == 0 && ((uintptr_t)G & 15) == 0) {
         hipLaunchKernelGGL((square_sum_kernel<DT, VEC<DT>>), g1, dim3(256), 0, st, G, parts, rows * cols, pl.nparts);
-        hipLaunchKernelGGL((convert_kernel<DT, VEC<DT>>), g2, dim3(256), 0, st, G, (unsigned short *)X, parts, fac, rows, cols, pl.rp, pl.cp, pl.nparts, eps);
+        hipLaunchKernelGGL((convert_kernel<DT, VEC<DT>>), g2, dim3(256), 0, st, G, (unsigned short *)X, pl.lo_part, parts, fac, rows, cols, pl.rp, pl.cp, pl.nparts, eps);
     } else {
         hipLaunchKernelGGL((square_sum_kernel<DT, 1>), g1, dim3(256), 0, st, G, parts, rows * cols, pl.nparts);
-        hipLaunchKernelGGL((convert_kernel<DT, 1>), g2, dim3(256), 0, st, G, (unsigned short *)X, parts, fac, rows, cols, pl.rp, pl.cp, pl.nparts, eps);
+        hipLaunchKernelGGL((convert_kernel<DT, 1>), g2, dim3(256), 0, st, G, (unsigned short *)X, pl.lo_part, parts, fac, rows, cols, pl.rp, pl.cp, pl.nparts, eps);
     }
     return gnk_check_launch("orthogonalize");
 }
@@ -676,7 +722,12 @@ struct SideStream {
 
 extern "C" int64_t gnk_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) {
     if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
-    return make_plan(batch, rows, cols).total;
+    return make_plan(batch, rows, cols, true).total;
+}
+
+extern "C" int64_t gnk_orthogonalize_workspace_bytes_of(int out_dtype, int64_t batch, int64_t rows, int64_t cols) {
+    if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    return make_plan(batch, rows, cols, wants_pairs(out_dtype)).total;
 }
 
 extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
@@ -690,7 +741,8 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
     if (batch > 65535 || rows > (1 << 20) || cols > (1 << 20)) return gnk_fail(GNK_ERR_UNSUPPORTED, "%s: %lld matrices of %lld x %lld", name, (long long)batch, (long long)rows, (long long)cols);
     if (batch == 0 || rows == 0 || cols == 0) return GNK_OK;
     if (!G || !out) return gnk_fail(GNK_ERR_BAD_ARG, "%s: null pointer", name);
-    const Plan pl = make_plan(batch, rows, cols);
+    const bool pairs = wants_pairs(out_dtype);
+    const Plan pl = make_plan(batch, rows, cols, pairs);
     if (!workspace || workspace_bytes < pl.total || ((uintptr_t)workspace & 15) != 0)
         return gnk_fail(GNK_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %lld bytes", name, (long long)pl.total);
     int rc = gnk_init();
@@ -709,11 +761,11 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
     const bool wide = rows <= cols;
     float sq = 32768.0f;                     // scale of Q - mu I: |Q|, |mu| <= |a| + 2 |b| + 4 |c| while the singular values stay below sqrt 2
     while (sq * cmax >= 16384.0f) sq *= 0.5f;
-    const bool with_mu = (wide ? rows : cols) < MU_ROWS;
+    const bool with_mu = !pairs && (wide ? rows : cols) < MU_ROWS;
     const int64_t lo = pl.lo, ldx = 2 * pl.cp, lds = 2 * lo;
     // chosen for the whole stack, however it is split below: the results do not depend on the split
-    const Choice c_gram = choose_tile(lo, lo, wide ? pl.cp : pl.rp, true, batch), c_poly = choose_tile(lo, lo, lo, true, batch);
-    const Choice c_next = choose_tile(pl.rp, pl.cp, lo, false, batch);
+    const Choice c_gram = choose_tile(lo, lo, wide ? pl.cp : pl.rp, true, batch, pairs), c_poly = choose_tile(lo, lo, lo, true, batch, pairs);
+    const Choice c_next = choose_tile(pl.rp, pl.cp, lo, false, batch, pairs);
     // one step of matrices b0 .. b0 + n - 1 on stream s
     auto one_step = [&](int it, int64_t b0, int64_t n, hipStream_t s) -> int {
         const bool last = it + 1 == steps;
@@ -723,6 +775,7 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         memset(&p, 0, sizeof(p));
         p.batch = (int)n;
         p.fstride = 2;
+        p.a_lo = p.b_lo = p.c_lo = p.d_lo = pl.lo_part;
         p.mu = with_mu ? (float *)(ws + pl.off_mu) + b0 : nullptr;
         // S
         p.A = p.B = X; p.ba = p.bb = pl.x_bytes; p.lda = p.ldb = ldx;
@@ -732,7 +785,9 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.f = it == 0 ? SS : SS / (SX * SX);
         p.fdev = it == 0 ? fac + 2 * b0 : nullptr;
         p.out_dtype = GNK_F16;
-        int rc = wide ? run_product<true, true, GRAM, true>(p, c_gram, s) : run_product<false, false, GRAM, true>(p, c_gram, s);
+        int rc = pairs  ? (wide ? run_pairs<true, true, GRAM, true>(p, c_gram, s) : run_pairs<false, false, GRAM, true>(p, c_gram, s))
+                 : wide ? run_product<true, true, GRAM, true>(p, c_gram, s)
+                        : run_product<false, false, GRAM, true>(p, c_gram, s);
         if (rc) return rc;
         // Q - mu I = (a - mu) I + b S + c S^2
         p.A = p.B = S; p.ba = p.bb = pl.s_bytes; p.lda = p.ldb = lds;
@@ -742,7 +797,7 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.f = c * sq / (SS * SS); p.g = b * sq / SS; p.h = a; p.k = sq;
         p.c0 = a; p.c1 = b; p.c2 = c; p.diag_scale = 1.0f / (SS * (float)(wide ? rows : cols));
         p.fdev = nullptr;
-        rc = run_product<true, true, POLY, true>(p, c_poly, s);
+        rc = pairs ? run_pairs<true, true, POLY, true>(p, c_poly, s) : run_product<true, true, POLY, true>(p, c_poly, s);
         if (rc) return rc;
         // X <- Q X or X Q: the product with Q - mu I, and mu X
         p.A = wide ? Q : X; p.ba = wide ? pl.s_bytes : pl.x_bytes; p.lda = wide ? lds : ldx;
@@ -756,6 +811,8 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.out_dtype = last ? out_dtype : GNK_F16;
         p.f = (last ? 1.0f : SX) / (it == 0 ? sq : sq * SX);
         p.fdev = it == 0 ? fac + 2 * b0 + 1 : nullptr;
+        if (last) p.c_lo = 0;
+        if (pairs) return wide ? run_pairs<true, false, GRAM, false>(p, c_next, s) : run_pairs<true, true, GRAM, false>(p, c_next, s);
         if (with_mu) return wide ? run_product<true, false, UPDATE, false>(p, c_next, s) : run_product<true, true, UPDATE, false>(p, c_next, s);
         return wide ? run_product<true, false, GRAM, false>(p, c_next, s) : run_product<true, true, GRAM, false>(p, c_next, s);
     };

@@ -366,9 +366,9 @@ at::Tensor orthogonalize(const at::Tensor &G_in, int64_t steps, double a, double
     for (int64_t d = 0; d < G.dim() - 2; ++d) batch *= G.size(d);
     at::Tensor out = at::empty(G.sizes(), G.options());
     const c10::hip::OptionalHIPGuardMasqueradingAsCUDA guard(G.device());
-    const int64_t nws = gnk_orthogonalize_workspace_bytes(batch, rows, cols);
-    const at::Tensor ws = workspace_for(G, nws);
     const int code = dtype_code(G.scalar_type(), op);
+    const int64_t nws = gnk_orthogonalize_workspace_bytes_of(code, batch, rows, cols);
+    const at::Tensor ws = workspace_for(G, nws);
     check(gnk_orthogonalize(G.data_ptr(), code, out.data_ptr(), code, batch, rows, cols, (int)steps, (float)a, (float)b, (float)c, (float)eps,
                             nws > 0 ? ws.data_ptr() : nullptr, nws, stream_of(G)),
           op);

@@ -45,7 +45,7 @@ def _hip(G: Tensor, steps: int, a: float, b: float, c: float, eps: float):
     out = torch.empty_like(G)
     L, code = _cabi.load(), _cabi.DTYPE_CODE[G.dtype]
     with _cabi.device_of(G):
-        nws = L.gnk_orthogonalize_workspace_bytes(batch, rows, cols)
+        nws = L.gnk_orthogonalize_workspace_bytes_of(code, batch, rows, cols)
         ws = torch.empty(nws, dtype=torch.uint8, device=G.device) if nws else None
         rc = L.gnk_orthogonalize(G.data_ptr(), code, out.data_ptr(), code, batch, rows, cols, steps, a, b, c, eps, ws.data_ptr() if nws else None, nws,
                                  _cabi.stream_of(G))

@@ -206,3 +206,73 @@ def test_refusals():
         torch.ops.gn_kernels.orthogonalize(torch.zeros(4, 4, device=DEV), 5, 1e6, 0.0, 0.0, 1e-7)
     assert gn_kernels.orthogonalize(torch.zeros(0, 4, 5, device=DEV)).shape == (0, 4, 5)
     assert gn_kernels.orthogonalize(torch.zeros(3, 0, 5, device=DEV)).shape == (3, 0, 5)
+
+
+# ------------------------------------------------------------------------------------------------ results of more than 8 bits
+# Every matrix is kept in two fp16 parts: |v - hi| <= 2^-11 |v|, the rounding of that 2^-22 |v|; a product drops lo lo, 2^-22 of sum |a b|.  Four such
+# perturbations per step (S, S^2, Q, X), each stretched by later steps by at most a = 3.4445: 4 (a^5 - 1) / (a - 1) 2^-22 = 1.9e-4 of the norm, 3e-4 with the
+# fp32 sums and norms that shrink to 0.7 on the way; plus half a step of the result's type.  (One fp16 part per matrix is off by 1.1e-3.)
+def compare_closely(got, G, **kw):
+    want = iterate(G, kw.get("steps", 5), kw.get("co", COEFFS), 1e-7, False)
+    assert got.dtype is G.dtype and got.shape == G.shape
+    err = (got.double().cpu() - want).norm().item() / want.norm().item()
+    tol = 3e-4 + torch.finfo(G.dtype).eps / 2
+    assert err <= tol, f"{err:.3e} off, tolerance {tol:.3e}"
+    return err
+
+
+@pytest.mark.parametrize("m,n", [(1, 1), (3, 2), (36, 2230), (200, 96), (129, 127), (333, 999), (999, 333), (600, 600), (1100, 700)])
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("kind", ["gauss", "momentum"])
+def test_more_bits(forced, m, n, dt, kind):
+    G = matrix(m, n, dt, seed=m, kind=kind)
+    compare_closely(gn_kernels.orthogonalize(G.to(DEV)), G)
+
+
+@pytest.mark.parametrize("dt", ["f16", "f32"])
+@pytest.mark.parametrize("scale", [1e-4, 1.0, 200.0])
+def test_more_bits_stacks_scales_steps(dt, scale):
+    G = torch.stack([matrix(150, 260, dt, seed=i, kind="gauss") * scale for i in range(5)])
+    got = gn_kernels.orthogonalize(G.to(DEV))
+    for x, g in zip(got, G):
+        compare_closely(x, g)
+    for steps in (1, 2, 4):
+        compare_closely(gn_kernels.orthogonalize(G[0].to(DEV), steps=steps), G[0], steps=steps)
+    compare_closely(gn_kernels.orthogonalize(G[1].to(DEV), coefficients=(2.0, -1.5, 0.5)), G[1], co=(2.0, -1.5, 0.5))
+
+
+def test_more_bits_large_stack_and_graph():
+    """Two streams outside a captured graph, one inside: the same bits."""
+    G = torch.stack([matrix(2048, 4224, "f16", seed=i, kind="gauss") for i in range(3)]).to(DEV)
+    want = gn_kernels.orthogonalize(G)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = gn_kernels.orthogonalize(G)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    X = want[0].float()
+    one = torch.linalg.svdvals(X[:, :2048].contiguous())
+    assert torch.isfinite(want).all() and one.max() < 1.5
+    sub = G[:1, :512, :1024].contiguous()
+    compare_closely(gn_kernels.orthogonalize(sub)[0], sub[0].cpu())
+
+
+def test_more_bits_special_values():
+    for dt in (torch.float16, torch.float32):
+        G = torch.randn(3, 40, 70, generator=torch.Generator().manual_seed(1)).to(dt)
+        G[0, 3, 5], G[1] = float("nan"), 0.0
+        got = gn_kernels.orthogonalize(G.to(DEV))
+        assert got[0].isnan().all() and (got[1] == 0).all()
+        compare_closely(got[2], G[2])
+
+
+def test_workspace_is_half_for_bf16():
+    L, d = _cabi.load(), _cabi.DTYPE_CODE
+    need = lambda dt: L.gnk_orthogonalize_workspace_bytes_of(d[dt], 2, 500, 700)  # noqa: E731
+    assert need(torch.bfloat16) < 0.51 * need(torch.float32) and need(torch.float16) == need(torch.float32) == L.gnk_orthogonalize_workspace_bytes(2, 500, 700)
+    G = matrix(500, 700, "f16").to(DEV)
+    out, ws = torch.empty_like(G), torch.empty(L.gnk_orthogonalize_workspace_bytes_of(d[torch.bfloat16], 1, 500, 700), dtype=torch.uint8, device=DEV)
+    rc = L.gnk_orthogonalize(G.data_ptr(), d[G.dtype], out.data_ptr(), d[G.dtype], 1, 500, 700, 5, *COEFFS, 1e-7, ws.data_ptr(), ws.numel(), None)
+    assert rc == -4 and b"workspace" in L.gnk_last_error()
