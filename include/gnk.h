@@ -312,8 +312,8 @@ int gnk_quantize_int8_grouped(const void *x, int x_dtype, const int32_t *ends, i
  * Newton-Schulz orthogonalisation of a stack of matrices (the update of an optimizer that orthogonalises its momentum; no reference counterpart):
  *   X = G / max(|G|_F, eps);  `steps` times:  X <- a X + b (X X^T) X + c (X X^T)^2 X      (the smaller of X X^T and X^T X is formed)
  * G and out (batch, rows, cols) contiguous, any of BF16 / F16 / F32 each; 1 <= steps <= 100.  The intermediate matrices are fp16 scaled by powers
- * of two, sums fp32, the norm fp64: the result is off by about 1.5e-3 of its norm for five steps of the usual (3.4445, -4.7750, 2.0315) on matrices
- * with singular values within a factor of 1000, more for directions below that.  The coefficients must keep the singular values below sqrt 2 (larger
+ * of two (one part for a BF16 result, two, of 22 bits together, for the others), sums fp32, the norm fp64: for five steps of the usual (3.4445, -4.7750, 2.0315)
+ * the result is off by about 1.2e-3 of its norm beside its rounding in BF16, 3e-6 in the others.  The coefficients must keep the singular values below sqrt 2 (larger
  * intermediates may overflow to Inf).  A matrix that holds a NaN or Inf comes out as NaN; one of zeros as zeros.  rows, cols <= 2^20, batch < 2^16.
  * workspace: gnk_orthogonalize_workspace_bytes_of() bytes for results of that type (half as much for BF16 as for the others), or
  * gnk_orthogonalize_workspace_bytes(), enough for any; 16-byte aligned, need not be cleared.  Overlapping calls need one each.

@@ -12,7 +12,7 @@
 //   rounding of X is most of the error (512 x 512: 1.4e-3 of 1.6e-3) and the second read of X costs 15 % of that product: mu = 0 there.
 // That is an eighth of what a bf16 result is rounded by and five times a fp16 result's rounding, so results of 11 and 24 bits (fp16, fp32) are computed with every
 // matrix in two fp16 parts, hi + lo (PAIRS; 22 bits, no mu): a product is hi hi + lo hi + hi lo, one loop over three times the contraction.  Off by 2.1e-4 of the
-// norm for fp16, its rounding, and ORTHO_F32_ERR for fp32; ORTHO_F16_TIMES.
+// norm for fp16, its rounding, and 1-3e-6 for fp32, where one part each gave 1.1e-3; 999 x 333 228 us instead of 120, 8 x 2048 x 5632 8.8 ms instead of 2.9.
 // Shapes are padded with zeros to multiples of 128 in the workspace: zero rows and columns stay zero through every product.
 //
 // The products: `wide` S = X X^T reads both operands along K, Q X reads X as it lies (N-contiguous, transposed on the way out of LDS); `tall` S = X^T X
@@ -59,6 +59,7 @@ struct Product {
     int fstride;
     int out_dtype;
     int batch, grid_m, grid_n;
+    int parts;                               // PAIRS, 128 and 64 tiles: 3, or 1 where neither factor has a lo part
 };
 
 // Tile of a workgroup: the XCDs take contiguous runs of tiles (matrices one after the other), each walked in strips of four tile rows.
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = (v4f){0.f, 0.f, 0.f, 0.f};
-    const int nk_one = (int)(p.K / 64), nk_all = PAIRS ? 3 * nk_one : nk_one;
+    const int nk_one = (int)(p.K / 64), nk_all = PAIRS ? p.parts * nk_one : nk_one;
     const int nk = (nk_all + KG - 1 - kg) / KG, nk_most = KG == 1 ? nk : (nk_all + KG - 1) / KG;      // steps kg, kg + KG, ...
     const char *const a0 = sa.base, *const b0 = sb.base;
     if constexpr (KG > 1 && !PAIRS) {
@@ -405,21 +406,38 @@ template <int H, int I> __device__ __forceinline__ void fetch_row(v4f (&acc)[8][
 }
 
 // columns 64 H .. 64 H + 63 of the wave tile: accumulators -> values -> memory
-template <class Cfg, int EPI, int H>
-__device__ __forceinline__ void finish_half(const Product &p, const GemmParams &g, int b, bool mirror, const Finish &fin, char *smem, int wave, int lane, int64_t mw, int64_t nw) {
+template <class Cfg, int EPI, int H, bool PAIRS>
+__device__ __forceinline__ void finish_half(const Product &p, GemmParams g, int b, bool mirror, const Finish &fin, char *smem, int wave, int lane, int64_t mw, int64_t nw) {
     v4f acc[8][4];
     fetch_row<H, 0>(acc); fetch_row<H, 1>(acc); fetch_row<H, 2>(acc); fetch_row<H, 3>(acc);
     fetch_row<H, 4>(acc); fetch_row<H, 5>(acc); fetch_row<H, 6>(acc); fetch_row<H, 7>(acc);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) finish_value<EPI>(p, fin, acc[i][j], mw + 16 * i + (lane & 15), nw + 64 * H + 16 * j + 4 * (lane >> 4));
-    run_epilogue<Cfg>(g, acc, nullptr, smem, wave * 2 + H, lane, mw, nw + 64 * H);
-    if (mirror) store_mirror<8>(p, (char *)p.C + b * p.bc, acc, smem + (wave * 2 + H) * 16384, lane, mw, nw + 64 * H);     // the same slice: a wave's LDS accesses stay in order
+        for (int j = 0; j < 4; ++j) finish_value<EPI, PAIRS>(p, fin, acc[i][j], mw + 16 * i + (lane & 15), nw + 64 * H + 16 * j + 4 * (lane >> 4));
+    // all through the same slice of LDS: a wave's accesses stay in order
+    if constexpr (!PAIRS) {
+        run_epilogue<Cfg>(g, acc, nullptr, smem, wave * 2 + H, lane, mw, nw + 64 * H);
+        if (mirror) store_mirror<8>(p, (char *)g.C, acc, smem + (wave * 2 + H) * 16384, lane, mw, nw + 64 * H);
+    } else {                                                                  // no mirror images here (choose_tile)
+#pragma nounroll
+        for (int part = 0; part < (p.c_lo ? 2 : 1); ++part) {                 // hi, then what it leaves; not unrolled: registers
+            run_epilogue<Cfg>(g, acc, nullptr, smem, wave * 2 + H, lane, mw, nw + 64 * H);
+            g.C = (char *)g.C + p.c_lo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] -= (float)(_Float16)acc[i][j][r];
+        }
+    }
 }
 
-template <bool AK, bool BK, int EPI, bool SYM>
+// PAIRS: the loop three times, the second and third on top of the first one's sums (lo hi, hi lo).
+template <bool AK, bool BK, int EPI, bool SYM, bool PAIRS>
 __global__ void __launch_bounds__(256) product256_kernel(const Product p) {
+    static_assert(!PAIRS || (AK && !SYM), "with mirror images: too many registers");
     extern __shared__ __attribute__((aligned(16))) char smem[];
     typedef GemmCfg<256, 256, 2, 4, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;      // the epilogue's maps: 128 x 64 halves of a wave's 128 x 128
     const int lane = threadIdx.x & 63;
@@ -436,22 +454,28 @@ __global__ void __launch_bounds__(256) product256_kernel(const Product p) {
     const unsigned lds0 = (unsigned)(uintptr_t)(GNK_LDS char *)smem;
     const unsigned va = lds0 + (AK ? gnk_kmaj_frag_offset(wm * 128, 0, lane) : gnk_mn16_frag_offset<512>(wm * 128, 0, lane));
     const unsigned vb = lds0 + 65536 + (BK ? gnk_kmaj_frag_offset(wn * 128, 0, lane) : gnk_mn16_frag_offset<512>(wn * 128, 0, lane));
-    const unsigned alo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)sa.base), ahi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)sa.base >> 32));
-    const unsigned blo = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)sb.base), bhi = __builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)sb.base >> 32));
+    const auto low = [](const char *at) { return (unsigned)__builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)at); };
+    const auto high = [](const char *at) { return (unsigned)__builtin_amdgcn_readfirstlane((unsigned)((uintptr_t)at >> 32)); };
     const unsigned stepa = __builtin_amdgcn_readfirstlane((unsigned)sa.step), stepb = __builtin_amdgcn_readfirstlane((unsigned)sb.step);
     const unsigned ldsw = __builtin_amdgcn_readfirstlane(lds0 + wave * 1024);
     const int ns = (int)(p.K / 32);
     const int nit = __builtin_amdgcn_readfirstlane(ns >> 2), rem = __builtin_amdgcn_readfirstlane(ns - 1);
-#define GNK_ORTHO_RUN(TEXT)                                                                                                           \
-    asm volatile(TEXT : : [alo] "s"(alo), [ahi] "s"(ahi), [blo] "s"(blo), [bhi] "s"(bhi), [stepa] "s"(stepa), [stepb] "s"(stepb),      \
+#define GNK_ORTHO_RUN(TEXT, A, B)                                                                                                     \
+    asm volatile(TEXT : : [alo] "s"(low(A)), [ahi] "s"(high(A)), [blo] "s"(low(B)), [bhi] "s"(high(B)), [stepa] "s"(stepa), [stepb] "s"(stepb),      \
                  [lds] "s"(ldsw), [nit] "s"(nit), [rem] "s"(rem), [va] "v"(va), [vb] "v"(vb),                                         \
                  [oa0] "v"(sa.off[0]), [oa1] "v"(sa.off[1]), [oa2] "v"(sa.off[2]), [oa3] "v"(sa.off[3]),                              \
                  [oa4] "v"(sa.off[4]), [oa5] "v"(sa.off[5]), [oa6] "v"(sa.off[6]), [oa7] "v"(sa.off[7]),                              \
                  [ob0] "v"(sb.off[0]), [ob1] "v"(sb.off[1]), [ob2] "v"(sb.off[2]), [ob3] "v"(sb.off[3]),                              \
                  [ob4] "v"(sb.off[4]), [ob5] "v"(sb.off[5]), [ob6] "v"(sb.off[6]), [ob7] "v"(sb.off[7]) : GNK_W4_CLOBBERS)
-    if constexpr (AK && BK) GNK_ORTHO_RUN(GNK_W4_ASM_F16_KK);
-    else if constexpr (AK) GNK_ORTHO_RUN(GNK_W4_ASM_F16_KM);
-    else GNK_ORTHO_RUN(GNK_W4_ASM_F16_MM);
+    const char *const A = sa.base, *const B = sb.base;
+    if constexpr (AK && BK) GNK_ORTHO_RUN(GNK_W4_ASM_F16_KK, A, B);
+    else if constexpr (AK) GNK_ORTHO_RUN(GNK_W4_ASM_F16_KM, A, B);
+    else GNK_ORTHO_RUN(GNK_W4_ASM_F16_MM, A, B);
+    if constexpr (PAIRS) {
+        const char *const Al = A + p.a_lo, *const Bl = B + p.b_lo;
+        if constexpr (AK && BK) { GNK_ORTHO_RUN(GNK_W4_ASM_F16_KK_ADD, Al, B); GNK_ORTHO_RUN(GNK_W4_ASM_F16_KK_ADD, A, Bl); }
+        else { GNK_ORTHO_RUN(GNK_W4_ASM_F16_KM_ADD, Al, B); GNK_ORTHO_RUN(GNK_W4_ASM_F16_KM_ADD, A, Bl); }
+    }
 #undef GNK_ORTHO_RUN
     // the asm ends behind vmcnt(0) + a barrier: LDS is free for the epilogue
     float diag_sum = 0.0f;
@@ -460,8 +484,8 @@ __global__ void __launch_bounds__(256) product256_kernel(const Product p) {
     const GemmParams g = store_params(p, b);
     const int64_t mw = m0 + wm * 128, nw = n0 + wn * 128;
     const bool mirror = SYM && tm != tn;
-    finish_half<Cfg, EPI, 0>(p, g, b, mirror, fin, smem, wave, lane, mw, nw);
-    finish_half<Cfg, EPI, 1>(p, g, b, mirror, fin, smem, wave, lane, mw, nw);
+    finish_half<Cfg, EPI, 0, PAIRS>(p, g, b, mirror, fin, smem, wave, lane, mw, nw);
+    finish_half<Cfg, EPI, 1, PAIRS>(p, g, b, mirror, fin, smem, wave, lane, mw, nw);
 }
 
 // ------------------------------------------------------------------------------ sums of squares, conversion
@@ -580,7 +604,7 @@ __global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G
 template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM, bool PAIRS = false> int launch(const Product &p0, hipStream_t st) {
     constexpr int LDS_TOTAL = BM == 256 ? 131072 : KG * RingShape<BM == 256 ? 128 : BM>::LDS;
     void (*kernel)(const Product);
-    if constexpr (BM == 256) kernel = product256_kernel<AK, BK, EPI, SYM>;
+    if constexpr (BM == 256) kernel = product256_kernel<AK, BK, EPI, SYM, PAIRS>;
     else kernel = product_ring_kernel<BM, KG, AK, BK, EPI, SYM, PAIRS>;
     Product p = p0;
     p.grid_m = (int)((p.ext_a + BM - 1) / BM);
@@ -642,14 +666,16 @@ Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t ba
         return (sym ? gm * (gm + 1) / 2 : gm * gn) * (double)batch;
     };
     auto priced = [&](int bm, int kg, double slots, double per) { return Choice{bm, kg, ceil(tiles(bm) / slots) * per, tiles(bm) / slots * per}; };
-    Choice c256 = priced(256, 1, cus, 12.0 + 1.3 * ks);
-    if (pairs) c256.rounds_us = 1e30;                 // its loop walks one contraction
+    Choice c256 = priced(256, 1, cus, (pairs ? 20.0 : 12.0) + 1.3 * ks);      // pairs: three loops' first loads, two stores
+    // hi, lo and both mirror images together take more registers than the accumulators leave: the compiler would put values into those that are not read yet
+    const bool can256 = !(pairs && sym);
+    if (!can256) c256.rounds_us = 1e30;
     const Choice c128 = tiles(128) <= cus && ks >= 4.0 ? priced(128, 2, cus, 7.0 + 0.55 * ks) : priced(128, 1, 2.0 * cus, 6.0 + 1.0 * ks);
     const bool kg2 = tiles(64) <= cus && ks >= 4.0;
     const Choice c64 = priced(64, kg2 ? 2 : 1, 2.0 * cus, 4.0 + (kg2 ? 0.3 : 0.5) * ks);
     const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1, 5 and 6 force the 128, 256 and 64 tiles here as well
     if (forced == 6 || (forced != 1 && forced != 5 && c64.rounds_us <= c128.rounds_us && c64.rounds_us <= c256.rounds_us)) return c64;
-    if (!pairs && (forced == 5 || (forced != 1 && c256.rounds_us <= c128.rounds_us))) return c256;
+    if (can256 && (forced == 5 || (forced != 1 && c256.rounds_us <= c128.rounds_us))) return c256;
     return c128;
 }
 
@@ -661,6 +687,8 @@ template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p,
 }
 
 template <bool AK, bool BK, int EPI, bool SYM> int run_pairs(const Product &p, const Choice &c, hipStream_t st) {
+    if constexpr (!SYM)
+        if (c.bm == 256) return launch<256, 1, AK, BK, EPI, SYM, true>(p, st);
     if (c.bm == 128) return c.kg == 2 ? launch<128, 2, AK, BK, EPI, SYM, true>(p, st) : launch<128, 1, AK, BK, EPI, SYM, true>(p, st);
     return c.kg == 2 ? launch<64, 2, AK, BK, EPI, SYM, true>(p, st) : launch<64, 1, AK, BK, EPI, SYM, true>(p, st);
 }
@@ -785,10 +813,12 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         p.f = it == 0 ? SS : SS / (SX * SX);
         p.fdev = it == 0 ? fac + 2 * b0 : nullptr;
         p.out_dtype = GNK_F16;
+        p.parts = it == 0 && g_dtype != GNK_F32 ? 1 : 3;                       // X_0 of 16-bit inputs is exact
         int rc = pairs  ? (wide ? run_pairs<true, true, GRAM, true>(p, c_gram, s) : run_pairs<false, false, GRAM, true>(p, c_gram, s))
                  : wide ? run_product<true, true, GRAM, true>(p, c_gram, s)
                         : run_product<false, false, GRAM, true>(p, c_gram, s);
         if (rc) return rc;
+        p.parts = 3;
         // Q - mu I = (a - mu) I + b S + c S^2
         p.A = p.B = S; p.ba = p.bb = pl.s_bytes; p.lda = p.ldb = lds;
         p.C = Q; p.bc = pl.s_bytes;

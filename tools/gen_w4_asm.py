@@ -54,8 +54,9 @@ def rng(r, n):
 
 
 class Gen:
-    def __init__(self, op, ak, bk, ragged=False, rows=256):
+    def __init__(self, op, ak, bk, ragged=False, rows=256, add=False):
         self.op = op
+        self.add = add                   # on top of what the accumulators hold
         self.rows = rows                 # of the tile: 256, or 192 (int8, A K-major: three quarters of A's fragments, pieces and super-stage)
         assert rows == 256 or (rows == 192 and op == "i8" and ak)
         self.ragged = ragged
@@ -267,7 +268,7 @@ class Gen:
                 self.emit_piece(pc)
                 k += 1
                 upto = 256 * k // npieces
-                for r in range(cleared, upto):
+                for r in range(cleared, upto) if not self.add else ():
                     e(f"v_accvgpr_write_b32 a{r}, 0")
                 cleared = upto
             for operand in ("a", "b"):
@@ -305,10 +306,11 @@ HEAD = "// GENERATED by tools/gen_w4_asm.py -- do not edit; see that file for th
 
 
 def main():
-    # loops beside the dense 8-bit ones: ragged K (products grouped by expert), 16-bit floats
+    # loops beside the dense 8-bit ones: ragged K (products grouped by expert), 16-bit floats, the same on top of another loop's sums
     more = [HEAD] + [macro(f"GNK_W4_ASM_{op.upper()}_MM_RAGGED", Gen(op, False, False, ragged=True)) for op in ("i8", "f8")]
     more += [macro(f"GNK_W4_ASM_I8_K{'K' if bk else 'M'}_192", Gen("i8", True, bk, rows=192)) for bk in (True, False)]
-    more += [macro(f"GNK_W4_ASM_F16_{'K' if ak else 'M'}{'K' if bk else 'M'}", Gen("f16", ak, bk)) for ak, bk in ((True, True), (True, False), (False, False))]
+    more += [macro(f"GNK_W4_ASM_F16_{'K' if ak else 'M'}{'K' if bk else 'M'}{'_ADD' if add else ''}", Gen("f16", ak, bk, add=add))
+             for add in (False, True) for ak, bk in ((True, True), (True, False), (False, False)) if ak or not add]
     more.append("#define GNK_W4_CLOBBERS_RAGGED GNK_W4_CLOBBERS, " + ", ".join(f'"s{r}"' for r in range(92, 100)) + "\n")
     MORE.write_text("\n".join(more))
     parts = [HEAD]
