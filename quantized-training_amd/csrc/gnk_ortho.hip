@@ -12,7 +12,7 @@
 //   rounding of X is most of the error (512 x 512: 1.4e-3 of 1.6e-3) and the second read of X costs 15 % of that product: mu = 0 there.
 // That is an eighth of what a bf16 result is rounded by and five times a fp16 result's rounding, so results of 11 and 24 bits (fp16, fp32) are computed with every
 // matrix in two fp16 parts, hi + lo (PAIRS; 22 bits, no mu): a product is hi hi + lo hi + hi lo, one loop over three times the contraction.  Off by 2.1e-4 of the
-// norm for fp16, its rounding, and 1-3e-6 for fp32, where one part each gave 1.1e-3; 999 x 333 228 us instead of 120, 8 x 2048 x 5632 8.8 ms instead of 2.9.
+// norm for fp16, its rounding, and 1-3e-6 for fp32, where one part each gave 1.1e-3; 999 x 333 207 us instead of 120, 8 x 2048 x 5632 8.8 ms instead of 2.9.
 // Shapes are padded with zeros to multiples of 128 in the workspace: zero rows and columns stay zero through every product.
 //
 // The products: `wide` S = X X^T reads both operands along K, Q X reads X as it lies (N-contiguous, transposed on the way out of LDS); `tall` S = X^T X
@@ -222,20 +222,22 @@ template <bool KMAJOR, int BM> __device__ __forceinline__ v8h frag16(const char 
 // BM = 128: 2 x 2 waves of 64 x 64, two stages (64 KiB: two workgroups per CU).  BM = 64: 2 x 2 waves of 32 x 32 would halve the fragment reads, but the
 // stores want 64 columns per wave: 4 x 1 waves of 16 x 64; four stages (64 KiB) because few tiles are bound by the latency of a step, not by its work.
 // KG = 2 (at most one workgroup per CU): a second set of four waves with a ring of its own takes every other step of the contraction; the two
-// halves meet in LDS, in the same order on both sides, and then one set stores the tile and the other its mirror image.
+// halves meet in LDS, in the same order on both sides, and then one set stores the tile and the other its mirror image.  KG = 4 (64 tiles, from 24 steps on):
+// four sets with two stages each.  100 x 4096 153 -> 137 us, 3000 x 400 206 -> 184, 1024 x 1024 fp16 360 -> 322; with 16 steps 121 -> 118 for one part, but
+// 207 -> 216 us for pairs' 18 (999 x 333), with 8 slower everywhere.
 // Bound by latency: a launch with one step takes 3 us, each further 64-k step of a set 0.7 (fragment reads, barrier), so 333 x 333 over K = 1024 takes 8.2 us.
 // Two sets instead of one, tiles of 128: 2048 x 2048 530 -> 428 us, 2048 x 5632 749 -> 652 us (whole calls).
-template <int BM> struct RingShape {
-    static constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1, MT = BM / WM / 16, NST = BM == 128 ? 2 : 4, OPER = BM * 128, STAGE = 2 * OPER;
+template <int BM, int KG> struct RingShape {
+    static constexpr int WM = BM == 128 ? 2 : 4, WN = BM == 128 ? 2 : 1, MT = BM / WM / 16, NST = BM == 128 || KG == 4 ? 2 : 4, OPER = BM * 128, STAGE = 2 * OPER;
     static constexpr int LDS = NST * STAGE;
 };
 
 // PAIRS: the steps of hi hi, then lo hi, then hi lo; the result is stored as hi = fp16(v) and lo = fp16(v - hi), the last one in its own type.
 template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM, bool PAIRS>
-__global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2))) product_ring_kernel(const Product p) {
+__global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(KG == 4 ? 4 : 2))) product_ring_kernel(const Product p) {
     extern __shared__ __attribute__((aligned(16))) char smem_all[];
-    typedef RingShape<BM> R;
-    static_assert(KG == 1 || KG == 2, "one or two sets of waves");
+    typedef RingShape<BM, KG> R;
+    static_assert(KG == 1 || KG == 2 || (KG == 4 && BM == 64), "sets of waves");
     typedef GemmCfg<BM, BM, R::WM, R::WN, AK, BK, OP_F8, 0, 0, EPI_PLAIN> Cfg;     // fp32 accumulators and the epilogue's maps
     constexpr int MT = R::MT, NST = R::NST, PIECES = 2 * BM / 32;
     const int lane = threadIdx.x & 63;
@@ -298,17 +300,21 @@ __global__ void __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(2
     }
     if constexpr (KG > 1) {
         __syncthreads();                                               // both rings are free
-        char *const mine = smem_all + kg * BM * BM * 4, *const other = smem_all + (1 - kg) * BM * BM * 4;      // at most both rings together
+        // every set's sums (at most all rings together), added in the order of the sets wherever they are wanted
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) *(GNK_LDS v4f *)(GNK_LDS char *)(mine + 16 * (((wave * MT + i) * 4 + j) * 64 + lane)) = acc[i][j];
+            for (int j = 0; j < 4; ++j) *(GNK_LDS v4f *)(GNK_LDS char *)(smem_all + kg * BM * BM * 4 + 16 * (((wave * MT + i) * 4 + j) * 64 + lane)) = acc[i][j];
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                acc[i][j] += *(const GNK_LDS v4f *)(const GNK_LDS char *)(other + 16 * (((wave * MT + i) * 4 + j) * 64 + lane));     // a + b = b + a
+            for (int j = 0; j < 4; ++j) {
+                v4f sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KG; ++k) sum += *(const GNK_LDS v4f *)(const GNK_LDS char *)(smem_all + k * BM * BM * 4 + 16 * (((wave * MT + i) * 4 + j) * 64 + lane));
+                acc[i][j] = sum;
+            }
     }
     float diag_sum = 0.0f;
     if constexpr (EPI == POLY) {
@@ -602,7 +608,7 @@ __global__ void __launch_bounds__(256) convert_kernel(const void *__restrict__ G
 }
 
 template <int BM, int KG, bool AK, bool BK, int EPI, bool SYM, bool PAIRS = false> int launch(const Product &p0, hipStream_t st) {
-    constexpr int LDS_TOTAL = BM == 256 ? 131072 : KG * RingShape<BM == 256 ? 128 : BM>::LDS;
+    constexpr int LDS_TOTAL = BM == 256 ? 131072 : KG * RingShape<BM == 256 ? 128 : BM, KG>::LDS;
     void (*kernel)(const Product);
     if constexpr (BM == 256) kernel = product256_kernel<AK, BK, EPI, SYM, PAIRS>;
     else kernel = product_ring_kernel<BM, KG, AK, BK, EPI, SYM, PAIRS>;
@@ -671,8 +677,8 @@ Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t ba
     const bool can256 = !(pairs && sym);
     if (!can256) c256.rounds_us = 1e30;
     const Choice c128 = tiles(128) <= cus && ks >= 4.0 ? priced(128, 2, cus, 7.0 + 0.55 * ks) : priced(128, 1, 2.0 * cus, 6.0 + 1.0 * ks);
-    const bool kg2 = tiles(64) <= cus && ks >= 4.0;
-    const Choice c64 = priced(64, kg2 ? 2 : 1, 2.0 * cus, 4.0 + (kg2 ? 0.3 : 0.5) * ks);
+    const int kg = tiles(64) <= cus ? (ks >= 24.0 ? 4 : ks >= 4.0 ? 2 : 1) : 1;
+    const Choice c64 = priced(64, kg, 2.0 * cus, 4.0 + (kg == 4 ? 0.2 : kg == 2 ? 0.3 : 0.5) * ks);
     const int forced = gnk_forced_variant_get();      // gnk_set_gemm_variant: 1, 5 and 6 force the 128, 256 and 64 tiles here as well
     if (forced == 6 || (forced != 1 && forced != 5 && c64.rounds_us <= c128.rounds_us && c64.rounds_us <= c256.rounds_us)) return c64;
     if (can256 && (forced == 5 || (forced != 1 && c256.rounds_us <= c128.rounds_us))) return c256;
@@ -682,6 +688,7 @@ Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t ba
 template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p, const Choice &c, hipStream_t st) {
     if (c.bm == 256) return launch<256, 1, AK, BK, EPI, SYM>(p, st);
     if (c.bm == 128) return c.kg == 2 ? launch<128, 2, AK, BK, EPI, SYM>(p, st) : launch<128, 1, AK, BK, EPI, SYM>(p, st);
+    if (c.kg == 4) return launch<64, 4, AK, BK, EPI, SYM>(p, st);
     if (c.kg == 2) return launch<64, 2, AK, BK, EPI, SYM>(p, st);
     return launch<64, 1, AK, BK, EPI, SYM>(p, st);
 }
@@ -690,6 +697,7 @@ template <bool AK, bool BK, int EPI, bool SYM> int run_pairs(const Product &p, c
     if constexpr (!SYM)
         if (c.bm == 256) return launch<256, 1, AK, BK, EPI, SYM, true>(p, st);
     if (c.bm == 128) return c.kg == 2 ? launch<128, 2, AK, BK, EPI, SYM, true>(p, st) : launch<128, 1, AK, BK, EPI, SYM, true>(p, st);
+    if (c.kg == 4) return launch<64, 4, AK, BK, EPI, SYM, true>(p, st);
     return c.kg == 2 ? launch<64, 2, AK, BK, EPI, SYM, true>(p, st) : launch<64, 1, AK, BK, EPI, SYM, true>(p, st);
 }
 

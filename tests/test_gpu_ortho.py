@@ -276,3 +276,31 @@ def test_workspace_is_half_for_bf16():
     out, ws = torch.empty_like(G), torch.empty(L.gnk_orthogonalize_workspace_bytes_of(d[torch.bfloat16], 1, 500, 700), dtype=torch.uint8, device=DEV)
     rc = L.gnk_orthogonalize(G.data_ptr(), d[G.dtype], out.data_ptr(), d[G.dtype], 1, 500, 700, 5, *COEFFS, 1e-7, ws.data_ptr(), ws.numel(), None)
     assert rc == -4 and b"workspace" in L.gnk_last_error()
+
+
+@pytest.mark.parametrize("m,n", [(64, 4000), (4000, 64), (130, 1600), (100, 1530)])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+def test_long_contractions(forced, m, n, dt):
+    """24 steps of 64 and more: four sets of waves."""
+    G = matrix(m, n, dt, seed=n)
+    (compare if dt == "bf16" else compare_closely)(gn_kernels.orthogonalize(G.to(DEV)), G)
+
+
+@pytest.mark.parametrize("g_dt,out_dt", [("bf16", "f32"), ("f32", "bf16"), ("f16", "bf16"), ("bf16", "f16")])
+def test_result_of_another_type(g_dt, out_dt):
+    """The C entry takes the two types apart: the result's decides how many bits the matrices are kept to."""
+    L, d = _cabi.load(), _cabi.DTYPE_CODE
+    m, n = 150, 310
+    G = matrix(m, n, g_dt, seed=2, kind="gauss").to(DEV)
+    out = torch.empty(m, n, dtype=DT[out_dt], device=DEV)
+    ws = torch.empty(L.gnk_orthogonalize_workspace_bytes_of(d[out.dtype], 1, m, n), dtype=torch.uint8, device=DEV)
+    assert L.gnk_orthogonalize(G.data_ptr(), d[G.dtype], out.data_ptr(), d[out.dtype], 1, m, n, 5, *COEFFS, 1e-7, ws.data_ptr(), ws.numel(),
+                               torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    want, tol = reference(G.cpu())
+    err = (out.double().cpu() - want).norm().item()
+    if out_dt != "bf16":
+        tol = (3e-4 + torch.finfo(out.dtype).eps / 2) * want.norm().item()
+    else:
+        tol += torch.finfo(out.dtype).eps / 2 * want.norm().item()
+    assert err <= tol
