@@ -196,3 +196,24 @@ def test_refusals(bad):
             F.grouped_mm(x.float(), wd.transpose(-2, -1), offs=offs)
         else:
             F.grouped_mm(x, wd.transpose(-2, -1), offs=offs, **({"bias": w[:, 0].to(DEV)} if bad == "bias" else {"out_dtype": torch.float32} if bad == "out_dtype" else {}))
+
+
+@pytest.mark.parametrize("sizes,pad,K,N", [([20000, 100], 3, 64, 96), ([9000], 0, 33, 21), ([4000, 0, 4200], 40, 512, 16)])
+def test_many_rows_of_small_experts(sizes, pad, K, N):
+    """The weight gradient's contraction is long and its tiles are few (cut into parts, or shared by two sets of waves): the call for both gradients, the op by op
+    form and the formula agree, and no gradient that is not asked for is made."""
+    from gn_kernels import grouped
+    from gn_kernels._lib import lib_ops
+
+    x, w, gy = make(sizes, pad, K, N, seed=4)
+    offs = offs_of(sizes)
+    xd, wd, gd = x.to(DEV), w.to(DEV).transpose(1, 2), gy.to(DEV)
+    gx, gw = lib_ops.grouped_linear_int8_backward(gd, xd, wd, offs, True, True)
+    one = grouped.linear_backward(gd, xd, wd, offs, True, True, False)
+    assert torch.equal(gx, one[0]) and torch.equal(gw, one[1])
+    only_w = lib_ops.grouped_linear_int8_backward(gd, xd, wd, offs, False, True)
+    assert only_w[0].shape == (0, K) and torch.equal(only_w[1], gw)
+    _, want_x, want_w = formula(x, w, gy, sizes)
+    eps = (2.0 ** -8 + 3 * 2.0 ** -24) * (1 + 2.0 ** -8)
+    for got, want in ((gx, want_x), (gw, want_w)):
+        assert ((got.double().cpu() - want).abs() <= eps * want.abs()).all()
