@@ -45,8 +45,9 @@ typedef enum gnk_status {
  *   1: the first one.   2: gnk_scaled_mm_ws / gnk_scaled_mm_t, the fused quantize pair, gnk_quantize_int8_noalloc, the MX and BitNet
  *      entry points added; gnk_set_debug_flags removed from the shipped library; gnk_set_gemm_variant accepts 5, 6, -2 and -3; gnk_set_tile_rescale added.
  *   3: the products grouped by expert and their quantizer (gnk_grouped_scaled_mm_rows / _depth, gnk_quantize_int8_grouped).
- *   4: gnk_orthogonalize.   5: gnk_grouped_scaled_mm_depth_split_bytes.   6: gnk_orthogonalize_workspace_bytes_of. */
-#define GNK_ABI_VERSION 6
+ *   4: gnk_orthogonalize.   5: gnk_grouped_scaled_mm_depth_split_bytes.   6: gnk_orthogonalize_workspace_bytes_of.
+ *   7: gnk_grouped_scaled_mm_rows refuses int8 sums of more than 131071 products; _depth wants _split_bytes for int8 over more than 130816 rows. */
+#define GNK_ABI_VERSION 7
 int gnk_abi_version(void);
 
 /* Message for the last non-zero status returned on this thread ("" if none). */
@@ -276,12 +277,14 @@ int gnk_quantize_int8_noalloc(const void *x, int x_dtype, int64_t R, int64_t C, 
  * gnk_grouped_scaled_mm_depth:  C[e,m,n] = cast_out( (f32(sum_{t in e} A[m,t] * B[t,n]) * row_scale[e,m]) * col_scale[e,n] ); a group without rows
  *   gives 0 * row_scale * col_scale.  A (M, T) with strides (sam, sat); B (T, N) with strides (sbt, sbn); row_scale (E, M), col_scale (E, N), or (E,).
  *   The gradient of the experts' weights.
- * Dtypes, accumulation and scales as in gnk_scaled_mm (order 0); C contiguous.  T < 2^31, E < 2^20, feature sizes up to 2^22.
+ * Dtypes, accumulation and scales as in gnk_scaled_mm (order 0); C contiguous.  T < 2^31, E < 2^20, feature sizes up to 2^22; rows form, int8: K <= 131071,
+ * beyond which a sum may not fit its 32 bits (GNK_ERR_UNSUPPORTED).  The depth form adds longer int8 sums up in 64 bits: exact for any group.
  * workspace: gnk_grouped_scaled_mm_*_workspace_bytes() bytes, 16-byte aligned.  0 when the kernels can read both operands where they lie (16-byte
  * aligned bases and pitches, the contiguous extent a multiple of 16: rows form A K-contiguous and B K- or N-contiguous, depth form A M-contiguous and
  * B N-contiguous); otherwise room for a padded copy of those that they cannot.  Overlapping calls need a workspace each.
  * The depth form takes gnk_grouped_scaled_mm_depth_split_bytes() bytes more (beyond the former rounded up to 16) if the caller has them: where few tiles share
- * long contractions it cuts those into parts and adds their sums up from there, in a fixed order; without that room it does not.
+ * long contractions it cuts those into parts and adds their sums up from there, in a fixed order; without that room it does not.  For int8 and T > 130816 it
+ * needs that room (GNK_ERR_WORKSPACE otherwise): a group of more rows than that is summed in pieces.
  */
 int64_t gnk_grouped_scaled_mm_rows_workspace_bytes(const void *A, const void *B, int64_t T, int64_t E, int64_t N, int64_t K, int64_t sat, int64_t sak,
                                                    int64_t sbe, int64_t sbk, int64_t sbn);

@@ -25,6 +25,8 @@ struct GroupedParams {
     int splits;              // depth: parts that a group's contraction is cut into (1: none); their sums go to `slab`, part by part
     void *slab;
     int64_t slab_bytes;
+    int long_rows;           // depth: groups of more rows are left to a launch of their own (0: none are)
+    int pieces;              // depth: this is that launch, over at most so many pieces of them; their sums go to `slab`, piece by piece
 };
 
 typedef int (*gnk_grouped_launcher)(bool depth, bool b_kmajor, const GroupedParams &p, hipStream_t st);
@@ -122,6 +124,12 @@ __device__ __forceinline__ int count_pieces(const int *ends, int64_t E, int64_t 
 
 // Piece number `want`: its group e (E: rows of no group; -1: there are fewer pieces), its number within the group, the group's rows, and the
 // number of pieces of 1 << sh2 rows in the groups in front of it.
+// int8: 128 * 128 * 131071 is the largest sum of products that is sure to fit an accumulator's 32 bits.  The host knows the rows of all groups together, not of
+// one: beyond LONG_ROWS of them (whole steps of every loop) a group that has more is cut into pieces of LONG_ROWS, whose sums are added in 64 bits.
+constexpr int64_t INT8_TERMS = 131071;
+constexpr int LONG_ROWS = 511 * 256;
+static_assert(LONG_ROWS <= INT8_TERMS, "a piece's sums fit 32 bits");
+
 struct Piece { int e, idx, lo, hi, first2; };
 __device__ __forceinline__ Piece find_piece(const int *ends, int64_t E, int64_t T, int lane, int sh, int want, int sh2) {
     int before = 0, before2 = 0, end = 0;
@@ -138,6 +146,25 @@ __device__ __forceinline__ Piece find_piece(const int *ends, int64_t E, int64_t 
         }
         before = __builtin_amdgcn_readlane(incl, 63);
         before2 = __builtin_amdgcn_readlane(incl2, 63);
+    }
+    return {-1, 0, 0, 0, 0};
+}
+
+__device__ __forceinline__ int long_pieces_of(int rows) { return rows > LONG_ROWS ? (int)(((unsigned)rows + (LONG_ROWS - 1u)) / (unsigned)LONG_ROWS) : 0; }
+
+// Piece number `want` of the groups of more than LONG_ROWS rows, as find_piece has it (first2: the number of the group's first piece)
+__device__ __forceinline__ Piece find_long_piece(const int *ends, int64_t E, int64_t T, int lane, int want) {
+    int before = 0, end = 0;
+    for (int64_t g0 = 0; g0 < E; g0 += 64) {
+        int l, h;
+        lane_group(ends, E, T, g0, lane, end, l, h);
+        const int n = g0 + lane < E ? long_pieces_of(h - l) : 0, incl = wave_prefix(n) + before;
+        const unsigned long long hit = __ballot(incl > want);
+        if (hit) {
+            const int src = __builtin_ctzll(hit), first = __builtin_amdgcn_readlane(incl - n, src);
+            return {(int)g0 + src, want - first, __builtin_amdgcn_readlane(l, src), __builtin_amdgcn_readlane(h, src), first};
+        }
+        before = __builtin_amdgcn_readlane(incl, 63);
     }
     return {-1, 0, 0, 0, 0};
 }
@@ -191,6 +218,15 @@ template <int STEP> __device__ __forceinline__ Tile depth_tile(const GroupedPara
     tm = first + r % gsz;
     tn = r / gsz;
     t.tm = tm; t.tn = tn;
+    if (p.pieces) {                          // (one part each: t.e counted the pieces)
+        t.part = t.e;
+        const Piece pc = find_long_piece(p.ends, p.E, p.T, lane, t.part);
+        t.e = pc.e;
+        t.work = pc.e >= 0;
+        t.lo = pc.lo + (int64_t)pc.idx * LONG_ROWS;
+        t.hi = t.lo + LONG_ROWS < pc.hi ? t.lo + LONG_ROWS : pc.hi;
+        return t;
+    }
     int lo, hi;
     one_group(p.ends, p.E, p.T, t.e, lane, lo, hi);
     t.lo = lo; t.hi = hi;
@@ -199,7 +235,7 @@ template <int STEP> __device__ __forceinline__ Tile depth_tile(const GroupedPara
         t.lo = t.lo + t.part * each < t.hi ? t.lo + t.part * each : t.hi;
         t.hi = t.lo + each < t.hi ? t.lo + each : t.hi;
     }
-    t.work = true;
+    t.work = !p.long_rows || hi - lo <= p.long_rows;
     return t;
 }
 
@@ -212,7 +248,7 @@ __device__ __forceinline__ GemmParams tile_params(const GroupedParams &p, const 
         g.K = rows;
         g.A += t.lo * g.lda;
         g.B += t.lo * g.ldb;
-        g.C = (char *)g.C + ((int64_t)t.part * p.E + t.e) * g.M * g.N * p.out_bytes;
+        g.C = (char *)g.C + (p.pieces ? (int64_t)t.part : (int64_t)t.part * p.E + t.e) * g.M * g.N * p.out_bytes;
         g.s0 = (const char *)g.s0 + (int64_t)t.e * g.M * p.scale_bytes;
         ext_a = p.ext_a;
     } else {
@@ -538,55 +574,96 @@ template <class Kernel> static int reserve_lds(Kernel k, int bytes, std::atomic<
 // lands in a slab of its own and this kernel adds them in order (so that equal calls give equal bits), scales and rounds once.  HBM-bound; V = 4 adjacent
 // columns per thread where N allows.  Whole calls, one part -> the parts chosen, int8: 1024 x 1024 over 32768 rows 182 -> 49 us (16 parts, 1.4 POP/s; the slabs,
 // 67 MB written and read, are half of it), 4096 x 1024 252 -> 115 (4), 64 x 64 127 -> 16 (32), four groups of 512 x 512 51 -> 28 (8).
-template <int OP, int V>
-__global__ void __launch_bounds__(256) join_kernel(const void *__restrict__ slab, char *__restrict__ C, const char *__restrict__ s0, const char *__restrict__ s1, int64_t E,
-                                                   int64_t M, int64_t N, int splits, int scale_dtype, int col_scalar, int out_dtype) {
+// The parts of an int8 sum fit 32 bits; the sum of all of them does for up to INT8_TERMS rows, WIDE otherwise (64 bits: 1024 x 1024 in 16 parts 51 -> 52 us).
+template <int OP, bool WIDE> struct JoinT { typedef float type; };
+template <> struct JoinT<OP_I8, false> { typedef int type; };
+template <> struct JoinT<OP_I8, true> { typedef long long type; };
+
+// `count` sums `stride` bytes apart, V adjacent columns each, added in order, scaled, rounded and stored at element `out_at` of C
+template <int OP, int V, bool WIDE>
+__device__ __forceinline__ void join_columns(const char *src, int64_t stride, int count, float rs, const float (&cs)[V], char *__restrict__ C, int64_t out_at, int out_dtype) {
     typedef typename AccT<OP>::type acc_t;                   // v4i or v4f
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, total = E * M * N;
-    if (i >= total) return;
-    const int64_t row = i / N, n = i - row * N, e = row / M;
-    const float rs = gnk_load_scalar_rt(s0, scale_dtype, row);
-    float cs[V];
+    typename JoinT<OP, WIDE>::type acc[V];
 #pragma unroll
-    for (int r = 0; r < V; ++r) cs[r] = gnk_load_scalar_rt(s1, scale_dtype, col_scalar ? e : e * N + n + r);
-    const char *src = (const char *)slab + 4 * i;
-    acc_t acc = {0, 0, 0, 0};
-    for (int k0 = 0; k0 < splits; k0 += 4) {                 // four loads in flight
-        acc_t part[4];
+    for (int r = 0; r < V; ++r) acc[r] = 0;
+    constexpr int FLIGHT = 8;                                // loads in flight (four: 20 instead of 16 us for 64 x 64 in 32 parts)
+    for (int k0 = 0; k0 < count; k0 += FLIGHT) {
+        acc_t part[FLIGHT];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            part[k] = (acc_t){0, 0, 0, 0};
-            if (k0 + k < splits) {
-                if constexpr (V == 4) part[k] = *(const acc_t *)(src + (k0 + k) * total * 4);
-                else __builtin_memcpy(&part[k], src + (k0 + k) * total * 4, 4);
-            }
+        for (int k = 0; k < FLIGHT; ++k) {                   // past the end the last one again, for nothing
+            const char *at = src + (k0 + k < count ? k0 + k : count - 1) * stride;
+            if constexpr (V == 4) part[k] = *(const acc_t *)at;
+            else __builtin_memcpy(&part[k], at, 4);
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) acc += part[k];
+        for (int k = 0; k < FLIGHT; ++k)
+            if (k0 + k < count)
+#pragma unroll
+                for (int r = 0; r < V; ++r) acc[r] += part[k][r];
     }
-    float v[4];
+    float v[V];
 #pragma unroll
     for (int r = 0; r < V; ++r) v[r] = __fmul_rn(__fmul_rn((float)acc[r], rs), cs[r]);
     if constexpr (V == 4) {
-        if (out_dtype == GNK_F32) *(v4f *)(C + 4 * i) = (v4f){v[0], v[1], v[2], v[3]};
-        else if (out_dtype == GNK_BF16) *(v2i *)(C + 2 * i) = (v2i){(int)gnk_pack2_bf16(v[0], v[1]), (int)gnk_pack2_bf16(v[2], v[3])};
-        else *(v2i *)(C + 2 * i) = (v2i){(int)gnk_pack2_f16(v[0], v[1]), (int)gnk_pack2_f16(v[2], v[3])};
+        if (out_dtype == GNK_F32) *(v4f *)(C + 4 * out_at) = (v4f){v[0], v[1], v[2], v[3]};
+        else if (out_dtype == GNK_BF16) *(v2i *)(C + 2 * out_at) = (v2i){(int)gnk_pack2_bf16(v[0], v[1]), (int)gnk_pack2_bf16(v[2], v[3])};
+        else *(v2i *)(C + 2 * out_at) = (v2i){(int)gnk_pack2_f16(v[0], v[1]), (int)gnk_pack2_f16(v[2], v[3])};
     } else {
-        gnk_store_scalar_rt(C, out_dtype, i, v[0]);
+        gnk_store_scalar_rt(C, out_dtype, out_at, v[0]);
     }
 }
 
+template <int OP, int V, bool WIDE>
+__global__ void __launch_bounds__(256) join_kernel(const void *__restrict__ slab, char *__restrict__ C, const char *__restrict__ s0, const char *__restrict__ s1, int64_t E,
+                                                   int64_t M, int64_t N, int splits, int scale_dtype, int col_scalar, int out_dtype) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, total = E * M * N;
+    if (i >= total) return;
+    const int64_t row = i / N, n = i - row * N, e = row / M;
+    float cs[V];
+#pragma unroll
+    for (int r = 0; r < V; ++r) cs[r] = gnk_load_scalar_rt(s1, scale_dtype, col_scalar ? e : e * N + n + r);
+    join_columns<OP, V, WIDE>((const char *)slab + 4 * i, total * 4, splits, gnk_load_scalar_rt(s0, scale_dtype, row), cs, C, i, out_dtype);
+}
+
+// The pieces of the groups of more than LONG_ROWS rows: the workgroups of a group's first piece (blockIdx.y) add them all.  5632 x 2048, groups of 139000 and 1000
+// rows: 14 us of 1410.
+template <int V>
+__global__ void __launch_bounds__(256) join_long_kernel(const GroupedParams p) {
+    const Piece pc = find_long_piece(p.ends, p.E, p.T, threadIdx.x & 63, (int)blockIdx.y);
+    if (pc.e < 0 || pc.idx != 0) return;
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V, each = p.g.M * p.g.N;
+    if (i >= each) return;
+    const int64_t m = i / p.g.N, n = i - m * p.g.N, e = pc.e;
+    float cs[V];
+#pragma unroll
+    for (int r = 0; r < V; ++r) cs[r] = gnk_load_scalar_rt(p.g.s1, p.g.scale_dtype, p.g.col_scalar ? e : e * p.g.N + n + r);
+    join_columns<OP_I8, V, true>((const char *)p.slab + ((int64_t)blockIdx.y * each + i) * 4, each * 4, long_pieces_of(pc.hi - pc.lo),
+                        gnk_load_scalar_rt(p.g.s0, p.g.scale_dtype, e * p.g.M + m), cs, (char *)p.g.C, e * each + i, p.g.out_dtype);
+}
+
+static inline bool join_quads(const GroupedParams &p) { return p.g.N % 4 == 0 && ((uintptr_t)p.g.C & 15) == 0; }
+
 template <int OP> int join_parts(const GroupedParams &p, hipStream_t st) {
     const int64_t total = p.E * p.g.M * p.g.N;
-    const bool quads = p.g.N % 4 == 0 && ((uintptr_t)p.g.C & 15) == 0;
+    const bool quads = join_quads(p);
     const int64_t blocks = (total / (quads ? 4 : 1) + 255) / 256;
     const auto args = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, p.slab, (char *)p.g.C, (const char *)p.g.s0, (const char *)p.g.s1, p.E, p.g.M, p.g.N, p.splits,
                            p.g.scale_dtype, p.g.col_scalar, p.g.out_dtype);
     };
-    if (quads) args(join_kernel<OP, 4>);
-    else args(join_kernel<OP, 1>);
+    if (OP == OP_I8 && p.T > INT8_TERMS) quads ? args(join_kernel<OP, 4, true>) : args(join_kernel<OP, 1, true>);
+    else quads ? args(join_kernel<OP, 4, false>) : args(join_kernel<OP, 1, false>);
     return gnk_check_launch("grouped mm: joining the parts");
+}
+
+static inline int join_long(const GroupedParams &p, hipStream_t st) {
+    const bool quads = join_quads(p);
+    const int64_t blocks = (p.g.M * p.g.N / (quads ? 4 : 1) + 255) / 256;
+    if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "grouped mm: too many outputs");
+    const dim3 grid((unsigned)blocks, (unsigned)p.pieces);
+    if (quads) hipLaunchKernelGGL((join_long_kernel<4>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((join_long_kernel<1>), grid, dim3(256), 0, st, p);
+    return gnk_check_launch("grouped mm: joining the pieces of long groups");
 }
 
 // Tile sizes of a launch over the whole grid; KERNEL with its LDS.
@@ -594,7 +671,7 @@ template <class Kernel> int launch_tiles(Kernel kernel, std::atomic<bool> (&done
     GroupedParams p = p0;
     p.g.grid_n = (int)((p.g.N + bn - 1) / bn);
     p.g.grid_m = depth ? (int)((p.g.M + bm - 1) / bm) : 0;
-    const int64_t blocks = (depth ? p.E * p.g.grid_m * p.splits : max_row_tiles(p.T, p.E, bm)) * p.g.grid_n;
+    const int64_t blocks = (depth ? (p.pieces ? p.pieces : p.E) * p.g.grid_m * p.splits : max_row_tiles(p.T, p.E, bm)) * p.g.grid_n;
     if (blocks >= (1LL << 31)) return gnk_fail(GNK_ERR_UNSUPPORTED, "grouped mm: too many tiles");
     const int rc = reserve_lds(kernel, lds, done);
     if (rc) return rc;
@@ -669,6 +746,9 @@ static inline Plan choose_variant(int64_t T, int64_t groups_n, int64_t M, int64_
 
 static inline int64_t split_bytes(int splits, int64_t E, int64_t M, int64_t N) { return splits > 1 ? splits * E * M * N * 4 : 0; }
 
+// pieces that groups of more than LONG_ROWS rows can come to, T rows in all: the sum of ceil(rows / LONG_ROWS) over at most T / (LONG_ROWS + 1) groups
+static inline int64_t most_long_pieces(int64_t T) { return T / LONG_ROWS + T / (LONG_ROWS + 1); }
+
 template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const GroupedParams &p0, hipStream_t st) {
     const bool can_w4 = depth ? p0.T * (p0.g.lda > p0.g.ldb ? p0.g.lda : p0.g.ldb) < (1LL << 32) : p0.g.K >= 256 && p0.g.K % 256 == 0;
     const bool can_192 = OP == OP_I8 && !depth && can_w4;
@@ -681,14 +761,29 @@ template <int OP, int FA, int FB> int launch(bool depth, bool b_kmajor, const Gr
     GroupedParams p = p0;
     p.splits = plan.splits;
     while (p.splits > 1 && split_bytes(p.splits, p.E, p.g.M, p.g.N) > p.slab_bytes) p.splits /= 2;       // no room for the parts: fewer of them
+    const auto plain_sums = [&](GroupedParams q) {
+        q.g.C = q.slab;
+        q.g.out_dtype = OP == OP_I8 ? GNK_I32 : GNK_F32;
+        q.out_bytes = 4;
+        return variant == GNK_VARIANT_256_W4 ? launch_w4<PP2Cfg<false, false, OP, FA, FB, EPI_PLAIN>, true>(q, st)
+                                             : launch_two_buffer<GemmCfg<128, 128, 2, 2, false, false, OP, FA, FB, EPI_PLAIN>, true>(q, st);
+    };
+    if constexpr (OP == OP_I8) {
+        // parts of at most LONG_ROWS rows, whoever has them, or groups of more in pieces
+        if (depth && p.T > LONG_ROWS && p.splits * (int64_t)LONG_ROWS < p.T) {
+            p.splits = 1;
+            p.long_rows = LONG_ROWS;
+            GroupedParams q = p;
+            q.pieces = (int)most_long_pieces(p.T);
+            if (p.slab_bytes < q.pieces * p.g.M * p.g.N * 4)
+                return gnk_fail(GNK_ERR_WORKSPACE, "grouped_scaled_mm: int8 sums over %lld rows need the workspace of gnk_grouped_scaled_mm_depth_split_bytes", (long long)p.T);
+            int rc = plain_sums(q);
+            if (!rc) rc = join_long(q, st);
+            if (rc) return rc;
+        }
+    }
     if (p.splits > 1) {
-        p.g.C = p.slab;
-        p.g.out_dtype = OP == OP_I8 ? GNK_I32 : GNK_F32;
-        p.out_bytes = 4;
-        const int rc = variant == GNK_VARIANT_256_W4 ? launch_w4<PP2Cfg<false, false, OP, FA, FB, EPI_PLAIN>, true>(p, st)
-                                                     : launch_two_buffer<GemmCfg<128, 128, 2, 2, false, false, OP, FA, FB, EPI_PLAIN>, true>(p, st);
-        p.g.C = p0.g.C;
-        p.g.out_dtype = p0.g.out_dtype;
+        const int rc = plain_sums(p);
         return rc ? rc : join_parts<OP>(p, st);
     }
     if constexpr (OP == OP_I8) {

@@ -130,6 +130,8 @@ extern "C" int gnk_grouped_scaled_mm_rows(const void *A, int a_dtype, const void
     const char *name = "grouped_scaled_mm";
     int rc = check_call(name, a_dtype, b_dtype, out_dtype, scale_dtype, T, E, N, K);
     if (rc) return rc;
+    if (a_dtype == GNK_I8 && K > INT8_TERMS)
+        return gnk_fail(GNK_ERR_UNSUPPORTED, "%s: int8 sums over %lld products may not fit 32 bits (at most %lld)", name, (long long)K, (long long)INT8_TERMS);
     if (T == 0 || N == 0) return GNK_OK;
     if (!C || !row_scale || (E > 0 && (!ends || !col_scale || (K > 0 && (!A || !B))))) return gnk_fail(GNK_ERR_BAD_ARG, "%s: null pointer", name);
     rc = gnk_init();
@@ -166,7 +168,9 @@ extern "C" int64_t gnk_grouped_scaled_mm_depth_split_bytes(int64_t T, int64_t E,
     if (T <= 0 || E <= 0 || M <= 0 || N <= 0 || E >= (1LL << 20) || M > MAX_PITCH || N > MAX_PITCH) return 0;
     const int64_t pitch = up16(M > N ? M : N);
     const int f = gnk_forced_variant_get(), forced = f == GNK_VARIANT_128 || f == GNK_VARIANT_64X128 || (f == GNK_VARIANT_256_W4 && T * pitch < (1LL << 32)) ? f : -1;
-    return split_bytes(choose_variant(T, E, M, N, 0, true, false, T * pitch < (1LL << 32), false, forced).splits, E, M, N);
+    const int64_t parts = split_bytes(choose_variant(T, E, M, N, 0, true, false, T * pitch < (1LL << 32), false, forced).splits, E, M, N);
+    const int64_t long_groups = T > LONG_ROWS ? most_long_pieces(T) * M * N * 4 : 0;
+    return parts > long_groups ? parts : long_groups;
 }
 
 extern "C" int gnk_grouped_scaled_mm_depth(const void *A, int a_dtype, const void *B, int b_dtype, void *C, int out_dtype, const void *row_scale,

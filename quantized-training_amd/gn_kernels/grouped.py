@@ -37,6 +37,7 @@ def grouped_scaled_mm(A: Tensor, B: Tensor, scale_A: Tensor, scale_B: Tensor, of
     16 and whose rows are 16-byte aligned are read where they lie: A along K and B along K or N (rows form), A along M and B along N (second
     form).  Others are copied first.  scales are contiguous, the result has their dtype.  offs: int32 on the same device, not decreasing,
     at most T (not checked, as that would wait for the device: a value below an earlier one counts as that one, one beyond T as T).
+    int8 sums are exact: over any number of rows in the second form; the first one refuses K > 131071, where they may not fit 32 bits.
     """
     dt, E = A.dtype, offs.shape[0]
     assert (dt is torch.int8 and B.dtype is torch.int8) or (dt in _FP8 and B.dtype in _FP8)

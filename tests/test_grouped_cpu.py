@@ -222,3 +222,13 @@ def test_grouped_mm_refusals(kwargs, error):
     with pytest.raises(NotImplementedError):
         part = MixedPrecisionLinearWeight(torch.zeros(3, 12, 8, dtype=torch.bfloat16), MixedPrecisionConfig(grad_input=False))
         F.grouped_mm(torch.zeros(4, 8, dtype=torch.bfloat16), part.transpose(-2, -1), offs=torch.tensor([1, 2, 4], dtype=torch.int32))
+
+
+def test_int8_sums_that_may_not_fit_32_bits():
+    L = _cabi.load()
+    rows = lambda dt, K: L.gnk_grouped_scaled_mm_rows(None, dt, None, dt, None, _cabi.BF16, None, None, _cabi.BF16, 0, None, 4, 2, 16, K, K, 1, 16 * K, 1, K, None, 0, None)  # noqa: E731
+    assert rows(_cabi.I8, 131072) == -2 and b"32 bits" in L.gnk_last_error()
+    assert rows(_cabi.I8, 131071) == -1 and rows(_cabi.E4M3, 131072) == -1         # null pointers: the size is taken
+    # room for the pieces of a group of more than 130816 rows, whatever else a call asks for
+    assert L.gnk_grouped_scaled_mm_depth_split_bytes(130817, 64, 2048, 2048) >= 2 * 2048 * 2048 * 4
+    assert L.gnk_grouped_scaled_mm_depth_split_bytes(3 * 130817, 64, 2048, 2048) >= 6 * 2048 * 2048 * 4
