@@ -19,7 +19,8 @@ def _plain(t: Tensor) -> Tensor:
 class Muon(torch.optim.Optimizer):
     """m <- momentum m + g;  u = orthogonalize(g + momentum m) (nesterov) or orthogonalize(m);  p <- (1 - lr weight_decay) p - lr max(1, rows / cols)^0.5 u.
 
-    The momentum m is held in fp32 whatever the weights' type (a bf16 sum would lose gradients below 2^-8 of it); u is rounded once, to the gradient's type.
+    The momentum m is held in fp32 whatever the weights' type (a bf16 sum would lose gradients below 2^-8 of it).  bf16 gradients: what is orthogonalised is
+    rounded once to bf16; fp16: it stays fp32, as the sum may be 1 / (1 - momentum) times the gradients and leave fp16's range.
     Weights of one shape and type share a call of `orthogonalize`: equal layers fill the chip where one matrix does not."""
 
     def __init__(self, params, lr: float = 0.02, *, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
@@ -59,7 +60,7 @@ class Muon(torch.optim.Optimizer):
                 if "momentum" not in state:
                     state["momentum"] = torch.zeros_like(g, dtype=torch.float32, memory_format=torch.contiguous_format)
                 m = state["momentum"].mul_(group["momentum"]).add_(g)
-                u = (torch.add(g, m, alpha=group["momentum"]) if group["nesterov"] else m).to(g.dtype)
+                u = (torch.add(g, m, alpha=group["momentum"]) if group["nesterov"] else m).to(torch.float32 if g.dtype is torch.float16 else g.dtype)
                 alike.setdefault((tuple(p.shape[-2:]), u.dtype, u.device), []).append((p, u))
             for (shape, _, _), pairs in alike.items():
                 # one stack of all matrices of this shape; a single one goes as it is

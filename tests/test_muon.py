@@ -149,3 +149,21 @@ def test_update_on_the_device():
         want = b.double() - 0.5 * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5 * u.double()
         # the stack and the single call round alike; the sum is rounded to bf16 once (the scaled update once more where the factor is no power of two)
         assert ((p.detach().double() - want).abs() <= 2.0 ** -8 * (want.abs() + u.double().abs())).all()
+
+
+def test_fp16_gradients_whose_momentum_leaves_fp16(cpu_op):
+    """Gradients near fp16's largest value (as a loss scale leaves them): the momentum is 1.9 of them after two steps, more than fp16 holds; the update is the
+    formula's, in fp32, rounded once to the weight."""
+    g = torch.Generator().manual_seed(3)
+    p = nn.Parameter(torch.zeros(6, 10, dtype=torch.float16))
+    opt = Muon([p], lr=0.5)
+    want, mom = torch.zeros(6, 10, dtype=torch.float64), torch.zeros(6, 10, dtype=torch.float64)
+    gr = (torch.randn(6, 10, generator=g).clamp(-1, 1) * 6e4).half()
+    for _ in range(2):
+        p.grad = gr.clone()
+        opt.step()
+        mom = 0.95 * mom + gr.double()
+        want = want - 0.5 * newton_schulz(gr.double() + 0.95 * mom, 5, 3.4445, -4.7750, 2.0315, 1e-7)
+    assert (gr.double() + 0.95 * mom).abs().max() > 65504
+    # two roundings to fp16 (2^-11 of values up to 1.3 each) and fp32's in the momentum, stretched by 3.4^5
+    assert torch.isfinite(p).all() and ((p.detach().double() - want).abs() <= 2 * 1.3 * 2.0 ** -11 + 2e-4).all()
