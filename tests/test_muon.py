@@ -167,3 +167,56 @@ def test_fp16_gradients_whose_momentum_leaves_fp16(cpu_op):
     assert (gr.double() + 0.95 * mom).abs().max() > 65504
     # two roundings to fp16 (2^-11 of values up to 1.3 each) and fp32's in the momentum, stretched by 3.4^5
     assert torch.isfinite(p).all() and ((p.detach().double() - want).abs() <= 2 * 1.3 * 2.0 ** -11 + 2e-4).all()
+
+
+def test_calls_are_bounded_whatever_the_number_of_layers(cpu_op, monkeypatch):
+    """Many equal layers and a stack that is larger than a call: the update of one call per matrix, from calls of at most the bound (not one for everything)."""
+    import muon
+
+    per = 4
+    monkeypatch.setattr(muon, "_CALL_WORK", per * 6.0 * 6 * 10)
+    seen, op = [], muon.orthogonalize
+    monkeypatch.setattr(muon, "orthogonalize", lambda G, **kw: seen.append(G.shape[0]) or op(G, **kw))
+    g = torch.Generator().manual_seed(4)
+    shapes = [(6, 10)] * 7 + [(11, 6, 10), (2, 6, 10), (0, 6, 10)]
+    grads = [torch.randn(s, generator=g) for s in shapes]
+    ps, alone = ([nn.Parameter(torch.zeros(s)) for s in shapes] for _ in range(2))
+    for group in (ps, alone):
+        for p, gr in zip(group, grads):
+            p.grad = gr.clone()
+    Muon(ps, lr=0.1, weight_decay=0.1).step()
+    assert sum(seen) == 20 and max(seen) <= per and len(seen) == 5
+    for p in alone:
+        Muon([p], lr=0.1, weight_decay=0.1).step()
+    # the host's products may add in another order for another batch: rounding of values around 1 in 64 bits, then to fp32 (2^-24), and of the update's sum
+    for p, q in zip(ps, alone):
+        torch.testing.assert_close(p.detach(), q.detach(), rtol=2.0 ** -22, atol=2.0 ** -24)
+
+
+def test_matrices_per_call():
+    from muon import matrices_per_call
+
+    assert matrices_per_call(2048, 5632, 44) == 15 and matrices_per_call(5632, 2048, 16) == 16 and matrices_per_call(2048, 5632, 1) == 1
+    assert matrices_per_call(1, 1, 200000) == 50000 and matrices_per_call(64, 1 << 20, 100) == 4 and matrices_per_call(20000, 50000, 3) == 1
+    assert matrices_per_call(8, 8, 0) == 1
+
+
+@pytest.mark.gpu
+def test_bounded_calls_on_the_device(monkeypatch):
+    """The same in bf16 on the device, where another batch may take other tiles: both updates are within the operator's error of the definition, 2e-3 of the norm
+    each, and the result's and the weight's rounding, 2^-8 each."""
+    import muon
+
+    g = torch.Generator().manual_seed(5)
+    shapes = [(64, 96)] * 5 + [(3, 64, 96)]
+    grads = [torch.randn(s, generator=g).bfloat16().cuda() for s in shapes]
+    results = []
+    for work in (muon._CALL_WORK, 3.0 * 64 * 64 * 96):
+        monkeypatch.setattr(muon, "_CALL_WORK", work)
+        ps = [nn.Parameter(torch.zeros(s, dtype=torch.bfloat16, device="cuda")) for s in shapes]
+        for p, gr in zip(ps, grads):
+            p.grad = gr.clone()
+        Muon(ps, lr=1.0).step()
+        results.append([p.detach().double() for p in ps])
+    for a, b in zip(*results):
+        assert (a - b).norm() <= 2 * (2e-3 + 2 * 2.0 ** -8) * b.norm() and b.norm() > 0
