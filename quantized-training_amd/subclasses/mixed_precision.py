@@ -58,7 +58,9 @@ _REWRAP_OPS = frozenset({
     aten.clone.default,
 })
 
-_VIEW_OPS = frozenset({aten.detach.default, aten.transpose.int})
+# a stack of experts' weights (three dims) seen in another order is the stack still
+_REORDER_OPS = frozenset({aten.transpose.int, aten.permute.default})
+_VIEW_OPS = _REORDER_OPS | {aten.detach.default}
 
 
 class MixedPrecisionLinearWeight(Tensor):
@@ -120,7 +122,7 @@ class MixedPrecisionLinearWeight(Tensor):
 
     @classmethod
     def __torch_dispatch__(cls, func, types, args, kwargs):
-        # the two ops that every call of F.grouped_mm makes on its weight, without the tree walk (15 us each)
+        # the ops that every call of F.grouped_mm makes on its weight, without the tree walk (15 us each)
         if func in _VIEW_OPS and not torch.compiler.is_compiling() and isinstance(args[0], cls) and args[0].ndim == 3 and not kwargs:
             return cls._wrap(func(args[0]._data, *args[1:]), args[0].config)
         seen: list[MixedPrecisionConfig] = []
@@ -135,7 +137,7 @@ class MixedPrecisionLinearWeight(Tensor):
         out = func(*pytree.tree_map_only(cls, unwrap, args), **pytree.tree_map_only(cls, unwrap, kwargs or {}))
         if func is aten.copy_.default:
             return args[0]                       # in-place: hand back the original wrapper
-        if func in _REWRAP_OPS or (func is aten.transpose.int and args[0].ndim == 3):     # a stack of experts' weights, seen as (E, K, N)
+        if func in _REWRAP_OPS or (func in _REORDER_OPS and args[0].ndim == 3):
             return pytree.tree_map_only(Tensor, lambda t: cls(t, seen[0]), out)
         return out
 

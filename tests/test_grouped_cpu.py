@@ -232,3 +232,25 @@ def test_int8_sums_that_may_not_fit_32_bits():
     # room for the pieces of a group of more than 130816 rows, whatever else a call asks for
     assert L.gnk_grouped_scaled_mm_depth_split_bytes(130817, 64, 2048, 2048) >= 2 * 2048 * 2048 * 4
     assert L.gnk_grouped_scaled_mm_depth_split_bytes(3 * 130817, 64, 2048, 2048) >= 6 * 2048 * 2048 * 4
+
+
+@pytest.mark.parametrize("compiled", [False, True])
+@pytest.mark.parametrize("turn", [lambda w: w.permute(0, 2, 1), lambda w: w.movedim(1, 2), lambda w: w.permute(0, -1, -2), lambda w: w.swapaxes(1, 2), lambda w: w.mT,
+                                  lambda w: torch.permute(w, (0, 2, 1))], ids=["permute", "movedim", "negative", "swapaxes", "mT", "function"])
+def test_other_ways_to_transpose_a_stack_reach_the_operator(cpu_ops, turn, compiled):
+    """A permuted stack is the mixed-precision weight still: F.grouped_mm on it is the operator's (which is registered for host tensors here; plain grouped_mm in
+    float64 does not exist), forward and backward."""
+    g = torch.Generator().manual_seed(6)
+    x, w, gy = (torch.randn(s, generator=g, dtype=torch.float64) for s in ((5, 8), (2, 12, 8), (5, 12)))
+    offs = torch.tensor([2, 5], dtype=torch.int32)
+    wp = nn.Parameter(MixedPrecisionLinearWeight(w, MixedPrecisionConfig()))
+    assert isinstance(turn(wp), MixedPrecisionLinearWeight) and turn(wp).shape == (2, 8, 12) and torch.equal(turn(wp)._data, w.mT)
+
+    def call(x, wp, offs):
+        return F.grouped_mm(x, turn(wp), offs=offs)
+
+    y = (torch.compile(call, backend="aot_eager") if compiled else call)(x, wp, offs)
+    y.backward(gy)
+    gw = getattr(wp.grad, "_data", wp.grad)
+    torch.testing.assert_close(y.detach(), torch.cat([x[:2] @ w[0].T, x[2:] @ w[1].T]), rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(gw, torch.stack([gy[:2].T @ x[:2], gy[2:].T @ x[2:]]), rtol=1e-12, atol=1e-12)
