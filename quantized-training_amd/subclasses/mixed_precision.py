@@ -376,7 +376,7 @@ class _Int8MixedPrecisionGroupedMM(torch.autograd.Function):
         return gx if need_x else None, gw.transpose(1, 2) if need_w else None, None      # gw is stored (E, N, K), as the weight is
 
 
-def _grouped_mm(mat_a: Tensor, mat_b: Tensor, *, offs: Tensor | None = None, bias: Tensor | None = None, out_dtype: torch.dtype | None = None) -> Tensor:
+def _grouped_mm(mat_a: Tensor, mat_b: Tensor, offs: Tensor | None = None, bias: Tensor | None = None, out_dtype: torch.dtype | None = None) -> Tensor:
     """`torch.nn.functional.grouped_mm(x (T, K), weight (E, K, N), offs=...)` whose three products run in INT8."""
     if not isinstance(mat_b, MixedPrecisionLinearWeight) or isinstance(mat_a, MixedPrecisionLinearWeight):
         raise NotImplementedError("grouped_mm: the mixed-precision weight is the second operand")

@@ -254,3 +254,15 @@ def test_other_ways_to_transpose_a_stack_reach_the_operator(cpu_ops, turn, compi
     gw = getattr(wp.grad, "_data", wp.grad)
     torch.testing.assert_close(y.detach(), torch.cat([x[:2] @ w[0].T, x[2:] @ w[1].T]), rtol=1e-12, atol=1e-12)
     torch.testing.assert_close(gw, torch.stack([gy[:2].T @ x[:2], gy[2:].T @ x[2:]]), rtol=1e-12, atol=1e-12)
+
+
+def test_ends_by_position(cpu_ops):
+    """torch._grouped_mm takes the ends as its third positional argument."""
+    g = torch.Generator().manual_seed(7)
+    x, w = torch.randn(5, 8, generator=g, dtype=torch.float64), torch.randn(2, 12, 8, generator=g, dtype=torch.float64)
+    wp, offs = MixedPrecisionLinearWeight(w, MixedPrecisionConfig()), torch.tensor([2, 5], dtype=torch.int32)
+    y = torch._grouped_mm(x, wp.mT, offs)
+    torch.testing.assert_close(y, torch.cat([x[:2] @ w[0].T, x[2:] @ w[1].T]), rtol=1e-12, atol=1e-12)
+    for bad in (lambda: torch._grouped_mm(x, wp.mT, offs, torch.zeros(2, 12)), lambda: torch._grouped_mm(x, wp.mT, None), lambda: torch._grouped_mm(x, wp.mT, offs, None, torch.float32)):
+        with pytest.raises(NotImplementedError):
+            bad()
