@@ -392,13 +392,21 @@ def _grouped_mm(mat_a: Tensor, mat_b: Tensor, offs: Tensor | None = None, bias: 
 
 def convert_mixed_precision_experts(module: nn.Module, *, config: MixedPrecisionConfig = MixedPrecisionConfig()):
     """Wrap every stack of experts' weights under `module` -- a floating 3-D nn.Parameter (E, N, K) outside convolutions -- in a
-    MixedPrecisionLinearWeight (in place).  The module has to multiply with `F.grouped_mm(x, weight.transpose(-2, -1), offs=offs)`."""
+    MixedPrecisionLinearWeight (in place).  The module has to multiply with `F.grouped_mm(x, weight.transpose(-2, -1), offs=offs)`.
+
+    A parameter that several modules share, or one module under several names, stays one."""
+    places: dict[int, list] = {}
     for m in module.modules():
         if isinstance(m, nn.modules.conv._ConvNd):
             continue
-        for name, p in list(m.named_parameters(recurse=False)):
+        for name, p in m.named_parameters(recurse=False, remove_duplicate=False):
             if p.ndim == 3 and p.is_floating_point() and not isinstance(p, MixedPrecisionLinearWeight):
-                setattr(m, name, nn.Parameter(MixedPrecisionLinearWeight(p.detach(), config=config), requires_grad=p.requires_grad))
+                places.setdefault(id(p), []).append((m, name, p))
+    for found in places.values():
+        p = found[0][2]
+        new = nn.Parameter(MixedPrecisionLinearWeight(p.detach(), config=config), requires_grad=p.requires_grad)
+        for m, name, _ in found:
+            setattr(m, name, new)
     return module
 
 

@@ -266,3 +266,20 @@ def test_ends_by_position(cpu_ops):
     for bad in (lambda: torch._grouped_mm(x, wp.mT, offs, torch.zeros(2, 12)), lambda: torch._grouped_mm(x, wp.mT, None), lambda: torch._grouped_mm(x, wp.mT, offs, None, torch.float32)):
         with pytest.raises(NotImplementedError):
             bad()
+
+
+class Tied(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.first, self.second = Experts(torch.float32), Experts(torch.float32)
+        self.second.up = self.first.up
+        self.first.also = self.first.down
+
+
+def test_shared_stacks_stay_shared():
+    m = convert_mixed_precision_experts(Tied())
+    assert isinstance(m.first.up, MixedPrecisionLinearWeight) and m.first.up is m.second.up and m.first.also is m.first.down
+    assert m.second.down is not m.first.down and isinstance(m.second.down, MixedPrecisionLinearWeight)
+    assert sum(isinstance(p, MixedPrecisionLinearWeight) for p in m.parameters()) == 3
+    again = convert_mixed_precision_experts(m)
+    assert again.first.up is m.second.up and not isinstance(m.first.up._data, MixedPrecisionLinearWeight)
