@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import threading
 import weakref
-from typing import NamedTuple
+from typing import Callable, NamedTuple
 
 import torch
 import torch.nn.functional as F
@@ -390,23 +390,25 @@ def _grouped_mm(mat_a: Tensor, mat_b: Tensor, offs: Tensor | None = None, bias: 
     return _Int8MixedPrecisionGroupedMM.apply(mat_a, mat_b, offs)
 
 
-def convert_mixed_precision_experts(module: nn.Module, *, config: MixedPrecisionConfig = MixedPrecisionConfig()):
+def convert_mixed_precision_experts(module: nn.Module, *, config: MixedPrecisionConfig = MixedPrecisionConfig(), filter_fn: Callable[[str, nn.Parameter], bool] | None = None):
     """Wrap every stack of experts' weights under `module` -- a floating 3-D nn.Parameter (E, N, K) outside convolutions -- in a
     MixedPrecisionLinearWeight (in place).  The module has to multiply with `F.grouped_mm(x, weight.transpose(-2, -1), offs=offs)`.
 
-    A parameter that several modules share, or one module under several names, stays one."""
+    Three dims are all that is looked at: where `module` holds other such parameters (a position embedding (1, L, D)), `filter_fn(name, parameter)` says which
+    are meant.  A parameter that several modules share, or one module under several names, stays one (and is meant if any of its names is)."""
     places: dict[int, list] = {}
-    for m in module.modules():
+    for prefix, m in module.named_modules():
         if isinstance(m, nn.modules.conv._ConvNd):
             continue
         for name, p in m.named_parameters(recurse=False, remove_duplicate=False):
             if p.ndim == 3 and p.is_floating_point() and not isinstance(p, MixedPrecisionLinearWeight):
-                places.setdefault(id(p), []).append((m, name, p))
+                places.setdefault(id(p), []).append((m, name, f"{prefix}.{name}" if prefix else name, p))
     for found in places.values():
-        p = found[0][2]
-        new = nn.Parameter(MixedPrecisionLinearWeight(p.detach(), config=config), requires_grad=p.requires_grad)
-        for m, name, _ in found:
-            setattr(m, name, new)
+        p = found[0][3]
+        if filter_fn is None or any(filter_fn(full, p) for _, _, full, _ in found):
+            new = nn.Parameter(MixedPrecisionLinearWeight(p.detach(), config=config), requires_grad=p.requires_grad)
+            for m, name, _, _ in found:
+                setattr(m, name, new)
     return module
 
 

@@ -283,3 +283,13 @@ def test_shared_stacks_stay_shared():
     assert sum(isinstance(p, MixedPrecisionLinearWeight) for p in m.parameters()) == 3
     again = convert_mixed_precision_experts(m)
     assert again.first.up is m.second.up and not isinstance(m.first.up._data, MixedPrecisionLinearWeight)
+
+
+def test_conversion_of_named_stacks_only():
+    """Three dims do not make a stack of experts: a position embedding (1, L, D) is one that the caller knows."""
+    m = Experts()
+    m.positions = nn.Parameter(torch.zeros(1, 5, 8))
+    m.inner = Experts()
+    convert_mixed_precision_experts(m, filter_fn=lambda name, p: "positions" not in name and name != "inner.down")
+    assert isinstance(m.up, MixedPrecisionLinearWeight) and isinstance(m.inner.up, MixedPrecisionLinearWeight)
+    assert not isinstance(m.positions, MixedPrecisionLinearWeight) and not isinstance(m.inner.down, MixedPrecisionLinearWeight)
