@@ -46,8 +46,9 @@ typedef enum gnk_status {
  *      entry points added; gnk_set_debug_flags removed from the shipped library; gnk_set_gemm_variant accepts 5, 6, -2 and -3; gnk_set_tile_rescale added.
  *   3: the products grouped by expert and their quantizer (gnk_grouped_scaled_mm_rows / _depth, gnk_quantize_int8_grouped).
  *   4: gnk_orthogonalize.   5: gnk_grouped_scaled_mm_depth_split_bytes.   6: gnk_orthogonalize_workspace_bytes_of.
- *   7: gnk_grouped_scaled_mm_rows refuses int8 sums of more than 131071 products; _depth wants _split_bytes for int8 over more than 130816 rows. */
-#define GNK_ABI_VERSION 7
+ *   7: gnk_grouped_scaled_mm_rows refuses int8 sums of more than 131071 products; _depth wants _split_bytes for int8 over more than 130816 rows.
+ *   8: gnk_orthogonalize_chains. */
+#define GNK_ABI_VERSION 8
 int gnk_abi_version(void);
 
 /* Message for the last non-zero status returned on this thread ("" if none). */
@@ -320,9 +321,13 @@ int gnk_quantize_int8_grouped(const void *x, int x_dtype, const int32_t *ends, i
  * intermediates may overflow to Inf).  A matrix that holds a NaN or Inf comes out as NaN; one of zeros as zeros.  rows, cols <= 2^20, batch < 2^16.
  * workspace: gnk_orthogonalize_workspace_bytes_of() bytes for results of that type (half as much for BF16 as for the others), or
  * gnk_orthogonalize_workspace_bytes(), enough for any; 16-byte aligned, need not be cleared.  Overlapping calls need one each.
+ * Large stacks run as two chains of products, half of the matrices each, the second one on a stream of the library's own (one per device) between events on
+ * `stream`; a stream that is being captured runs both.  Same results.  Calls from different streams share that second stream, so that such a call can wait for
+ * work that was submitted before it on another stream.  gnk_orthogonalize_chains(): 2 where a call outside a capture runs so, 1 otherwise, 0 for an empty one.
  */
 int64_t gnk_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
 int64_t gnk_orthogonalize_workspace_bytes_of(int out_dtype, int64_t batch, int64_t rows, int64_t cols);
+int gnk_orthogonalize_chains(int out_dtype, int64_t batch, int64_t rows, int64_t cols);
 int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
                       float eps, void *workspace, int64_t workspace_bytes, void *stream);
 

@@ -685,6 +685,20 @@ Choice choose_tile(int64_t ext_a, int64_t ext_b, int64_t K, bool sym, int64_t ba
     return c128;
 }
 
+// The tiles of a step's three products, chosen for the whole stack however it is split: the results do not depend on the split.  `two`: as two chains of half
+// the stack each, where that is worth the second stream: large products (below B m^2 n = 1e11 two short chains get in each other's way: 8 x 1024 x 4096 734 us
+// alone, 966 us as two) whose last rounds are partly empty.  8 x 2048 x 5632: 3.35 -> 2.89 ms, 2 x 4096 x 4096: 2.84 -> 2.36.
+struct Schedule { Choice gram, poly, next; bool two; };
+Schedule make_schedule(const Plan &pl, int64_t batch, int64_t rows, int64_t cols, bool pairs) {
+    Schedule s;
+    s.gram = choose_tile(pl.lo, pl.lo, rows <= cols ? pl.cp : pl.rp, true, batch, pairs);
+    s.poly = choose_tile(pl.lo, pl.lo, pl.lo, true, batch, pairs);
+    s.next = choose_tile(pl.rp, pl.cp, pl.lo, false, batch, pairs);
+    const double rounds = s.gram.rounds_us + s.poly.rounds_us + s.next.rounds_us, work = s.gram.work_us + s.poly.work_us + s.next.work_us;
+    s.two = batch > 1 && (double)batch * (double)pl.lo * (double)pl.rp * (double)pl.cp >= 1.0e11 && work <= 0.9 * rounds;
+    return s;
+}
+
 template <bool AK, bool BK, int EPI, bool SYM> int run_product(const Product &p, const Choice &c, hipStream_t st) {
     if (c.bm == 256) return launch<256, 1, AK, BK, EPI, SYM>(p, st);
     if (c.bm == 128) return c.kg == 2 ? launch<128, 2, AK, BK, EPI, SYM>(p, st) : launch<128, 1, AK, BK, EPI, SYM>(p, st);
@@ -766,6 +780,12 @@ extern "C" int64_t gnk_orthogonalize_workspace_bytes_of(int out_dtype, int64_t b
     return make_plan(batch, rows, cols, wants_pairs(out_dtype)).total;
 }
 
+extern "C" int gnk_orthogonalize_chains(int out_dtype, int64_t batch, int64_t rows, int64_t cols) {
+    if (batch <= 0 || rows <= 0 || cols <= 0) return 0;
+    const bool pairs = wants_pairs(out_dtype);
+    return make_schedule(make_plan(batch, rows, cols, pairs), batch, rows, cols, pairs).two ? 2 : 1;
+}
+
 extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_dtype, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
                                  float eps, void *workspace, int64_t workspace_bytes, void *stream) {
     const char *name = "orthogonalize";
@@ -799,9 +819,8 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
     while (sq * cmax >= 16384.0f) sq *= 0.5f;
     const bool with_mu = !pairs && (wide ? rows : cols) < MU_ROWS;
     const int64_t lo = pl.lo, ldx = 2 * pl.cp, lds = 2 * lo;
-    // chosen for the whole stack, however it is split below: the results do not depend on the split
-    const Choice c_gram = choose_tile(lo, lo, wide ? pl.cp : pl.rp, true, batch, pairs), c_poly = choose_tile(lo, lo, lo, true, batch, pairs);
-    const Choice c_next = choose_tile(pl.rp, pl.cp, lo, false, batch, pairs);
+    const Schedule plan = make_schedule(pl, batch, rows, cols, pairs);
+    const Choice c_gram = plan.gram, c_poly = plan.poly, c_next = plan.next;
     // one step of matrices b0 .. b0 + n - 1 on stream s
     auto one_step = [&](int it, int64_t b0, int64_t n, hipStream_t s) -> int {
         const bool last = it + 1 == steps;
@@ -854,11 +873,8 @@ extern "C" int gnk_orthogonalize(const void *G, int g_dtype, void *out, int out_
         if (with_mu) return wide ? run_product<true, false, UPDATE, false>(p, c_next, s) : run_product<true, true, UPDATE, false>(p, c_next, s);
         return wide ? run_product<true, false, GRAM, false>(p, c_next, s) : run_product<true, true, GRAM, false>(p, c_next, s);
     };
-    // Two chains of half the stack each where that is worth the second stream: large products (below B m^2 n = 1e11 two short chains get in each other's way:
-    // 8 x 1024 x 4096 734 us alone, 966 us as two) whose last rounds are partly empty.  8 x 2048 x 5632: 3.35 -> 2.89 ms, 2 x 4096 x 4096: 2.84 -> 2.36.
-    const double rounds = c_gram.rounds_us + c_poly.rounds_us + c_next.rounds_us, work = c_gram.work_us + c_poly.work_us + c_next.work_us;
     SideStream side;
-    const bool two = batch > 1 && (double)batch * (double)lo * (double)pl.rp * (double)pl.cp >= 1.0e11 && work <= 0.9 * rounds && side.fork(st);
+    const bool two = plan.two && side.fork(st);
     const int64_t half = two ? batch / 2 : batch;
     for (int it = 0; it < steps && !rc; ++it) {
         rc = one_step(it, 0, half, st);

@@ -11,7 +11,7 @@ import torch
 
 # GNK_LIBRARY: tuning only (an A/B build of the same sources, e.g. `make ABLATE=1 OUT=...`); the shipped library is the default
 _LIB_PATH = Path(os.environ.get("GNK_LIBRARY") or Path(__file__).resolve().parent / "libgnk_hip.so")
-ABI_VERSION = 7   # include/gnk.h GNK_ABI_VERSION
+ABI_VERSION = 8   # include/gnk.h GNK_ABI_VERSION
 
 BF16, F16, F32, I8, E4M3, E5M2, I32 = range(7)
 DTYPE_CODE = {
@@ -122,6 +122,7 @@ def load() -> ctypes.CDLL:
     L.gnk_orthogonalize_workspace_bytes.restype = i64
     L.gnk_orthogonalize_workspace_bytes_of.argtypes = [ci] + [i64] * 3
     L.gnk_orthogonalize_workspace_bytes_of.restype = i64
+    L.gnk_orthogonalize_chains.argtypes = [ci] + [i64] * 3
     L.gnk_orthogonalize.argtypes = [vp, ci, vp, ci, i64, i64, i64, ci, f32, f32, f32, f32, vp, i64, vp]
     if L.gnk_abi_version() != ABI_VERSION:
         raise RuntimeError(f"libgnk_hip.so ABI {L.gnk_abi_version()} != expected {ABI_VERSION}; rebuild it")
