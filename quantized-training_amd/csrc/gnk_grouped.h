@@ -278,7 +278,7 @@ __device__ __forceinline__ void zero_tile(char *C, int64_t rows, int64_t N, int6
 // ------------------------------------------------------------------------------ two-buffer kernel (any K, any group size)
 // The loop of gemm_kernel (row / column epilogue) on one group's tile.  128 x 128 over four waves: 64 KiB of LDS and at most 256
 // registers, two workgroups per CU.  Bound by a tile's fixed cost (~6 us: first loads, epilogue) beside 1 us per 128 k, and by whole rounds of tiles:
-// 4099 rows over 16 experts, 1024 -> 4096, e4m3: 30-32 us, 3.4 TB/s of its 105 MB (21 us at a copy's rate), 1.1 PFLOP/s.
+// 4099 rows over 16 experts, 1024 -> 4096, e4m3: 30-33 us, 3.3 TB/s of its 105 MB (21 us at a copy's rate), 1.1 PFLOP/s.
 template <class Cfg, bool DEPTH>
 __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cfg::NT == 256 ? 2 : 1))) two_buffer_kernel(const GroupedParams gp) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(Cfg::NT) __attribute__((amdgpu_waves_per_eu(Cf
 // flight.  Three 128-k stages of 16 KiB are, behind the one being read (2 workgroups per CU: ~50 KiB of weights in flight per CU), one barrier per
 // stage.  Stage t lands before the barrier of step t (vmcnt leaves the pieces of t + 1 and t + 2 in flight); the buffer of stage t - 1, which every
 // wave has read by then, takes stage t + 3 behind it.  Towards the end nothing is left to issue and the wait is for everything.
-// 16 rows over 8 experts, 1024 -> 4096, int8: 8.4 us a call for 30 MB of weights, 3.5 TB/s (5.9 us at a copy's rate; the rest is the launch and the
+// 16 rows over 8 experts, 1024 -> 4096, int8: 7.9-8.4 us a call for 30 MB of weights, 3.5 TB/s (5.9 us at a copy's rate; the rest is the launch and the
 // first loads); depth form, 1021 rows over 8 experts to 512 x 256: 5 us.
 // KG = 2 (at most one workgroup per CU): a second set of four waves with a ring of its own takes every other step; the two halves are added in LDS.
 // 16 rows over 4 experts, 4096 -> 1024: 17.7 -> 11.6 us with B K-major, 23.2 -> 18.2 N-major (rows of 64 bytes are half lines); 5632 -> 2048, one row: 18.2 -> 15.0.
@@ -464,8 +464,8 @@ __device__ __forceinline__ void finish_half_192(const GemmParams &p, char *smem,
 // runs over ceil(T_e / 256) * 256 of them (a group without rows: once over zeros).  Host-checked: T * pitch < 2^32 (the descriptors' sizes).
 // BM = 192 (rows, int8): the same loop with three quarters of the rows, for tile counts that leave the last round of 256-row tiles nearly empty.
 // Bound by the matrix cores and ~12 us per tile in which they stand still (first loads, epilogue; one workgroup per CU leaves nothing to run meanwhile):
-// int8 over 8 experts, rows form 32768 x 2048 -> 5632 (twelve rounds of 16 steps): 350-357 us, 2.15 POP/s, matrix pipes 57 % busy; depth form 5632 x 2048
-// over the same rows (three rounds of 32 steps): 307-314 us, 2.45 POP/s, 69 %.  192: 16384 x 4096 -> 1024 over 32 experts in two rounds: 86 us, 1.6 POP/s.
+// int8 over 8 experts, rows form 32768 x 2048 -> 5632 (twelve rounds of 16 steps): 350-370 us, 2.1 POP/s, matrix pipes 57 % busy; depth form 5632 x 2048
+// over the same rows (three rounds of 32 steps): 301-328 us, 2.4 POP/s, 69 %; e4m3 298-313.  192: 16384 x 4096 -> 1024 over 32 experts in two rounds: 86-88 us, 1.6 POP/s.
 template <class Cfg, bool DEPTH, int BM = 256>
 __global__ void __launch_bounds__(256) w4_kernel(const GroupedParams gp) {
     extern __shared__ __attribute__((aligned(16))) char smem[];

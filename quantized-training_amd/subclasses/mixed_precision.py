@@ -346,8 +346,10 @@ class _Int8MixedPrecisionLinear(torch.autograd.Function):
 
 # ---------------------------------------------------------------------------------------------------------------------
 # A stack of experts' weights: `F.grouped_mm(x, weight.transpose(-2, -1), offs=offs)` on a MixedPrecisionLinearWeight (E, N, K).  No
-# counterpart in the reference (its models are dense); the arithmetic per expert is that of the Linear above.  Rows are sorted by expert
-# and `offs` stays on the device, so every operand is quantized along its contraction by one kernel over all groups:
+# counterpart in the reference (its models are dense); the arithmetic per expert is that of the Linear above but for one rounding: the grouped quantizer
+# (w of dX, both operands of dW) multiplies the column maximum by fl(1/127) where `quantize_int8` divides by 127, scales 1.5 fp32 steps apart at most, so that a
+# value next to a tie may be quantized one step off the dense Linear's.  A sum has at most 131071 terms in the forward (K) and in dX (N; more are refused), any
+# number in dW.  Rows are sorted by expert and `offs` stays on the device, so every operand is quantized along its contraction by one kernel over all groups:
 #   forward   x per row, w per (e, n)            rows form, (T, K) x (E, K, N)
 #   dX        dY per row, w per (e, k)           rows form, (T, N) x (E, N, K); the columns of one expert are a "group" of N rows
 #   dW        dY and x per (group, column)       the contraction runs over each group's rows, (N, T) x (T, K) -> (E, N, K)

@@ -293,3 +293,16 @@ def test_conversion_of_named_stacks_only():
     convert_mixed_precision_experts(m, filter_fn=lambda name, p: "positions" not in name and name != "inner.down")
     assert isinstance(m.up, MixedPrecisionLinearWeight) and isinstance(m.inner.up, MixedPrecisionLinearWeight)
     assert not isinstance(m.positions, MixedPrecisionLinearWeight) and not isinstance(m.inner.down, MixedPrecisionLinearWeight)
+
+
+def test_a_slice_of_the_experts_reaches_the_operator(cpu_ops):
+    """As a rank that holds some of the experts takes them; the gradient of the others is zero."""
+    g = torch.Generator().manual_seed(8)
+    x, w = torch.randn(5, 8, generator=g, dtype=torch.float64), torch.randn(4, 12, 8, generator=g, dtype=torch.float64)
+    wp = nn.Parameter(MixedPrecisionLinearWeight(w, MixedPrecisionConfig()))
+    y = F.grouped_mm(x, wp[1:3].transpose(-2, -1), offs=torch.tensor([2, 5], dtype=torch.int32))
+    torch.testing.assert_close(y.detach(), torch.cat([x[:2] @ w[1].T, x[2:] @ w[2].T]), rtol=1e-12, atol=1e-12)
+    y.sum().backward()
+    gw = getattr(wp.grad, "_data", wp.grad)
+    assert gw.shape == w.shape and (gw[0] == 0).all() and (gw[3] == 0).all()
+    torch.testing.assert_close(gw[1], x[:2].sum(0).expand(12, 8), rtol=1e-12, atol=1e-12)
