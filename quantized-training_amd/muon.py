@@ -90,17 +90,17 @@ class Muon(torch.optim.Optimizer):
                 state["momentum"].mul_(group["momentum"]).add_(g)
                 # what is orthogonalised (u) has the gradient's type; fp16 does not hold the sum
                 dtype = torch.float32 if g.dtype is torch.float16 else g.dtype
-                alike.setdefault((tuple(p.shape[-2:]), dtype, g.device), []).append([t if t.ndim == 3 else t[None] for t in (_plain(p), g, state["momentum"])])
+                alike.setdefault((tuple(p.shape[-2:]), dtype, g.device), []).append((_plain(p), *(t if t.ndim == 3 else t[None] for t in (g, state["momentum"]))))
             for ((rows, cols), dtype, _), weights in alike.items():
-                counts = [w.shape[0] for w, _, _ in weights]
+                counts = [g.shape[0] for _, g, _ in weights]
                 for call in _calls(counts, matrices_per_call(rows, cols, sum(counts))):
                     u = [(torch.add(g[a:b], m[a:b], alpha=group["momentum"]) if group["nesterov"] else m[a:b]).to(dtype) for i, a, b in call for _, g, m in (weights[i],)]
                     out = orthogonalize(u[0] if len(u) == 1 else torch.cat(u), steps=group["steps"], coefficients=group["coefficients"], eps=group["eps"])
                     at, scale = 0, -group["lr"] * max(1.0, rows / cols) ** 0.5
                     for i, a, b in call:
-                        w = weights[i][0][a:b]
+                        w = weights[i][0] if b - a == counts[i] else weights[i][0][a:b]       # whole where it can be: not every weight class has views
                         if group["weight_decay"]:
                             w.mul_(1 - group["lr"] * group["weight_decay"])
-                        w.add_(out[at:at + b - a], alpha=scale)
+                        w.add_(out[at:at + b - a].view(w.shape), alpha=scale)
                         at += b - a
         return loss

@@ -220,3 +220,23 @@ def test_bounded_calls_on_the_device(monkeypatch):
         results.append([p.detach().double() for p in ps])
     for a, b in zip(*results):
         assert (a - b).norm() <= 2 * (2e-3 + 2 * 2.0 ** -8) * b.norm() and b.norm() > 0
+
+
+@pytest.mark.parametrize("kind", ["int8", "bitnet", "mixed_precision"])
+def test_quantized_weights_are_updated(cpu_op, kind):
+    """Every weight class whose in-place arithmetic an optimizer uses: the step moves it by lr u (u: singular values near 1), however it stores itself."""
+    from subclasses import convert_bitnet, convert_int8_quantized_training, convert_mixed_precision
+
+    torch.manual_seed(0)
+    m = nn.Sequential(nn.Linear(8, 16, bias=False).bfloat16())
+    {"int8": convert_int8_quantized_training, "bitnet": convert_bitnet, "mixed_precision": convert_mixed_precision}[kind](m)
+    p = m[0].weight
+    values = lambda: (p.dequantize() if kind == "int8" else p._data).double()  # noqa: E731
+    before, p.grad = values(), torch.randn(16, 8).bfloat16()
+    u = newton_schulz(p.grad.double() * 1.95, 5, 3.4445, -4.7750, 2.0315, 1e-7)
+    Muon([p], lr=0.5).step()
+    step = values() - before
+    # sqrt(2) lr u; bf16's roundings (u, the weight) and, for int8, a step of the row's scale (amax / 127) on either side
+    want = -0.5 * 2 ** 0.5 * u
+    tol = 2.0 ** -7 + (2 * (values().abs().amax() + before.abs().amax()) / 127 if kind == "int8" else 0.0)
+    assert type(p).__name__ != "Parameter" and ((step - want).abs() <= tol).all()
